@@ -16,6 +16,7 @@ _PKG = Path(__file__).resolve().parent
 LIBRARY = _PKG.parent / "lib" / "libgcq.so"
 HEADERS = [_PKG.parents[1] / "include" / h for h in ("gcq.h", "ggml_compiler_rt.h", "ggml.h", "ggml-backend.h",
                                                      "ggml-alloc.h")]
+PAGED_HEADER = _PKG.parents[1] / "include" / "gcq_paged.h"
 
 
 class GcqError(RuntimeError):
@@ -46,6 +47,18 @@ class Stats(ctypes.Structure):
 class Builder(ctypes.Structure):
     """ggml_compiler_builder (include/ggml_compiler_rt.h)."""
     _fields_ = [("stage", ctypes.c_char_p), ("build", ctypes.c_void_p)]
+
+
+class PagedCache(ctypes.Structure):
+    """gcq_paged_cache (include/gcq_paged.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("n_head_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class PagedBatch(ctypes.Structure):
+    """gcq_paged_batch (include/gcq_paged.h)."""
+    _fields_ = [("pages", ctypes.c_void_p), ("ld_pages", ctypes.c_int64), ("starts", ctypes.c_void_p),
+                ("past", ctypes.c_void_p), ("n_seq", ctypes.c_int32), ("max_pages", ctypes.c_int32)]
 
 
 def library_path() -> Path:
@@ -98,6 +111,12 @@ SIGNATURES = {
     "gcq_fill_normal": ([p, i64, u64, u64, f32, p], i32),
     "gcq_stream_read": ([p, sz, i32, i32, p, p], i32),
     "gcq_fill_ids": ([p, i64, u64, u64, ctypes.c_int32, p], i32),
+    # gcq_paged.h
+    "gcq_paged_cache_size": ([i32, i32, i32, i32], sz),
+    "gcq_paged_append": ([p, p, i64, p, i64, i64, p, i64, i64, p, i64, i64, i32, p, p, i32, f32, p], i32),
+    "gcq_paged_read": ([p, p, i64, p, p, p], i32),
+    "gcq_paged_attn_workspace": ([p, p, i64, i32, i64], sz),
+    "gcq_paged_attn": ([p, p, i64, p, i64, i64, i32, i64, i32, f32, p, p, sz, p], i32),
     "gcq_llama_create": ([p, i32], p),
     "gcq_llama_free": ([p], None),
     "gcq_llama_init_random": ([p, u64, f32], i32),

@@ -8,10 +8,11 @@ stands for and its reference call site are named per function.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
+from . import _lib
 from ._lib import GcqError, check, load
 
 F32, F16, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, Q8_K = 0, 1, 2, 8, 12, 13, 14, 15
@@ -236,6 +237,166 @@ def flash_attn_ext(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torc
                                     v.stride(0), v.stride(1), _p(mask), 0 if mask is None else mask.stride(0),
                                     _p(out), Dk, v.shape[2], Sq, H, Hkv, n_kv, float(scale), _p(ws), ws.numel(),
                                     _stream()))
+    return out
+
+
+# ------------------------------------------------------------------ paged 4-bit key / value cache
+
+
+@dataclass
+class PagedCache:
+    """One layer's keys and values in n_pages pages of page_size tokens, held as Q4_0 blocks (include/gcq_paged.h).
+    page_size 32, 64, 128 or 256; head dim D 64, 128 or 256."""
+
+    n_pages: int
+    page_size: int
+    Hkv: int
+    D: int
+    data: torch.Tensor  # uint8, gcq_paged_cache_size bytes
+    _c: _lib.PagedCache = field(init=False, repr=False, compare=False)
+
+    def __post_init__(self) -> None:
+        n = int(load().gcq_paged_cache_size(self.n_pages, self.page_size, self.Hkv, self.D))
+        if n == 0:
+            raise _lib.error()
+        _cuda(self.data, torch.uint8, "data")
+        if self.data.numel() != n or not self.data.is_contiguous():
+            raise ValueError(f"data must be {n} contiguous bytes, got {self.data.numel()}")
+        self._c = _lib.PagedCache(self.data.data_ptr(), self.n_pages, self.page_size, self.Hkv, self.D)
+        self._at = ctypes.addressof(self._c)
+
+    @classmethod
+    def new(cls, n_pages: int, page_size: int, Hkv: int, D: int, device=None) -> "PagedCache":
+        n = int(load().gcq_paged_cache_size(n_pages, page_size, Hkv, D))
+        if n == 0:
+            raise _lib.error()
+        return cls(n_pages, page_size, Hkv, D, torch.zeros(n, dtype=torch.uint8, device=device or "cuda"))
+
+
+@dataclass
+class PagedBatch:
+    """Sequences and their new rows, packed: sequence s owns rows starts[s] .. starts[s + 1] - 1, the first of them at
+    position past[s]; position p lives in page pages[s, p // page_size]. int32 on the device: pages [S, max_pages] (an
+    entry outside the pool: no such tokens), starts [S + 1], past [S]. The kernels read them, so a captured graph
+    follows their contents."""
+
+    pages: torch.Tensor
+    starts: torch.Tensor
+    past: torch.Tensor
+    _c: _lib.PagedBatch = field(init=False, repr=False, compare=False)
+
+    def __post_init__(self) -> None:
+        for name in ("pages", "starts", "past"):
+            _cuda(getattr(self, name), torch.int32, name)
+        if self.pages.dim() != 2 or self.pages.stride(1) != 1:
+            raise ValueError("pages must be [sequences, pages] with contiguous rows")
+        S, n = self.pages.shape
+        if self.starts.shape != (S + 1,) or self.past.shape != (S,):
+            raise ValueError(f"{S} sequences need starts [{S + 1}] and past [{S}], got {tuple(self.starts.shape)} and "
+                             f"{tuple(self.past.shape)}")
+        if not self.starts.is_contiguous() or not self.past.is_contiguous():
+            raise ValueError("starts and past must be contiguous")
+        self._c = _lib.PagedBatch(self.pages.data_ptr(), max(self.pages.stride(0), n), self.starts.data_ptr(),
+                                  self.past.data_ptr(), S, n)
+        self._at = ctypes.addressof(self._c)
+
+
+def _paged(cache: PagedCache, batch: PagedBatch, *rest: torch.Tensor) -> None:
+    """All on the current device, whose current stream takes the launch."""
+    d = torch.cuda.current_device()
+    for t in (cache.data, batch.pages, batch.starts, batch.past, *rest):
+        if t.get_device() != d:
+            raise ValueError(f"a tensor on {t.device}, the current device is {d}")
+
+
+def _paged_rows(x: torch.Tensor, dtype: torch.dtype, name: str, n: int, heads: int, D: int) -> torch.Tensor:
+    _cuda(x, dtype, name)
+    if x.dim() != 3 or x.shape[0] != n or x.shape[1] != heads or x.shape[2] != D:
+        raise ValueError(f"{name} must be [{n}, {heads}, {D}], got {tuple(x.shape)}")
+    if x.stride(2) != 1:
+        raise ValueError(f"{name} needs a unit stride along the head dim")
+    return x
+
+
+def _paged_out(out: torch.Tensor | None, shape, dtype: torch.dtype, device, name: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _cuda(out, dtype, name)
+    if tuple(out.shape) != tuple(shape) or not out.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {tuple(shape)}, got {tuple(out.shape)}")
+    return out
+
+
+def rope_freqs(n_dims: int, base: float, freq_scale: float = 1.0, ff: torch.Tensor | None = None,
+               device=None) -> torch.Tensor:
+    """paged_append's table: freq_scale base^(-2 i / n_dims) / ff[i] for i < n_dims / 2, rounded to f32 once."""
+    i = torch.arange(n_dims // 2, dtype=torch.float64)
+    f = freq_scale * float(base) ** (-2.0 * i / n_dims)
+    if ff is not None:
+        f = f / ff.detach().to("cpu", torch.float64)
+    return f.to(torch.float32).to(device or "cuda")
+
+
+def paged_append(cache: PagedCache, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
+                 freqs: torch.Tensor | None = None, attn_factor: float = 1.0,
+                 q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Rows k, v f32 [n, Hkv, D] (strided allowed, unit inner stride) into the cache as Q4_0, the keys' NEOX pairs
+    (i, i + len(freqs)) turned by position * freqs[i] (freqs None: unrotated). q f32 [n, H, D]: turned alike and
+    returned as f16 [n, H, D], paged_attn's input (q_out: into it; rows of no sequence stay as they are)."""
+    n, Hkv, D = k.shape[0], cache.Hkv, cache.D
+    _paged_rows(k, torch.float32, "k", n, Hkv, D)
+    _paged_rows(v, torch.float32, "v", n, Hkv, D)
+    rest, H = [k, v], 0
+    if q is not None:
+        H = q.shape[1] if q.dim() == 3 else 0
+        _paged_rows(q, torch.float32, "q", n, H, D)
+        q_out = _paged_out(q_out, (n, H, D), torch.float16, q.device, "q_out")
+        rest += [q, q_out]
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if freqs is not None:
+        _cuda(freqs, torch.float32, "freqs")
+        if freqs.dim() != 1 or not freqs.is_contiguous():
+            raise ValueError("freqs must be contiguous, one value for each pair")
+        rest.append(freqs)
+    _paged(cache, batch, *rest)
+    sq = (0, 0) if q is None else q.stride()
+    check(load().gcq_paged_append(cache._at, batch._at, n, _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
+                                  v.stride(1), _p(q), sq[0], sq[1], H, _p(q_out), _p(freqs),
+                                  0 if freqs is None else 2 * freqs.numel(), float(attn_factor), _stream()))
+    return q_out
+
+
+def paged_read(cache: PagedCache, batch: PagedBatch, n: int, k: torch.Tensor | None = None,
+               v: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """What the cache holds for the batch's n rows: k, v f32 [n, Hkv, D] (zeros for tokens that are not there; into
+    k, v if given; rows of no sequence stay as they are)."""
+    shape = (n, cache.Hkv, cache.D)
+    k = _paged_out(k, shape, torch.float32, cache.data.device, "k")
+    v = _paged_out(v, shape, torch.float32, cache.data.device, "v")
+    _paged(cache, batch, k, v)
+    check(load().gcq_paged_read(cache._at, batch._at, n, _p(k), _p(v), _stream()))
+    return k, v
+
+
+def paged_attn(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, scale: float, max_rows: int | None = None,
+               window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of the batch's rows over their sequences' cached tokens (their own appended before), the last
+    `window` of them if window > 0. q f16 [n, H, D] (strides multiples of 8, unit inner stride) -> f32 [n, H, D] (into
+    out if given; rows of no sequence stay as they are; a row that sees no token gives zeros). max_rows: no sequence
+    has more rows than this (default n); 1 for a decode step."""
+    n, H = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+    _paged_rows(q, torch.float16, "q", n, H, cache.D)
+    out = _paged_out(out, (n, H, cache.D), torch.float32, q.device, "out")
+    _paged(cache, batch, q, out)
+    max_rows = max(n, 1) if max_rows is None else int(max_rows)
+    lib = load()
+    ws_n = int(lib.gcq_paged_attn_workspace(cache._at, batch._at, n, H, max_rows))
+    if ws_n == 0:
+        raise _lib.error()
+    ws = workspace(ws_n, q.device)
+    check(lib.gcq_paged_attn(cache._at, batch._at, n, _p(q), q.stride(0), q.stride(1), H, max_rows, int(window),
+                             float(scale), _p(out), _p(ws), ws.numel(), _stream()))
     return out
 
 
