@@ -15,7 +15,7 @@
 namespace gcq {
 
 constexpr int kPagedTile = 32;
-constexpr float kPagedMax = 524032.0f;  // 8 * 65504: the largest value a block's f16 scale reaches
+constexpr float kPagedMax = 65504.0f;  // the largest f16: every value d (c - 8) is within it
 
 struct Paged {
     uint8_t * data;

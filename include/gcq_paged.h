@@ -53,8 +53,8 @@ GCQ_API size_t gcq_paged_cache_size(int n_pages, int page_size, int n_head_kv, i
  * position * freqs[i] radians and scaled by attn_factor (ggml_rope_ext's NEOX pairs; freqs[i] =
  * freq_scale base^(-2 i / n_dims) / ff[i]); dims n_dims .. D - 1 pass through. Angle, sine and cosine
  * are taken in 64 bits and a rotated value is rounded once, to 32, whatever the position (gcq_rope_neox
- * keeps ggml's 32-bit angles). Blocks are then encoded as gcq_quantize encodes Q4_0, with two
- * exceptions that keep every scale finite: values beyond +-524032 (what a block can hold) are taken as that, NaNs as 0.
+ * keeps ggml's 32-bit angles). Blocks are then encoded as gcq_quantize encodes Q4_0, but for values beyond +-65504
+ * (f16's largest), which are taken as that, and NaNs, which are taken as 0: all that the cache holds is finite.
  * q (or NULL) [r][h][d] f32 at (q_r, q_h), n_head heads: rotated alike into q_out [n_rows][n_head][D] f16, what
  * gcq_paged_attn takes. */
 GCQ_API int gcq_paged_append(const gcq_paged_cache * cache, const gcq_paged_batch * batch, int64_t n_rows,

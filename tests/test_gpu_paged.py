@@ -238,7 +238,7 @@ def test_append_special_values(gops, orc):
     x[1, 0, 3], x[1, 0, 9], x[1, 0, 40], x[1, 0, 41] = 2.0, -2.0, -3.0, 3.0
     x[2] = np.random.default_rng(1).standard_normal((1, D)) * 1e-6
     x[3] = np.random.default_rng(2).standard_normal((1, D)) * 1e-42
-    x[4, 0, :8] = [1e9, -3e38, 1.0, 524032.0, 524033.0, -7e5, 2.0, 1e5]
+    x[4, 0, :8] = [1e9, -3e38, 1.0, 65504.0, 65505.0, -7e5, 2.0, 6e4]
     x[5, 0, 5], x[5, 0, 6], x[5, 0, 33] = np.inf, 4.0, -np.inf
     x[6, 0, :40] = 1.0
     x[6, 0, 7], x[6, 0, 20] = np.nan, -2.0
@@ -247,7 +247,7 @@ def test_append_special_values(gops, orc):
     t = torch.from_numpy(x).cuda()
     gops.paged_append(c.cache, c.batch(), t, t)
     k, v = gops.paged_read(c.cache, c.batch(), 8)
-    clean = np.clip(np.nan_to_num(x, nan=0.0, posinf=524032.0, neginf=-524032.0), -524032.0, 524032.0)
+    clean = np.clip(np.nan_to_num(x, nan=0.0, posinf=65504.0, neginf=-65504.0), -65504.0, 65504.0)
     want = q4_values(orc, clean)
     assert np.isfinite(want).all()
     for y in (k, v):
@@ -316,7 +316,7 @@ def test_attention_scales(gops, scale, rows, past):
 
 
 def test_attention_large_scores(gops):
-    """Scores in the thousands: one key takes all the weight; and cached values of 2^14 and more."""
+    """Scores in the thousands: one key takes all the weight; and cached values up to f16's largest."""
     c = Case(gops, [1, 70], [300, 10], 1, 128, 64, seed=15)
     run_attn(gops, c, 4, scale=5.0, q_scale=30.0)
     c = Case(gops, [1, 70], [300, 10], 1, 64, 64, seed=16)
