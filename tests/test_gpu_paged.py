@@ -330,6 +330,26 @@ def test_attention_large_scores(gops):
     check_attn(c, got, want, bound, 301)
 
 
+def test_attention_huge_scores(gops):
+    """Scores past 2^24, where f32 holds no fraction: the largest key takes all the weight unless another's score rounds to
+    the same; NaN-free, and each output a mean of cached values of near-largest scores (within 2^-22 of them)."""
+    c = Case(gops, [1, 70], [300, 10], 1, 128, 64, seed=26)
+    c.fill_past()
+    q = (torch.randn((c.n, 4, 128), device="cuda") * 3000).half()
+    got = gops.paged_attn(c.cache, c.batch(), q, 2000.0).double()
+    want, _ = attn_reference(c, q, 2000.0)
+    for s in range(2):
+        k, v = c.k[c.key0[s]:c.key0[s + 1], 0], c.v[c.key0[s]:c.key0[s + 1], 0]
+        for r in range(c.rows[s]):
+            for h in range(4):
+                x = k[:c.past[s] + r + 1] @ q[c.starts[s] + r, h].double() * 2000.0
+                near = x >= x.max() - x.abs().max() * 2.0 ** -20
+                lo, hi = v[:len(x)][near].amin(0), v[:len(x)][near].amax(0)
+                o = got[c.starts[s] + r, h]
+                assert x.max() > 2.0 ** 24 or r < 4
+                assert ((o >= lo - 1e-5) & (o <= hi + 1e-5)).all()
+
+
 def test_attention_tiny_values(gops):
     """Cached values whose scales are f16 subnormals keep their bits."""
     c = Case(gops, [2, 64], [90, 0], 1, 128, 32, seed=17)
