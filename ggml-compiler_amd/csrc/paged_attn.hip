@@ -1,6 +1,6 @@
 // paged_attn.hip - attention over the paged 4-bit cache (include/gcq_paged.h; layout in paged.h).
 //
-// k_paged_few: a wavefront takes 16 rows, a row being a (query, head) pair of one KV head (row j G + g), and tiles of 32
+// k_paged_attn: a wavefront takes 16 rows, a row being a (query, head) pair of one KV head (row j G + g), and tiles of 32
 // keys, straight from memory into the matrix cores' operands:
 //   - scores S^T[key][row] = K Q^T, one v_mfma_f32_16x16x32_f16 per Q4_0 block of 32 dims and 16 keys, on the codes c - 8
 //     themselves (exact in f16); a block's sum is scaled by its d in f32.
@@ -29,7 +29,6 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
-typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr int kMinChunk = 16;    // tiles: a shorter split costs more in the merge than it saves
 constexpr float kSlack = 4.0f;   // how far a score's exponent may pass R
@@ -87,6 +86,7 @@ struct Plan {
     const AttnArgs & a;
     SeqWork w;  // of sequence s0 + lane
     int chunk, s, base, lane_at;
+    int64_t first_item;
 
     __device__ __forceinline__ Plan(const AttnArgs & args) : a(args) {
         const int lane = threadIdx.x & 63;
@@ -111,6 +111,27 @@ struct Plan {
         base = __builtin_amdgcn_readfirstlane(base);
         s = __builtin_amdgcn_readfirstlane(s);
         return {pick(w.r0), pick(w.rows), pick(w.tile0), pick(w.tiles), pick(w.rts), pick(w.past)};
+    }
+    // To the sequence of row tile `id` (counted as the items are, but for the splits); base: its first, first_item: its first item.
+    __device__ __forceinline__ bool find_tile(int id) {
+        const int lane = threadIdx.x & 63;
+        base = 0;
+        first_item = 0;
+        for (int s0 = 0; s0 < a.p.n_seq; s0 += 64) {
+            if (s0) w = seq_work<ROWS>(a, s0 + lane);
+            const int n = w.rts * a.p.Hkv, sum = wave_scan(n), m = items(w), isum = wave_scan(m);
+            const uint64_t at = __ballot(base + sum > id);
+            if (at) {
+                lane_at = __builtin_ctzll(at);
+                base += __builtin_amdgcn_readlane(sum - n, lane_at);
+                first_item += __builtin_amdgcn_readlane(isum - m, lane_at);
+                s = s0 + lane_at;
+                return true;
+            }
+            base += __builtin_amdgcn_readlane(sum, 63);
+            first_item += __builtin_amdgcn_readlane(isum, 63);
+        }
+        return false;
     }
     // To the sequence that `found` (a ballot over the sequences s0 .. s0 + 63, their inclusive item sums given) picks
     // first.
@@ -179,12 +200,9 @@ __device__ __forceinline__ void lds_load(const uint8_t * base, uint32_t voff, ui
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" ::"v"(voff), "s"(base), "s"(lds), "n"(OFF) : "memory");
 }
 template <int D>
-__device__ __forceinline__ void tile_load(const uint8_t * data, int64_t off, uint32_t lds, int lane) {
-    const uint64_t p = (uint64_t) (uintptr_t) (data + off);
-    const uint8_t * t = (const uint8_t *) (uintptr_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((int) (p >> 32)) << 32 |
-                                                       (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) p));
-    lds = __builtin_amdgcn_readfirstlane(lds);
+__device__ __forceinline__ void tile_load(const uint8_t * t, uint32_t lds, int lane) {  // (t, lds: uniform)
     constexpr int full = 36 * D / 1024, rest = (36 * D % 1024) / 16;
+    lds = __builtin_amdgcn_readfirstlane(lds);
 #pragma unroll
     for (int i = 0; i < full; i += 3) {
         const uint32_t v = 16 * lane + 1024 * i;
@@ -197,13 +215,13 @@ __device__ __forceinline__ void tile_load(const uint8_t * data, int64_t off, uin
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-template <int D> constexpr int kRing = D == 64 ? 4 : 2;  // tiles in LDS per wavefront
-// Wavefronts per SIMD that the registers hold.
-template <int D, int RT> constexpr int kPerSimd = D * RT <= 128 ? 4 : D * RT <= 256 ? 2 : 1;
+// Wavefronts per SIMD that the registers (and, heads of 256, LDS) hold; and of a workgroup.
+constexpr int per_simd(int D, int RT) { return D * RT <= 128 ? 4 : D * RT == 256 && RT == 2 ? 3 : 2; }
+constexpr int waves(int D, int rows) { return D == 256 && rows == 32 ? 8 : 4; }
 
 template <int D, int RT, int NW>
-__global__ __launch_bounds__(64 * NW, (kPerSimd<D, RT>)) void k_paged_few(const AttnArgs a) {
-    constexpr int ROWS = 16 * RT, NB = D / 32, NT = D / 16, RING = kRing<D>, NL = kTileLoads<D>, P = D + 4;
+__global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const AttnArgs a) {
+    constexpr int ROWS = 16 * RT, NB = D / 32, NT = D / 16, RING = 2, NL = kTileLoads<D>, P = D + 4;
     // LDS: the wavefronts' rings (then their sums of 16 rows), and the row tile's Q as MFMA operands (from two times 16
     // rows on; registers hold 16)
     constexpr int kRings = NW * RING * 36 * D, kSums = NW * 16 * (P * 4 + 8), kQ = RT > 1 ? ROWS * D * 2 : 0;
@@ -224,13 +242,24 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<D, RT>)) void k_paged_few(const 
     const int last = min(sw.tile0 + min(sw.tiles, (split + 1) * plan.chunk), (int) ((min(pos1 + 1, cap) + 31) >> 5));
     const int e0 = a.window ? (int) ((pos1 - a.window) >> 5) + 1 : 0, e1 = (int) ((pos0 + 1) >> 5);
 
-    // the tiles of this wavefront: first + wave, + NW, ..; their page entries lie in the lanes, 64 at a time
+    // The tiles of this wavefront: first + wave, + NW, ..; lane i holds the address of tile k0 + i, 0 for one that is not there.
     const int n = first + wave < last ? (last - first - wave + NW - 1) / NW : 0;
     const int32_t * pages = a.p.pages + plan.s * a.p.ld;
     const int sub = a.p.shift - 5;
-    int ent = -1;
-    const auto entries = [&](int k) { ent = k + lane < n ? pages[(first + wave + NW * (k + lane)) >> sub] : -1; };
-    if (n) entries(0);
+    int entry = -1;
+    const auto entries = [&](int k0) {
+        if (k0 + lane < n) entry = pages[(first + wave + NW * (k0 + lane)) >> sub];
+    };
+    uint32_t at_lo, at_hi;
+    const auto addresses = [&](int k0) {
+        const int t = first + wave + NW * (k0 + lane);
+        const uint64_t at = (uint64_t) (uintptr_t) a.p.data + (((((uint64_t) (uint32_t) entry * a.p.Hkv + hk) << sub) + (t & ((1 << sub) - 1))) * (36 * D));
+        const bool there = k0 + lane < n && (unsigned) entry < (unsigned) a.p.n_pages;
+        at_lo = there ? (uint32_t) at : 0;
+        at_hi = there ? (uint32_t) (at >> 32) : 0;
+        asm volatile("" : "+v"(at_lo), "+v"(at_hi));  // (the entries are waited for here, once)
+    };
+    entries(0);
 
     // Q: of a lane's row, dims 32 b + 8 g + order(0 .. 7)
     const auto load_q = [&](int i, int b) {
@@ -251,22 +280,23 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<D, RT>)) void k_paged_few(const 
 
     uint8_t * const ring = shared + wave * (RING * 36 * D);
     const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (__attribute__((address_space(3))) uint8_t *) ring);
-    int at = 0, issued = 0, tile_of = 0;  // next of this wavefront's tiles, tiles under way or done, the ring's tiles (by lane)
-    const auto issue = [&] {
-        for (; at < n; at++) {
-            if ((at & 63) == 0 && at) entries(at);
-            const int e = __builtin_amdgcn_readlane(ent, at & 63), t = first + wave + NW * at;
-            if ((unsigned) e >= (unsigned) a.p.n_pages) continue;  // a page that is not there
-            const int slot = issued % RING;
-            tile_of = lane == slot ? t : tile_of;
-            tile_load<D>(a.p.data, ((((int64_t) e * a.p.Hkv + hk) << sub) + (t & ((1 << sub) - 1))) * (36 * D), ring_at + slot * (36 * D), lane);
-            issued++;
-            at++;
-            return;
+    // the next tile that is there, from k on, sent into a slot; n if there is none
+    const auto issue = [&](int k, int slot) {
+        for (; k < n; k++) {
+            if ((k & 63) == 0 && k) {
+                entries(k);
+                addresses(k);
+            }
+            const uint32_t lo = __builtin_amdgcn_readlane(at_lo, k & 63), hi = __builtin_amdgcn_readlane(at_hi, k & 63);
+            if (lo | hi) {
+                tile_load<D>(reinterpret_cast<const uint8_t *>((uint64_t) hi << 32 | lo), ring_at + slot * (36 * D), lane);
+                break;
+            }
         }
+        return k;
     };
-#pragma unroll
-    for (int i = 0; i < RING; i++) issue();
+    addresses(0);
+    int at = issue(0, 0), after = issue(at + 1, 1);
 
     // the work on RA times 16 rows
     const auto body = [&](auto ra) {
@@ -289,10 +319,10 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<D, RT>)) void k_paged_few(const 
         // lane lr = 4 g' + i takes the keys 8 g' + order(4 T + i), T = 0, 1, as its MFMA row
         const uint32_t ko = (8 * (lr >> 2) + paged_order(lr & 3)) * (D / 2) + g * (D / 8), vo = 16 * D + 16 * lane, so = 32 * D + 16 * g;
 
-        for (int done = 0; done < issued; done++) {
-            if (issued - done == RING) wait_loads<(RING - 1) * NL>();
+        for (int slot = 0; at < n; slot ^= 1) {
+            if (after < n) wait_loads<NL>();
             else wait_loads<0>();
-            const int slot = done % RING, tile = __builtin_amdgcn_readlane(tile_of, slot);
+            const int tile = first + wave + NW * at;
             uint8_t * const t = ring + slot * (36 * D);
 
             // scores: a block's MFMAs, then the next block's Q on its way while the sums are scaled
@@ -346,6 +376,7 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<D, RT>)) void k_paged_few(const 
                 int low, span;
 #pragma unroll
                 for (int i = 0; i < RA; i++) {
+                    barrier();
                     const int64_t pos = (int64_t) sw.past + (x0 + min(16 * i + lr, nr - 1)) / a.G;
                     seen(pos, pos, low, span);
 #pragma unroll
@@ -367,13 +398,18 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<D, RT>)) void k_paged_few(const 
                     *vd = z;
                 }
             }
-            h8_t ph[RA], pl[RA];
+            // the weights: R first, for all rows in one branch, then exponents
+            float mx[RA];
+            bool move = false;
 #pragma unroll
             for (int i = 0; i < RA; i++) {
-                barrier();
-                const float mx = max8(S[i]) * c2;
-                if (__any(mx > top[i])) {
-                    const float m = xor16_max(mx), Rn = m > top[i] ? ceilf(m) : R[i];  // (a row's R goes by its own scores)
+                mx[i] = max8(S[i]) * c2;
+                move = move || mx[i] > top[i];
+            }
+            if (__any(move)) {
+#pragma unroll
+                for (int i = 0; i < RA; i++) {
+                    const float m = xor16_max(mx[i]), Rn = m > top[i] ? ceilf(m) : R[i];  // (a row's R goes by its own scores)
                     const float al = R[i] == Rn ? 1.0f : __builtin_amdgcn_exp2f(R[i] - Rn);
                     R[i] = Rn;
                     top[i] = Rn + kSlack;
@@ -383,32 +419,32 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<D, RT>)) void k_paged_few(const 
                     for (int t = 0; t < NT; t++) O[i][t] *= al;
                     big = big || __any(fabsf(Rn) >= kBig && Rn != -INFINITY);
                 }
-                float c = c2;
-                if (big) {  // a row's R is its largest exponent rounded: round all alike
+            }
+            float c[RA], sh[RA];
+#pragma unroll
+            for (int i = 0; i < RA; i++) c[i] = c2, sh[i] = shift[i];
+            if (big) {  // a row's R is its largest exponent rounded: round all alike
+#pragma unroll
+                for (int i = 0; i < RA; i++) {
                     const bool mine = fabsf(shift[i]) >= kBig;
 #pragma unroll
                     for (int e = 0; e < 8; e++) S[i][e] = mine ? rounded(S[i][e] * c2) - R[i] : S[i][e];
-                    c = mine ? 1.0f : c2;
+                    c[i] = mine ? 1.0f : c2;
+                    sh[i] = mine ? kP : shift[i];
                 }
-                const float sh = big && fabsf(shift[i]) >= kBig ? kP : shift[i];
+            }
+            h8_t ph[RA], pl[RA];
 #pragma unroll
-                for (int e = 0; e < 8; e++) S[i][e] = __builtin_amdgcn_exp2f(fmaf(S[i][e], c, sh));
+            for (int i = 0; i < RA; i++)
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) {
-                    const float p0 = S[i][e], p1 = S[i][e + 1];
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(S[i][e], c[i], sh[i])), p1 = __builtin_amdgcn_exp2f(fmaf(S[i][e + 1], c[i], sh[i]));
                     const h2_t w = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
                     const h2_t u = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) w.x, -1.0f, p0), fmaf((float) w.y, -1.0f, p1)));
                     ph[i][e] = w.x, ph[i][e + 1] = w.y, pl[i][e] = u.x, pl[i][e + 1] = u.y;
                 }
-                h8_t one;
-#pragma unroll
-                for (int e = 0; e < 8; e++) one[e] = (_Float16) 1.0f;
-                f4_t z = {};
-                z = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, pl[i], z, 0, 0, 0);
-                z = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, ph[i], z, 0, 0, 0);
-                l[i] += z[0];
-            }
-            // P V: 16 dims' MFMAs, then the next 16 dims' operands while they run, then their sums
+            // P V: 16 dims' MFMAs, then the next 16 dims' operands and the last ones' sums while they run; a row of ones at the
+            // end for the sum of weights
             u4_t vc;
             h8_t vd[2], vh, vl;
             const auto next_v = [&](int n) {  // n: [b][u][low, high nibbles]
@@ -428,29 +464,44 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<D, RT>)) void k_paged_few(const 
                     vh[2 * i] = hi.x, vh[2 * i + 1] = hi.y, vl[2 * i] = lo.x, vl[2 * i + 1] = lo.y;
                 }
             };
+            f4_t z[2][RA];
+            const auto add = [&](int n) {
+                const int td = 2 * (n >> 2) + (n >> 1 & 1) + (n & 1) * (D / 32);  // dims 16 td ..
+#pragma unroll
+                for (int i = 0; i < RA; i++) {
+                    O[i][td] += z[n & 1][i];
+                    asm volatile("" : "+v"(O[i][td]));  // here: put off to the loop's end, every z keeps its registers
+                }
+            };
             next_v(0);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const int td = 2 * (n >> 2) + (n >> 1 & 1) + (n & 1) * (D / 32);  // dims 16 td ..
-                f4_t z[RA];
                 barrier();
 #pragma unroll
-                for (int i = 0; i < RA; i++) z[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[i], f4_t{}, 0, 0, 0);
+                for (int i = 0; i < RA; i++) z[n & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[i], f4_t{}, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < RA; i++) z[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[i], z[i], 0, 0, 0);
+                for (int i = 0; i < RA; i++) z[n & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[i], z[n & 1][i], 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < RA; i++) z[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[i], z[i], 0, 0, 0);
+                for (int i = 0; i < RA; i++) z[n & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[i], z[n & 1][i], 0, 0, 0);
                 barrier();
+                if (n) add(n - 1);
                 if (n + 1 < NT) next_v(n + 1);
-                barrier();
-#pragma unroll
-                for (int i = 0; i < RA; i++) {
-                    O[i][td] += z[i];
-                    asm volatile("" : "+v"(O[i][td]));  // here: put off to the loop's end, every z keeps its registers
-                }
             }
+            h8_t one;
+#pragma unroll
+            for (int e = 0; e < 8; e++) one[e] = (_Float16) 1.0f;
+            barrier();
+#pragma unroll
+            for (int i = 0; i < RA; i++) z[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, pl[i], f4_t{}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < RA; i++) z[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, ph[i], z[0][i], 0, 0, 0);
+            barrier();
+            add(NT - 1);
+#pragma unroll
+            for (int i = 0; i < RA; i++) l[i] += z[0][i][0];
             wait_lds();  // the slot is read before the next tile is sent into it
-            issue();
+            at = after;
+            after = issue(after + 1, slot);
         }
 
         // the wavefronts' sums, brought to one R and added, 16 rows at a time
@@ -498,365 +549,108 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<D, RT>)) void k_paged_few(const 
     else body(std::integral_constant<int, RT>{});
 }
 
-// ------------------------------------------------------------------------ many rows of a sequence
-
-// k_paged_many: a workgroup of four wavefronts takes 128 rows of a KV head, 32 a wavefront, and KT tiles of keys at a time. Each
-// wavefront turns its share of the tiles' codes into operands of v_mfma_f32_32x32x16_f16, K's and V's values d (c - 8) as two f16
-// parts each (15 bits: exact), and leaves them in LDS, lane by lane as the MFMAs take them, so that all four read them without a
-// conflict; the next tiles' codes come into registers meanwhile. Scores, weights and sums as in k_paged_few, but that a score's
-// chain runs over all dims (the small parts first). A lane holds the scores of one row and, of each tile, of the keys
-// 8 G + order(j), G = 2 kc + lk: what its P V operand of chunk kc holds, V's operand being made of the same keys.
-template <int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_paged_many(const AttnArgs a) {
-    constexpr int NW = 4, KT = D == 256 ? 1 : 2, PP = NW / KT, ROWS = 32 * NW, NC = D / 16, ND = D / 32;
-    constexpr int KU = D / 64 < PP / 2 ? 1 : D / 64 / (PP / 2);  // 64-dim groups of K codes of half the keys, per wavefront
-    constexpr int VU = D / 32 / PP;                              // 32-dim groups of V codes of all keys, per wavefront
-    __shared__ __align__(16) h8_t sk[KT][NC][2][64], sv[KT][ND][2][2][64];  // [tile][chunk][part][lane], [tile][dims][chunk][part][lane]
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31, lk = lane >> 5;
-    Plan<ROWS> plan(a);
-    if (!plan.find([&](int, int sum) { return __ballot(sum > (int) blockIdx.x); })) return;
-    const SeqWork sw = plan.picked();
-    const int ns = splits(sw.tiles, plan.chunk), id = blockIdx.x - plan.base;
-    const int split = id % ns, rt = sw.rts - 1 - id / ns % sw.rts, hk = id / ns / sw.rts;
-
-    const int rows = sw.rows * a.G, x0 = rt * ROWS, nr = min(ROWS, rows - x0);  // the workgroup's rows
-    const int w0 = 32 * wave, wn = max(0, min(32, nr - w0));                     // this wavefront's of them
-    const int64_t cap = (int64_t) a.p.max_pages << a.p.shift;
-    const auto pos_of = [&](int y) { return (int64_t) sw.past + (x0 + y) / a.G; };
-    const auto low_of = [&](int64_t pos) { return a.window ? max(pos - a.window + 1, (int64_t) 0) : (int64_t) 0; };
-    const int64_t pos0 = pos_of(0), pos1 = pos_of(nr - 1);
-    const int first = max(sw.tile0 + split * plan.chunk, (int) (low_of(pos0) >> 5));
-    const int last = min(sw.tile0 + min(sw.tiles, (split + 1) * plan.chunk), (int) ((min(pos1 + 1, cap) + 31) >> 5));
-    // the tiles that this wavefront's rows see; below e0 or from e1 on not whole
-    const int64_t wp0 = pos_of(min(w0, nr - 1)), wp1 = pos_of(min(w0 + max(wn, 1) - 1, nr - 1));
-    const int wf = wn ? (int) (low_of(wp0) >> 5) : 0, wl = wn ? (int) ((min(wp1 + 1, cap) + 31) >> 5) : 0;
-    const int e0 = a.window ? (int) ((wp1 - a.window) >> 5) + 1 : 0, e1 = (int) ((wp0 + 1) >> 5);
-
-    // the tiles' page entries, in the lanes, 64 at a time (KT divides 64)
-    const int n = max(0, last - first);
-    const int32_t * pages = a.p.pages + plan.s * a.p.ld;
-    const int sub = a.p.shift - 5;
-    int ent = -1;
-    const auto entries = [&](int k) { ent = k + lane < n ? pages[(first + k + lane) >> sub] : -1; };
-    if (n) entries(0);
-    const auto there = [&](int k) { return k < n && (unsigned) __builtin_amdgcn_readlane(ent, k & 63) < (unsigned) a.p.n_pages; };
-
-    // Q of the lane's row: chunk cc = [nibble H][block b of D/64][g >> 1], its half lk the dims D/2 H + 32 b + 8 g + order(0 .. 7)
-    const int row = x0 + min(w0 + lr, nr - 1);
-    const int64_t pos = (int64_t) sw.past + row / a.G;
-    h8_t qf[NC];
-    {
-        const _Float16 * qp = a.q + (int64_t) (sw.r0 + row / a.G) * a.q_r + (int64_t) (hk * a.G + row % a.G) * a.q_h + 8 * lk;
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            h8_t v = *reinterpret_cast<const h8_t *>(qp + 16 * c);
-            if (w0 + lr >= nr) v = h8_t{};
-            if (a.negate) v = -v;
-            qf[c] = h8_t{v[0], v[2], v[1], v[3], v[4], v[6], v[5], v[7]};
-        }
-    }
-
-    // This wavefront's share of a stage: of tile mt, K codes of the keys 16 T + (lane & 15), group g = lane >> 4 of 8 dims of each
-    // block, of the 64-dim groups kb ..; V codes of the lane's 8 keys and its dims of the 32-dim groups vb ..
-    const int mt = wave / PP, piece = wave % PP, T = piece & 1, c16 = lane & 15, g = lane >> 4;
-    const int kb = (piece >> 1) * KU, vb = piece * VU;
-    const int key = 16 * T + c16, slot = paged_order(key & 7);
-    const uint32_t ko = key * (D / 2) + g * (D / 8) + 8 * kb, kdo = 32 * D + 2 * ((key & 24) + slot);
-    // (MFMA row of the key: its slot (kc, lk, j) in P V's order)
-    const int krow = 16 * (key >> 4) + 8 * (slot >> 2) + 4 * (key >> 3 & 1) + (slot & 3) + 32 * (g & 1);
-    u2_t kr[KU], vr[VU];
-    _Float16 kd[KU][2] = {};
-    h8_t vd[VU][2] = {};
-    const auto load = [&](int k) {  // the tile k + mt
-        if (!there(k + mt)) {
-#pragma unroll
-            for (int u = 0; u < VU; u++) vd[u][0] = vd[u][1] = h8_t{};
-            return;
-        }
-        const int e = __builtin_amdgcn_readlane(ent, (k + mt) & 63), t = first + k + mt;
-        const uint8_t * p = a.p.data + ((((int64_t) e * a.p.Hkv + hk) << sub) + (t & ((1 << sub) - 1))) * (36 * D);
-#pragma unroll
-        for (int u = 0; u < KU; u++) {
-            kr[u] = *reinterpret_cast<const u2_t *>(p + ko + 8 * u);
-#pragma unroll
-            for (int H = 0; H < 2; H++) kd[u][H] = *reinterpret_cast<const _Float16 *>(p + kdo + 64 * (kb + u + H * (D / 64)));
-        }
-#pragma unroll
-        for (int u = 0; u < VU; u++) {  // 32-dim group vb + u: byte group u & 1 of t = u >> 1
-            vr[u] = *reinterpret_cast<const u2_t *>(p + 16 * D + 1024 * ((vb + u) >> 1) + 16 * lane + 8 * ((vb + u) & 1));
-#pragma unroll
-            for (int H = 0; H < 2; H++) vd[u][H] = *reinterpret_cast<const h8_t *>(p + 34 * D + 64 * (((vb + u) >> 1) + H * (D / 64)) + 16 * g);
-        }
-        // A key that no row sees may hold anything, a NaN for a scale too: its values' scales are taken as 0.
-        const int64_t k0 = 32 * (int64_t) t;
-        if (k0 + 31 > pos1 || k0 < low_of(pos0)) {
-            const int low = (int) max(low_of(pos0) - k0 - 8 * g, (int64_t) 0), span = max((int) (min(pos1 + 1, cap) - k0 - 8 * g) - low, 0);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const bool gone = (unsigned) (((j & 4) | (j & 1) << 1 | (j >> 1 & 1)) - low) >= (unsigned) span;
-#pragma unroll
-                for (int u = 0; u < VU; u++) {
-                    vd[u][0][j] = gone ? (_Float16) 0.0f : vd[u][0][j];
-                    vd[u][1][j] = gone ? (_Float16) 0.0f : vd[u][1][j];
-                }
-            }
-        }
-    };
-    const auto parts = [](const h2_t (&c)[4], const h8_t & d, h8_t & hi, h8_t & lo) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const h2_t di = {d[2 * i], d[2 * i + 1]}, h = c[i] * di, r = __builtin_elementwise_fma(c[i], di, -h);
-            hi[2 * i] = h.x, hi[2 * i + 1] = h.y, lo[2 * i] = r.x, lo[2 * i + 1] = r.y;
-        }
-    };
-    const auto store = [&] {
-#pragma unroll
-        for (int u = 0; u < KU; u++)
-#pragma unroll
-            for (int H = 0; H < 2; H++) {
-                h2_t c[4];
-                if (H) code_values<1>(kr[u].x, kr[u].y, c);
-                else code_values<0>(kr[u].x, kr[u].y, c);
-                h8_t d, hi, lo;
-#pragma unroll
-                for (int j = 0; j < 8; j++) d[j] = kd[u][H];
-                parts(c, d, hi, lo);
-                h8_t * o = sk[mt][((H * (D / 64) + kb + u) << 1) + (g >> 1)][0] + krow;
-                o[0] = hi;
-                o[64] = lo;
-            }
-#pragma unroll
-        for (int u = 0; u < VU; u++)
-#pragma unroll
-            for (int H = 0; H < 2; H++) {
-                h2_t c[4];
-                if (H) code_values<1>(vr[u].x, vr[u].y, c);
-                else code_values<0>(vr[u].x, vr[u].y, c);
-                h8_t hi, lo;
-                parts(c, vd[u][H], hi, lo);
-                h8_t * o = sv[mt][((vb + u) >> 1) + H * (D / 64)][g >> 1][0] + 16 * ((vb + u) & 1) + c16 + 32 * (g & 1);
-                o[0] = hi;
-                o[64] = lo;
-            }
-    };
-
-    v16f O[ND];
-    float R = -INFINITY, l = 0.0f, shift = kP;  // the reference exponent; this lane's part of the sum of weights; kP - R
-#pragma unroll
-    for (int t = 0; t < ND; t++) O[t] = v16f{};
-    const float c2 = a.c2;
-
-    // the next stage with a tile in it, from tile k on (a multiple of KT)
-    const auto next = [&](int k) {
-        for (; k < n; k += KT) {
-            if ((k & 63) == 0 && k) entries(k);
-            bool any = false;
-#pragma unroll
-            for (int t = 0; t < KT; t++) any = any || there(k + t);
-            if (any) break;
-        }
-        return k;
-    };
-    int k = next(0);
-    if (k < n) load(k);
-    while (k < n) {
-        uint32_t live = 0;  // tiles that are there and that some of this wavefront's rows see
-        const int tile0 = first + k;
-#pragma unroll
-        for (int t = 0; t < KT; t++) live |= (uint32_t) (there(k + t) && tile0 + t >= wf && tile0 + t < wl) << t;
-        __syncthreads();  // the last stage is read
-        store();
-        __syncthreads();
-        k = next(k + KT);
-        if (k < n) load(k);
-        if (!live) continue;
-
-        v16f S[KT];
-#pragma unroll
-        for (int t = 0; t < KT; t++) {
-            v16f A{};
-#pragma unroll
-            for (int p = 1; p >= 0; p--)
-#pragma unroll
-                for (int c = 0; c < NC; c++) A = __builtin_amdgcn_mfma_f32_32x32x16_f16(sk[t][c][p][lane], qf[c], A, 0, 0, 0);
-            S[t] = A;
-        }
-#pragma unroll
-        for (int t = 0; t < KT; t++)
-            if (tile0 + t < e0 || tile0 + t >= e1 || !(live >> t & 1)) {  // keys that some row does not see
-                const int64_t k0 = 32 * (int64_t) (tile0 + t) + 8 * lk;
-                const int low = (int) max(low_of(pos) - k0, (int64_t) 0), span = live >> t & 1 ? max((int) (min(pos + 1, cap) - k0) - low, 0) : 0;
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int j = 16 * (r >> 3) + ((r & 4) | (r & 1) << 1 | (r >> 1 & 1));  // 16 kc + order(j)
-                    S[t][r] = (unsigned) (j - low) < (unsigned) span ? S[t][r] : -INFINITY;
-                }
-            }
-        // exponents against R as it is; where one passes it by too much, R moves and they are formed again
-        float x[KT][16];
-        const auto exponents = [&] {
-#pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) x[t][r] = fmaf(S[t][r], c2, shift);
-        };
-        exponents();
-        float mx = x[0][0];
-#pragma unroll
-        for (int t = 0; t < KT; t++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) mx = fmaxf(mx, x[t][r]);
-        if (__any(mx > kP + kSlack || R == -INFINITY)) {
-            float m = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) m = fmaxf(m, S[t][r]);
-            m = row_pair<32>(m * c2, fmaxf_op);
-            const float Rn = m > R + kSlack ? ceilf(m) : R;  // (a row's R goes by its own scores)
-            const float al = R == Rn ? 1.0f : __builtin_amdgcn_exp2f(R - Rn);
-            R = Rn;
-            shift = kP - (Rn == -INFINITY ? 0.0f : Rn);
-            l *= al;
-#pragma unroll
-            for (int t = 0; t < ND; t++) O[t] *= al;
-            exponents();
-        }
-        if (__any(fabsf(shift) >= kBig)) {  // a row's R is its largest exponent rounded: round all alike
-            const bool mine = fabsf(shift) >= kBig;
-#pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) x[t][r] = mine ? (rounded(S[t][r] * c2) - R) + kP : x[t][r];
-        }
-        h8_t ph[KT][2], pl[KT][2];
-        float l2 = 0.0f;
-        constexpr h2_t one = {(_Float16) 1.0f, (_Float16) 1.0f};
-#pragma unroll
-        for (int t = 0; t < KT; t++)
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(x[t][r]), p1 = __builtin_amdgcn_exp2f(x[t][r + 1]);
-                const h2_t w = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-                const h2_t u = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) w.x, -1.0f, p0), fmaf((float) w.y, -1.0f, p1)));
-                l2 = __builtin_amdgcn_fdot2(w, one, l2, false);
-                l = __builtin_amdgcn_fdot2(u, one, l, false);
-                ph[t][r >> 3][r & 7] = w.x, ph[t][r >> 3][(r & 7) + 1] = w.y, pl[t][r >> 3][r & 7] = u.x, pl[t][r >> 3][(r & 7) + 1] = u.y;
-            }
-        l += l2;
-#pragma unroll
-        for (int d = 0; d < ND; d++) {
-            __builtin_amdgcn_sched_barrier(0);
-            v16f z{};
-#pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const h8_t vh = sv[t][d][c][0][lane], vl = sv[t][d][c][1][lane];
-                    z = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[t][c], z, 0, 0, 0);
-                    z = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[t][c], z, 0, 0, 0);
-                    z = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[t][c], z, 0, 0, 0);
-                }
-            O[d] += z;
-            asm volatile("" : "+v"(O[d]));  // here: put off to the loop's end, every z keeps its registers
-        }
-    }
-    l = row_pair<32>(l, op_add<float>);
-    if (w0 + lr >= nr) return;
-    float * o = ns == 1 ? a.out + ((int64_t) (sw.r0 + row / a.G) * a.H + hk * a.G + row % a.G) * D + 4 * lk
-                        : a.part_o + ((int64_t) blockIdx.x * ROWS + w0 + lr) * D + 4 * lk;
-    const float f = ns == 1 ? 1.0f / l : 1.0f;
-#pragma unroll
-    for (int t = 0; t < ND; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            f4_t y;
-#pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = ns == 1 && l == 0.0f ? 0.0f : O[t][4 * i + r] * f;
-            *reinterpret_cast<f4_t *>(o + 32 * t + 8 * i) = y;
-        }
-    if (ns > 1 && lk == 0) a.part_ml[(int64_t) blockIdx.x * ROWS + w0 + lr] = make_float2(R, l);
-}
-
-// One (row, head): its splits' sums, weighted by 2^(R - the largest R).
+// A row tile of several splits: their sums, weighted by 2^(R - the largest R). A workgroup takes one row, its wavefronts sharing the
+// splits, of a tile of 16 rows (few of them, in many splits); 16 rows, four to a wavefront, of a larger one.
 template <int D, int ROWS>
 __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a) {
-    const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    constexpr int WR = ROWS == 16 ? 4 : 1, per = ROWS == 16 ? 1 : 16;  // wavefronts to a row, rows to a workgroup
+    constexpr int L = D / 4, NP = WR * 64 / L;                         // lanes of a split, splits at a time
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     Plan<ROWS> plan(a);
-    if (!plan.find([&](int s, int) { return __ballot(s < a.p.n_seq && plan.w.r0 <= row && row < plan.w.r0 + plan.w.rows); })) return;
+    if (!plan.find_tile(blockIdx.x)) return;
     const SeqWork sw = plan.picked();
-    const int ns = splits(sw.tiles, plan.chunk), j = row - sw.r0;
+    const int ns = splits(sw.tiles, plan.chunk);
     if (ns == 1) return;
-    const int x = j * a.G + h % a.G;
-    const int64_t item = plan.base + ((int64_t) (h / a.G) * sw.rts + sw.rts - 1 - x / ROWS) * ns;
-    if (item < 0 || item + ns > a.items) return;  // (starts that do not ascend)
-    const float2 * ml = a.part_ml + item * ROWS + x % ROWS;
-    const float * o = a.part_o + (item * ROWS + x % ROWS) * D;
-    float R = -INFINITY;
-    for (int i = lane; i < ns; i += 64) R = fmaxf(R, ml[(int64_t) i * ROWS].x);
-    R = wave_max(R);
-    constexpr int NP = 256 / (D / 4);  // splits at a time, a thread taking four dims
-    const int d4 = tid % (D / 4), part = tid / (D / 4);
-    f4_t acc = {};
-    float l = 0.0f;
-#pragma unroll 4
-    for (int i = part; i < ns; i += NP) {
-        const float2 m = ml[(int64_t) i * ROWS];
-        const float w = m.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m.x - R);
-        l += m.y * w;
-        acc += *reinterpret_cast<const f4_t *>(o + (int64_t) i * ROWS * D + 4 * d4) * w;
+    const int id = blockIdx.x - plan.base, rt = sw.rts - 1 - id % sw.rts, hk = id / sw.rts;
+    const int64_t item = plan.first_item + (int64_t) id * ns;
+    if (item + ns > a.items) return;  // (starts that do not ascend)
+    const int x0 = rt * ROWS, y1 = min(min(ROWS, sw.rows * a.G - x0), (int) (blockIdx.y + 1) * per);
+    __shared__ f4_t so[WR > 1 ? NP : 1][L];
+    __shared__ float sl[WR > 1 ? NP : 1];
+    for (int y = blockIdx.y * per + wave / WR; y < y1; y += 4 / WR) {
+        const float2 * ml = a.part_ml + item * ROWS + y;
+        const float * o = a.part_o + (item * ROWS + y) * D;
+        float R = -INFINITY;
+        for (int i = lane; i < ns; i += 64) R = fmaxf(R, ml[(int64_t) i * ROWS].x);
+        R = wave_max(R);
+        const int part = (WR > 1 ? tid : lane) / L, d = lane % L;
+        f4_t acc = {};
+        float l = 0.0f;
+        for (int i = part; i < ns; i += 8 * NP) {  // eight loads under way at a time
+            float2 m[8];
+            f4_t v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int64_t at = min(i + k * NP, ns - 1);
+                m[k] = ml[at * ROWS];
+                v[k] = *reinterpret_cast<const f4_t *>(o + at * ROWS * D + 4 * d);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float w = i + k * NP >= ns || m[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k].x - R);
+                l += m[k].y * w;
+                acc += v[k] * w;
+            }
+        }
+        if constexpr (WR > 1) {
+            so[part][d] = acc;
+            if (d == 0) sl[part] = l;
+            __syncthreads();
+            if (part) return;  // (one row to a workgroup)
+#pragma unroll
+            for (int i = 1; i < NP; i++) {
+                acc += so[i][d];
+                l += sl[i];
+            }
+        } else {
+#pragma unroll
+            for (int s = 32; s >= L; s >>= 1) {
+                l += __shfl_xor(l, s, 64);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], s, 64);
+            }
+            if (part) continue;
+        }
+        const int x = x0 + y;
+        const float inv = 1.0f / l;
+        *reinterpret_cast<f4_t *>(a.out + ((int64_t) (sw.r0 + x / a.G) * a.H + hk * a.G + x % a.G) * D + 4 * d) = l == 0.0f ? f4_t{} : acc * inv;
     }
-    __shared__ f4_t so[NP][D / 4];
-    __shared__ float sl[NP];
-    so[part][d4] = acc;
-    if (d4 == 0) sl[part] = l;
-    __syncthreads();
-    if (part) return;
-    for (int i = 1; i < NP; i++) {
-        acc += so[i][d4];
-        l += sl[i];
-    }
-    const float inv = 1.0f / l;
-    *reinterpret_cast<f4_t *>(a.out + ((int64_t) row * a.H + h) * D + 4 * d4) = l == 0.0f ? f4_t{} : acc * inv;
 }
 
-// How a call is run: row tiles of `rows` rows (up to 32: k_paged_few), splits that aim at `target` workgroups, those resident at
-// once.
+// How a call is run: row tiles of `rows` rows, `waves` wavefronts to each, splits that aim at `target` workgroups, those
+// resident at once.
 struct Shape {
-    int rows, target;
-    int64_t items, most;  // workgroups that may have work; splits of a sequence
+    int rows, waves, target;
+    int64_t tiles, items, most;  // row tiles and workgroups that may have work; splits of a sequence
 };
 Shape shape_for(const Paged & p, int D, int G, int64_t max_rows) {
     Shape s{};
     const int64_t per_seq = std::min<int64_t>(max_rows, p.n_rows) * G;  // rows of a KV head
-    s.rows = per_seq <= 16 ? 16 : per_seq <= 32 ? 32 : 128;
-    s.target = 256 * (s.rows == 16 && D != 256 ? 4 : 2);
+    s.rows = per_seq <= 16 ? 16 : 32;
+    s.waves = waves(D, s.rows);
+    s.target = 256 * 4 * per_simd(D, s.rows / 16) / s.waves;
     // row tiles: the rows' whole tiles and one more for each sequence
-    const int64_t rts = p.Hkv * std::min<int64_t>((int64_t) p.n_rows * G / s.rows + std::min<int64_t>(p.n_seq, p.n_rows),
-                                                  p.n_seq * ((per_seq + s.rows - 1) / s.rows));
+    s.tiles = p.Hkv * std::min<int64_t>((int64_t) p.n_rows * G / s.rows + std::min<int64_t>(p.n_seq, p.n_rows),
+                                        p.n_seq * ((per_seq + s.rows - 1) / s.rows));
     s.most = (((int64_t) p.max_pages << p.shift) / kPagedTile + kMinChunk - 1) / kMinChunk;
-    s.items = std::min(rts + s.target, rts * s.most);
+    s.items = std::min(s.tiles + s.target, s.tiles * s.most);
     return s;
 }
 
-template <int D, int ROWS>
-void merge(const AttnArgs & a, const Shape & w, hipStream_t s) {
+template <int D, int RT>
+void launch(const AttnArgs & a, const Shape & w, hipStream_t s) {
+    constexpr int ROWS = 16 * RT, NW = waves(D, ROWS);
+    k_paged_attn<D, RT, NW><<<(unsigned) a.items, 64 * NW, 0, s>>>(a);
     check_launch("paged attn");
-    if (w.most > 1) k_paged_merge<D, ROWS><<<dim3((unsigned) a.p.n_rows, (unsigned) a.H), 256, 0, s>>>(a);
+    if (w.most == 1) return;
+    const int rows = (int) std::min<int64_t>(ROWS, (int64_t) a.max_rows * a.G), per = RT == 1 ? 1 : 16;
+    k_paged_merge<D, ROWS><<<dim3((unsigned) w.tiles, (unsigned) ((rows + per - 1) / per)), 256, 0, s>>>(a);
     check_launch("paged attn merge");
 }
 template <int D>
 void run(const AttnArgs & a, const Shape & w, hipStream_t s) {
-    if (w.rows == 16) {
-        k_paged_few<D, 1, 4><<<(unsigned) a.items, 256, 0, s>>>(a);
-        merge<D, 16>(a, w, s);
-    } else if (w.rows == 32) {
-        k_paged_few<D, 2, 4><<<(unsigned) a.items, 256, 0, s>>>(a);
-        merge<D, 32>(a, w, s);
-    } else {
-        k_paged_many<D><<<(unsigned) a.items, 256, 0, s>>>(a);
-        merge<D, 128>(a, w, s);
-    }
+    if (w.rows == 16) launch<D, 1>(a, w, s);
+    else launch<D, 2>(a, w, s);
 }
 
 }  // namespace
