@@ -39,11 +39,17 @@ struct AttnArgs {
     Paged p;
     const _Float16 * q;
     int64_t q_r, q_h;
-    int H, G, window, max_rows, items, target;  // target: workgroups that the splits aim at
+    int H, G, window, max_rows, items, target, min_chunk;  // target: workgroups that the splits aim at
     float c2;     // |scale| log2(e)
     bool negate;  // the scale is negative
     float * out, * part_o;
     float2 * part_ml;
+    struct Part * parts;  // one for each workgroup; null: nothing is split
+};
+
+// What k_paged_merge has to know of a workgroup's row tile.
+struct __align__(32) Part {
+    int ns, split, nr, hk, r0, x0;  // ns 0: no work
 };
 
 // A sequence's rows, and the tiles of the keys that any of them sees.
@@ -86,7 +92,6 @@ struct Plan {
     const AttnArgs & a;
     SeqWork w;  // of sequence s0 + lane
     int chunk, s, base, lane_at;
-    int64_t first_item;
 
     __device__ __forceinline__ Plan(const AttnArgs & args) : a(args) {
         const int lane = threadIdx.x & 63;
@@ -100,9 +105,8 @@ struct Plan {
         u = wave_sum_d(u) * a.p.Hkv;
         n = wave_sum_d(n) * a.p.Hkv;
         const double cut = fmax(a.target - n, 0.5 * a.target);
-        chunk = __builtin_amdgcn_readfirstlane((int) fmax((double) kMinChunk, fmin(u / cut + 1.0, 1e9)));
+        chunk = __builtin_amdgcn_readfirstlane((int) fmax((double) a.min_chunk, fmin(u / cut + 1.0, 1e9)));
     }
-    __device__ __forceinline__ int items(const SeqWork & x) const { return x.rts * a.p.Hkv * splits(x.tiles, chunk); }
 
     // The sequence found, uniform.
     __device__ __forceinline__ SeqWork picked() {
@@ -112,37 +116,14 @@ struct Plan {
         s = __builtin_amdgcn_readfirstlane(s);
         return {pick(w.r0), pick(w.rows), pick(w.tile0), pick(w.tiles), pick(w.rts), pick(w.past)};
     }
-    // To the sequence of row tile `id` (counted as the items are, but for the splits); base: its first, first_item: its first item.
-    __device__ __forceinline__ bool find_tile(int id) {
+    // To the sequence of item `id`; base: its first.
+    __device__ __forceinline__ bool find(int id) {
         const int lane = threadIdx.x & 63;
         base = 0;
-        first_item = 0;
         for (int s0 = 0; s0 < a.p.n_seq; s0 += 64) {
             if (s0) w = seq_work<ROWS>(a, s0 + lane);
-            const int n = w.rts * a.p.Hkv, sum = wave_scan(n), m = items(w), isum = wave_scan(m);
+            const int n = w.rts * a.p.Hkv * splits(w.tiles, chunk), sum = wave_scan(n);
             const uint64_t at = __ballot(base + sum > id);
-            if (at) {
-                lane_at = __builtin_ctzll(at);
-                base += __builtin_amdgcn_readlane(sum - n, lane_at);
-                first_item += __builtin_amdgcn_readlane(isum - m, lane_at);
-                s = s0 + lane_at;
-                return true;
-            }
-            base += __builtin_amdgcn_readlane(sum, 63);
-            first_item += __builtin_amdgcn_readlane(isum, 63);
-        }
-        return false;
-    }
-    // To the sequence that `found` (a ballot over the sequences s0 .. s0 + 63, their inclusive item sums given) picks
-    // first.
-    template <class F>
-    __device__ __forceinline__ bool find(F && found) {
-        const int lane = threadIdx.x & 63;
-        base = 0;
-        for (int s0 = 0; s0 < a.p.n_seq; s0 += 64) {
-            if (s0) w = seq_work<ROWS>(a, s0 + lane);
-            const int n = items(w), sum = wave_scan(n);
-            const uint64_t at = found(s0 + lane, base + sum);
             if (at) {
                 lane_at = __builtin_ctzll(at);
                 base += __builtin_amdgcn_readlane(sum - n, lane_at);
@@ -229,17 +210,21 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
     h8_t * const sq = reinterpret_cast<h8_t *>(shared + (kRings > kSums ? kRings : kSums));  // [16 rows][block][lane]
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     Plan<ROWS> plan(a);
-    if (!plan.find([&](int, int sum) { return __ballot(sum > (int) blockIdx.x); })) return;
+    if (!plan.find(blockIdx.x)) {
+        if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = Part{};
+        return;
+    }
     const SeqWork sw = plan.picked();
-    const int ns = splits(sw.tiles, plan.chunk), id = blockIdx.x - plan.base;
+    const int ns = splits(sw.tiles, plan.chunk), chunk = (sw.tiles + ns - 1) / ns, id = blockIdx.x - plan.base;
     const int split = id % ns, rt = sw.rts - 1 - id / ns % sw.rts, hk = id / ns / sw.rts;
 
     const int rows = sw.rows * a.G, x0 = rt * ROWS, nr = min(ROWS, rows - x0);  // this tile's rows
+    if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = {ns, split, nr, hk, sw.r0, x0};
     const int64_t pos0 = (int64_t) sw.past + x0 / a.G, pos1 = (int64_t) sw.past + (x0 + nr - 1) / a.G;
     // this row tile's keys within the split; tiles below e0 or from e1 on are not seen whole by every row
     const int64_t cap = (int64_t) a.p.max_pages << a.p.shift;
-    const int first = max(sw.tile0 + split * plan.chunk, a.window && pos0 - a.window + 1 > 0 ? (int) ((pos0 - a.window + 1) >> 5) : 0);
-    const int last = min(sw.tile0 + min(sw.tiles, (split + 1) * plan.chunk), (int) ((min(pos1 + 1, cap) + 31) >> 5));
+    const int first = max(sw.tile0 + split * chunk, a.window && pos0 - a.window + 1 > 0 ? (int) ((pos0 - a.window + 1) >> 5) : 0);
+    const int last = min(sw.tile0 + min(sw.tiles, (split + 1) * chunk), (int) ((min(pos1 + 1, cap) + 31) >> 5));
     const int e0 = a.window ? (int) ((pos1 - a.window) >> 5) + 1 : 0, e1 = (int) ((pos0 + 1) >> 5);
 
     // The tiles of this wavefront: first + wave, + NW, ..; lane i holds the address of tile k0 + i, 0 for one that is not there.
@@ -549,71 +534,94 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
     else body(std::integral_constant<int, RT>{});
 }
 
-// A row tile of several splits: their sums, weighted by 2^(R - the largest R). A workgroup takes one row, its wavefronts sharing the
-// splits, of a tile of 16 rows (few of them, in many splits); 16 rows, four to a wavefront, of a larger one.
+// A row tile of several splits: their sums, weighted by 2^(R - the largest R). The splits' workgroups share its rows, row y to
+// split y % ns's; a row's splits are read by the workgroup's four wavefronts together if they are more than one has under way.
 template <int D, int ROWS>
 __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a) {
-    constexpr int WR = ROWS == 16 ? 4 : 1, per = ROWS == 16 ? 1 : 16;  // wavefronts to a row, rows to a workgroup
-    constexpr int L = D / 4, NP = WR * 64 / L;                         // lanes of a split, splits at a time
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    Plan<ROWS> plan(a);
-    if (!plan.find_tile(blockIdx.x)) return;
-    const SeqWork sw = plan.picked();
-    const int ns = splits(sw.tiles, plan.chunk);
-    if (ns == 1) return;
-    const int id = blockIdx.x - plan.base, rt = sw.rts - 1 - id % sw.rts, hk = id / sw.rts;
-    const int64_t item = plan.first_item + (int64_t) id * ns;
-    if (item + ns > a.items) return;  // (starts that do not ascend)
-    const int x0 = rt * ROWS, y1 = min(min(ROWS, sw.rows * a.G - x0), (int) (blockIdx.y + 1) * per);
-    __shared__ f4_t so[WR > 1 ? NP : 1][L];
-    __shared__ float sl[WR > 1 ? NP : 1];
-    for (int y = blockIdx.y * per + wave / WR; y < y1; y += 4 / WR) {
-        const float2 * ml = a.part_ml + item * ROWS + y;
-        const float * o = a.part_o + (item * ROWS + y) * D;
-        float R = -INFINITY;
-        for (int i = lane; i < ns; i += 64) R = fmaxf(R, ml[(int64_t) i * ROWS].x);
-        R = wave_max(R);
-        const int part = (WR > 1 ? tid : lane) / L, d = lane % L;
-        f4_t acc = {};
-        float l = 0.0f;
-        for (int i = part; i < ns; i += 8 * NP) {  // eight loads under way at a time
+    constexpr int L = D / 4, N1 = 64 / L, N4 = 4 * N1;  // lanes of a split; splits at a time, a wavefront's and all four's
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), d = lane % L;
+    const Part w = a.parts[blockIdx.x];
+    const int ns = __builtin_amdgcn_readfirstlane(w.ns), split = __builtin_amdgcn_readfirstlane(w.split), item = blockIdx.x - split;
+    if (ns <= 1 || split >= w.nr || item + ns > a.items) return;  // (the last: starts that do not ascend)
+    __shared__ f4_t so[N4][L];
+    __shared__ float2 sml[N4];
+    const auto weight = [](float from, float to) { return from == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(from - to); };
+    const auto row = [&](int y, int part, int parts, f4_t & acc, float & R, float & l) {
+        const float2 * ml = a.part_ml + (int64_t) item * ROWS + y;
+        const float * o = a.part_o + ((int64_t) item * ROWS + y) * D;
+        R = -INFINITY;
+        acc = f4_t{};
+        l = 0.0f;
+        for (int i = part; i < ns; i += 8 * parts) {  // eight loads under way at a time
             float2 m[8];
             f4_t v[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const int64_t at = min(i + k * NP, ns - 1);
+                const int64_t at = min(i + k * parts, ns - 1);
                 m[k] = ml[at * ROWS];
                 v[k] = *reinterpret_cast<const f4_t *>(o + at * ROWS * D + 4 * d);
             }
+            float Rn = R;
+#pragma unroll
+            for (int k = 0; k < 8; k++) Rn = fmaxf(Rn, m[k].x);
+            const float al = weight(R, Rn);
+            l *= al;
+            acc *= al;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float w = i + k * NP >= ns || m[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k].x - R);
-                l += m[k].y * w;
-                acc += v[k] * w;
+                const float f = i + k * parts >= ns ? 0.0f : weight(m[k].x, Rn);
+                l += m[k].y * f;
+                acc += v[k] * f;
             }
+            R = Rn;
         }
-        if constexpr (WR > 1) {
-            so[part][d] = acc;
-            if (d == 0) sl[part] = l;
-            __syncthreads();
-            if (part) return;  // (one row to a workgroup)
-#pragma unroll
-            for (int i = 1; i < NP; i++) {
-                acc += so[i][d];
-                l += sl[i];
-            }
-        } else {
-#pragma unroll
-            for (int s = 32; s >= L; s >>= 1) {
-                l += __shfl_xor(l, s, 64);
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], s, 64);
-            }
-            if (part) continue;
-        }
-        const int x = x0 + y;
+    };
+    const auto put = [&](int y, f4_t acc, float l) {
+        const int x = w.x0 + y;
         const float inv = 1.0f / l;
-        *reinterpret_cast<f4_t *>(a.out + ((int64_t) (sw.r0 + x / a.G) * a.H + hk * a.G + x % a.G) * D + 4 * d) = l == 0.0f ? f4_t{} : acc * inv;
+        *reinterpret_cast<f4_t *>(a.out + ((int64_t) (w.r0 + x / a.G) * a.H + w.hk * a.G + x % a.G) * D + 4 * d) = l == 0.0f ? f4_t{} : acc * inv;
+    };
+    f4_t acc;
+    float R, l;
+    if (ns > 8 * N1) {  // (one or two rows: at most 32 of them)
+        for (int y = split; y < w.nr; y += ns) {
+            row(y, tid / L, N4, acc, R, l);
+            so[tid / L][d] = acc;
+            if (d == 0) sml[tid / L] = make_float2(R, l);
+            __syncthreads();
+            if (tid < L) {
+                float Rm = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < N4; i++) Rm = fmaxf(Rm, sml[i].x);
+                acc = f4_t{};
+                l = 0.0f;
+#pragma unroll
+                for (int i = 0; i < N4; i++) {
+                    const float f = weight(sml[i].x, Rm);
+                    l += sml[i].y * f;
+                    acc += so[i][d] * f;
+                }
+                put(y, acc, l);
+            }
+            __syncthreads();
+        }
+        return;
+    }
+    for (int y = split + wave * ns; y < w.nr; y += 4 * ns) {
+        row(y, lane / L, N1, acc, R, l);
+        float Rm = R;
+#pragma unroll
+        for (int s = 32; s >= L; s >>= 1) Rm = fmaxf(Rm, __shfl_xor(Rm, s, 64));
+        const float f = weight(R, Rm);
+        l *= f;
+        acc *= f;
+#pragma unroll
+        for (int s = 32; s >= L; s >>= 1) {
+            l += __shfl_xor(l, s, 64);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], s, 64);
+        }
+        if (lane < L) put(y, acc, l);
     }
 }
 
@@ -632,7 +640,8 @@ Shape shape_for(const Paged & p, int D, int G, int64_t max_rows) {
     // row tiles: the rows' whole tiles and one more for each sequence
     s.tiles = p.Hkv * std::min<int64_t>((int64_t) p.n_rows * G / s.rows + std::min<int64_t>(p.n_seq, p.n_rows),
                                         p.n_seq * ((per_seq + s.rows - 1) / s.rows));
-    s.most = (((int64_t) p.max_pages << p.shift) / kPagedTile + kMinChunk - 1) / kMinChunk;
+    const int64_t longest = ((int64_t) p.max_pages << p.shift) / kPagedTile;  // tiles
+    s.most = longest <= 2 * kMinChunk ? 1 : (longest + kMinChunk - 1) / kMinChunk;
     s.items = std::min(s.tiles + s.target, s.tiles * s.most);
     return s;
 }
@@ -643,8 +652,7 @@ void launch(const AttnArgs & a, const Shape & w, hipStream_t s) {
     k_paged_attn<D, RT, NW><<<(unsigned) a.items, 64 * NW, 0, s>>>(a);
     check_launch("paged attn");
     if (w.most == 1) return;
-    const int rows = (int) std::min<int64_t>(ROWS, (int64_t) a.max_rows * a.G), per = RT == 1 ? 1 : 16;
-    k_paged_merge<D, ROWS><<<dim3((unsigned) w.tiles, (unsigned) ((rows + per - 1) / per)), 256, 0, s>>>(a);
+    k_paged_merge<D, ROWS><<<(unsigned) a.items, 256, 0, s>>>(a);
     check_launch("paged attn merge");
 }
 template <int D>
@@ -658,7 +666,7 @@ void run(const AttnArgs & a, const Shape & w, hipStream_t s) {
 size_t paged_attn_workspace(const Paged & p, int D, int H, int64_t max_rows) {
     if (p.n_rows == 0) return 0;
     const Shape w = shape_for(p, D, H / p.Hkv, max_rows);
-    return w.most == 1 ? 0 : (size_t) w.items * w.rows * (D * sizeof(float) + sizeof(float2));
+    return w.most == 1 ? 0 : (size_t) w.items * (w.rows * (D * sizeof(float) + sizeof(float2)) + sizeof(Part));
 }
 
 void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int64_t q_h, int H, int64_t max_rows, int window,
@@ -673,8 +681,10 @@ void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int6
     const Shape w = shape_for(p, D, a.G, max_rows);
     require(w.items < INT32_MAX, "paged_attn: too many rows and heads");
     a.items = (int) w.items, a.target = w.target;
+    a.min_chunk = w.most == 1 ? 1 << 30 : kMinChunk;
     a.part_o = (float *) ws;
-    a.part_ml = (float2 *) ((char *) ws + (size_t) w.items * w.rows * D * sizeof(float));
+    a.part_ml = (float2 *) (a.part_o + (size_t) w.items * w.rows * D);
+    a.parts = w.most == 1 ? nullptr : (Part *) (a.part_ml + (size_t) w.items * w.rows);
     if (D == 64) run<64>(a, w, s);
     else if (D == 128) run<128>(a, w, s);
     else run<256>(a, w, s);
