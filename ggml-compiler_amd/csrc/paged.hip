@@ -165,9 +165,13 @@ __global__ __launch_bounds__(256) void k_paged_read(const ReadArgs a) {
 
 // ---------------------------------------------------------------------------------- checks
 
+// (messages are put together only where a check fails: a launch costs the host some 3 us, a call's strings were one more)
+void require(bool ok, const char * message) {
+    if (!ok) fail(message);
+}
 void need(const void * p, const char * what, size_t align = 1) {
-    require(p != nullptr, std::string("paged: ") + what + " is NULL");
-    require(aligned(p, align), std::string("paged: ") + what + " must be " + std::to_string(align) + "-byte aligned");
+    if (!p) fail(std::string("paged: ") + what + " is NULL");
+    if (!aligned(p, align)) fail(std::string("paged: ") + what + " must be " + std::to_string(align) + "-byte aligned");
 }
 
 bool shape_ok(int n_pages, int page, int Hkv, int D) {
@@ -306,7 +310,7 @@ int gcq_paged_attn(const gcq_paged_cache * cache, const gcq_paged_batch * batch,
         require(window >= 0, "paged_attn: window must not be negative");
         require(std::isfinite(scale), "paged_attn: scale must be finite");
         const size_t need_ws = std::max<size_t>(256, paged_attn_workspace(p, cache->head_dim, n_head, max_rows));
-        require(ws_size >= need_ws, "workspace of " + std::to_string(ws_size) + " bytes, need " + std::to_string(need_ws));
+        if (ws_size < need_ws) fail("workspace of " + std::to_string(ws_size) + " bytes, need " + std::to_string(need_ws));
         launch_paged_attn(p, cache->head_dim, q, q_r, q_h, n_head, max_rows, window, scale, out, ws, as_stream(stream));
     });
 }

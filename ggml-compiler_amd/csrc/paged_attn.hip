@@ -679,7 +679,7 @@ void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int6
     a.negate = scale < 0.0f;
     a.out = out;
     const Shape w = shape_for(p, D, a.G, max_rows);
-    require(w.items < INT32_MAX, "paged_attn: too many rows and heads");
+    if (w.items >= INT32_MAX) fail("paged_attn: too many rows and heads");
     a.items = (int) w.items, a.target = w.target;
     a.min_chunk = w.most == 1 ? 1 << 30 : kMinChunk;
     a.part_o = (float *) ws;

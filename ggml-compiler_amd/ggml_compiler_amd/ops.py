@@ -243,7 +243,7 @@ def flash_attn_ext(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torc
 # ------------------------------------------------------------------ paged 4-bit key / value cache
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class PagedCache:
     """One layer's keys and values in n_pages pages of page_size tokens, held as Q4_0 blocks (include/gcq_paged.h).
     page_size 32, 64, 128 or 256; head dim D 64, 128 or 256."""
@@ -253,7 +253,6 @@ class PagedCache:
     Hkv: int
     D: int
     data: torch.Tensor  # uint8, gcq_paged_cache_size bytes
-    _c: _lib.PagedCache = field(init=False, repr=False, compare=False)
 
     def __post_init__(self) -> None:
         n = int(load().gcq_paged_cache_size(self.n_pages, self.page_size, self.Hkv, self.D))
@@ -262,8 +261,7 @@ class PagedCache:
         _cuda(self.data, torch.uint8, "data")
         if self.data.numel() != n or not self.data.is_contiguous():
             raise ValueError(f"data must be {n} contiguous bytes, got {self.data.numel()}")
-        self._c = _lib.PagedCache(self.data.data_ptr(), self.n_pages, self.page_size, self.Hkv, self.D)
-        self._at = ctypes.addressof(self._c)
+        _paged_handle(self, _lib.PagedCache(self.data.data_ptr(), self.n_pages, self.page_size, self.Hkv, self.D), self.data)
 
     @classmethod
     def new(cls, n_pages: int, page_size: int, Hkv: int, D: int, device=None) -> "PagedCache":
@@ -273,7 +271,7 @@ class PagedCache:
         return cls(n_pages, page_size, Hkv, D, torch.zeros(n, dtype=torch.uint8, device=device or "cuda"))
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class PagedBatch:
     """Sequences and their new rows, packed: sequence s owns rows starts[s] .. starts[s + 1] - 1, the first of them at
     position past[s]; position p lives in page pages[s, p // page_size]. int32 on the device: pages [S, max_pages] (an
@@ -283,7 +281,6 @@ class PagedBatch:
     pages: torch.Tensor
     starts: torch.Tensor
     past: torch.Tensor
-    _c: _lib.PagedBatch = field(init=False, repr=False, compare=False)
 
     def __post_init__(self) -> None:
         for name in ("pages", "starts", "past"):
@@ -296,35 +293,52 @@ class PagedBatch:
                              f"{tuple(self.past.shape)}")
         if not self.starts.is_contiguous() or not self.past.is_contiguous():
             raise ValueError("starts and past must be contiguous")
-        self._c = _lib.PagedBatch(self.pages.data_ptr(), max(self.pages.stride(0), n), self.starts.data_ptr(),
-                                  self.past.data_ptr(), S, n)
-        self._at = ctypes.addressof(self._c)
+        if self.starts.get_device() != self.pages.get_device() or self.past.get_device() != self.pages.get_device():
+            raise ValueError("pages, starts and past must be on one device")
+        _paged_handle(self, _lib.PagedBatch(self.pages.data_ptr(), max(self.pages.stride(0), n), self.starts.data_ptr(),
+                                            self.past.data_ptr(), S, n), self.pages)
 
 
-def _paged(cache: PagedCache, batch: PagedBatch, *rest: torch.Tensor) -> None:
-    """All on the current device, whose current stream takes the launch."""
-    d = torch.cuda.current_device()
-    for t in (cache.data, batch.pages, batch.starts, batch.past, *rest):
-        if t.get_device() != d:
-            raise ValueError(f"a tensor on {t.device}, the current device is {d}")
+def _paged_handle(x: PagedCache | PagedBatch, c: ctypes.Structure, on: torch.Tensor) -> None:
+    """What every call needs of x: the C structure's address and the device."""
+    for name, value in (("_c", c), ("_at", ctypes.addressof(c)), ("_device", on.get_device())):
+        object.__setattr__(x, name, value)
 
 
-def _paged_rows(x: torch.Tensor, dtype: torch.dtype, name: str, n: int, heads: int, D: int) -> torch.Tensor:
-    _cuda(x, dtype, name)
-    if x.dim() != 3 or x.shape[0] != n or x.shape[1] != heads or x.shape[2] != D:
-        raise ValueError(f"{name} must be [{n}, {heads}, {D}], got {tuple(x.shape)}")
-    if x.stride(2) != 1:
-        raise ValueError(f"{name} needs a unit stride along the head dim")
-    return x
+def _paged_device(cache: PagedCache, batch: PagedBatch) -> int:
+    """The device of all operands: the current one, whose current stream takes the launch."""
+    d = torch._C._cuda_getDevice()
+    if cache._device != d or batch._device != d:
+        raise ValueError(f"cache on device {cache._device}, batch on {batch._device}, the current device is {d}")
+    return d
 
 
-def _paged_out(out: torch.Tensor | None, shape, dtype: torch.dtype, device, name: str) -> torch.Tensor:
+def _paged_rows(x: torch.Tensor, dtype: torch.dtype, name: str, shape: tuple, d: int) -> tuple[int, int]:
+    """x's strides, checked. (One test on the way through: these wrappers cost as much as a single token's kernels.)"""
+    s = x.stride()
+    if x.dtype != dtype or x.shape != shape or s[2] != 1 or x.get_device() != d:
+        _cuda(x, dtype, name)
+        if x.shape != shape:
+            raise ValueError(f"{name} must be {list(shape)}, got {list(x.shape)}")
+        if s[2] != 1:
+            raise ValueError(f"{name} needs a unit stride along the head dim")
+        raise ValueError(f"{name} on {x.device}, the current device is {d}")
+    return s[0], s[1]
+
+
+def _paged_out(out: torch.Tensor | None, shape: tuple, dtype: torch.dtype, name: str, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
     _cuda(out, dtype, name)
-    if tuple(out.shape) != tuple(shape) or not out.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {tuple(shape)}, got {tuple(out.shape)}")
+    if out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {list(shape)}, got {list(out.shape)}")
+    if out.get_device() != like.get_device():
+        raise ValueError(f"{name} on {out.device}, not on {like.device}")
     return out
+
+
+def _heads(x: torch.Tensor) -> int:
+    return x.shape[1] if x.dim() == 3 else 0
 
 
 def rope_freqs(n_dims: int, base: float, freq_scale: float = 1.0, ff: torch.Tensor | None = None,
@@ -343,27 +357,24 @@ def paged_append(cache: PagedCache, batch: PagedBatch, k: torch.Tensor, v: torch
     """Rows k, v f32 [n, Hkv, D] (strided allowed, unit inner stride) into the cache as Q4_0, the keys' NEOX pairs
     (i, i + len(freqs)) turned by position * freqs[i] (freqs None: unrotated). q f32 [n, H, D]: turned alike and
     returned as f16 [n, H, D], paged_attn's input (q_out: into it; rows of no sequence stay as they are)."""
-    n, Hkv, D = k.shape[0], cache.Hkv, cache.D
-    _paged_rows(k, torch.float32, "k", n, Hkv, D)
-    _paged_rows(v, torch.float32, "v", n, Hkv, D)
-    rest, H = [k, v], 0
+    d, n = _paged_device(cache, batch), k.shape[0]
+    kv = (n, cache.Hkv, cache.D)
+    ks, vs = _paged_rows(k, torch.float32, "k", kv, d), _paged_rows(v, torch.float32, "v", kv, d)
+    H, q_at, out_at, qs, f_at, n_dims = 0, None, None, (0, 0), None, 0
     if q is not None:
-        H = q.shape[1] if q.dim() == 3 else 0
-        _paged_rows(q, torch.float32, "q", n, H, D)
-        q_out = _paged_out(q_out, (n, H, D), torch.float16, q.device, "q_out")
-        rest += [q, q_out]
+        H = _heads(q)
+        shape = (n, H, cache.D)
+        qs = _paged_rows(q, torch.float32, "q", shape, d)
+        q_out = _paged_out(q_out, shape, torch.float16, "q_out", q)
+        q_at, out_at = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
     if freqs is not None:
-        _cuda(freqs, torch.float32, "freqs")
-        if freqs.dim() != 1 or not freqs.is_contiguous():
-            raise ValueError("freqs must be contiguous, one value for each pair")
-        rest.append(freqs)
-    _paged(cache, batch, *rest)
-    sq = (0, 0) if q is None else q.stride()
-    check(load().gcq_paged_append(cache._at, batch._at, n, _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
-                                  v.stride(1), _p(q), sq[0], sq[1], H, _p(q_out), _p(freqs),
-                                  0 if freqs is None else 2 * freqs.numel(), float(attn_factor), _stream()))
+        if freqs.dtype != torch.float32 or freqs.get_device() != d or freqs.dim() != 1 or not freqs.is_contiguous():
+            raise ValueError("freqs must be contiguous f32 on the rows' device, one value for each pair")
+        f_at, n_dims = freqs.data_ptr(), 2 * freqs.numel()
+    check(load().gcq_paged_append(cache._at, batch._at, n, k.data_ptr(), *ks, v.data_ptr(), *vs, q_at, *qs, H, out_at,
+                                  f_at, n_dims, attn_factor, torch._C._cuda_getCurrentRawStream(d)))
     return q_out
 
 
@@ -371,11 +382,11 @@ def paged_read(cache: PagedCache, batch: PagedBatch, n: int, k: torch.Tensor | N
                v: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """What the cache holds for the batch's n rows: k, v f32 [n, Hkv, D] (zeros for tokens that are not there; into
     k, v if given; rows of no sequence stay as they are)."""
-    shape = (n, cache.Hkv, cache.D)
-    k = _paged_out(k, shape, torch.float32, cache.data.device, "k")
-    v = _paged_out(v, shape, torch.float32, cache.data.device, "v")
-    _paged(cache, batch, k, v)
-    check(load().gcq_paged_read(cache._at, batch._at, n, _p(k), _p(v), _stream()))
+    d, shape = _paged_device(cache, batch), (n, cache.Hkv, cache.D)
+    k = _paged_out(k, shape, torch.float32, "k", cache.data)
+    v = _paged_out(v, shape, torch.float32, "v", cache.data)
+    check(load().gcq_paged_read(cache._at, batch._at, n, k.data_ptr(), v.data_ptr(),
+                                torch._C._cuda_getCurrentRawStream(d)))
     return k, v
 
 
@@ -385,18 +396,18 @@ def paged_attn(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, scale: flo
     `window` of them if window > 0. q f16 [n, H, D] (strides multiples of 8, unit inner stride) -> f32 [n, H, D] (into
     out if given; rows of no sequence stay as they are; a row that sees no token gives zeros). max_rows: no sequence
     has more rows than this (default n); 1 for a decode step."""
-    n, H = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-    _paged_rows(q, torch.float16, "q", n, H, cache.D)
-    out = _paged_out(out, (n, H, cache.D), torch.float32, q.device, "out")
-    _paged(cache, batch, q, out)
-    max_rows = max(n, 1) if max_rows is None else int(max_rows)
+    d, n, H = _paged_device(cache, batch), q.shape[0], _heads(q)
+    shape = (n, H, cache.D)
+    qs = _paged_rows(q, torch.float16, "q", shape, d)
+    out = _paged_out(out, shape, torch.float32, "out", q)
+    max_rows = max(n, 1) if max_rows is None else max_rows
     lib = load()
-    ws_n = int(lib.gcq_paged_attn_workspace(cache._at, batch._at, n, H, max_rows))
+    ws_n = lib.gcq_paged_attn_workspace(cache._at, batch._at, n, H, max_rows)
     if ws_n == 0:
         raise _lib.error()
-    ws = workspace(ws_n, q.device)
-    check(lib.gcq_paged_attn(cache._at, batch._at, n, _p(q), q.stride(0), q.stride(1), H, max_rows, int(window),
-                             float(scale), _p(out), _p(ws), ws.numel(), _stream()))
+    ws = cache.data.new_empty(ws_n)
+    check(lib.gcq_paged_attn(cache._at, batch._at, n, q.data_ptr(), *qs, H, max_rows, window, scale, out.data_ptr(),
+                             ws.data_ptr(), ws_n, torch._C._cuda_getCurrentRawStream(d)))
     return out
 
 
