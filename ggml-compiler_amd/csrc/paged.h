@@ -43,6 +43,50 @@ __device__ __forceinline__ int64_t paged_tile(const Paged & a, int s, int64_t po
     return ((((int64_t) e * a.Hkv + h) << (a.shift - 5)) + ((pos & ((1 << a.shift) - 1)) >> 5)) * (36 * D);
 }
 
+// Inclusive prefix sum over the wavefront.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15 into the next row, then 31 into the upper half
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
+// Tile `id` of those that the batch's new rows touch, a sequence's after the one's before: the sequence, its rows and the tile's
+// number in it (uniform; all lanes together).
+struct PagedSpan {
+    int s, r0, rows;
+    int64_t past, tile;
+};
+__device__ __forceinline__ bool paged_find(const Paged & a, int id, PagedSpan & w) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+        int r0 = 0, rows = 0, past = 0, n = 0;
+        if (s0 + lane < a.n_seq) {
+            r0 = a.starts[s0 + lane];
+            rows = r0 < 0 ? 0 : max(min(a.starts[s0 + lane + 1], a.n_rows) - r0, 0);
+            past = a.past[s0 + lane];
+            n = rows ? (int) ((((int64_t) past + rows - 1) >> 5) - (past >> 5)) + 1 : 0;
+        }
+        const int sum = wave_scan(n);
+        const uint64_t at = __ballot(base + sum > id);
+        if (at) {
+            const int l = __builtin_ctzll(at);
+            w.s = s0 + l;
+            w.r0 = __builtin_amdgcn_readlane(r0, l);
+            w.rows = __builtin_amdgcn_readlane(rows, l);
+            w.past = __builtin_amdgcn_readlane(past, l);
+            w.tile = (w.past >> 5) + id - base - __builtin_amdgcn_readlane(sum - n, l);
+            return true;
+        }
+        base += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
 // Within a tile: code byte i of token slot t, and the f16 scale of block b (byte offsets).
 template <int D> __device__ __forceinline__ int paged_k_byte(int t, int i) {
     return t * (D / 2) + (i >> 3 & 3) * (D / 8) + (i >> 5) * 8 + (i & 7);

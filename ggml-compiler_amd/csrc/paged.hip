@@ -11,6 +11,8 @@ namespace gcq {
 
 namespace {
 
+constexpr int kTileRows = 8;
+
 struct AppendArgs {
     Paged p;
     const float * k, * v, * q;
@@ -22,6 +24,20 @@ struct AppendArgs {
 };
 
 // ---------------------------------------------------------------------------------- append
+
+// One element of a turned pair: x c + p s, p its partner (s negated for the pair's first).
+__device__ __forceinline__ float turned(float x, double c, float p, double s) { return (float) fma((double) x, c, (double) p * s); }
+
+// What is held of a value: NaN as 0, the rest within f16.
+__device__ __forceinline__ float held(float w) { return w == w ? fminf(fmaxf(w, -kPagedMax), kPagedMax) : 0.0f; }
+
+// A block's scale from its largest value (ggml's Q4_0: the first of the largest becomes code 0), and a value's code.
+__device__ __forceinline__ float block_scale(float m, bool minus) { return (minus ? m : -m) * 0.125f; }
+__device__ __forceinline__ float block_inverse(float d) { return d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f; }
+__device__ __forceinline__ int code_of(float w, float inverse) {
+#pragma clang fp contract(off)
+    return max(min((int) (w * inverse + 8.5f), 15), 0);
+}
 
 // A wavefront takes `per` heads of one row. Lane i holds dims i and i + D / 2 (D = 64: a head per half wavefront; 256: two
 // such pairs), so a NEOX pair, a code byte and, per register and half wavefront, a whole block are at hand without an
@@ -71,15 +87,15 @@ __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
             y[n][1] = on ? x[i + D / 2] : 0.0f;
             if (turn && (is_q || is_k) && on) {
                 if constexpr (FULL) {
-                    const double u = y[n][0], w = y[n][1];
-                    y[n][0] = (float) (u * cs[n] - w * sn[n]);
-                    y[n][1] = (float) (u * sn[n] + w * cs[n]);
+                    const float u = y[n][0], w = y[n][1];
+                    y[n][0] = turned(u, cs[n], w, -sn[n]);
+                    y[n][1] = turned(w, cs[n], u, sn[n]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int d = i + e * (D / 2), c = 2 * n + e;
-                        if (d < half) y[n][e] = (float) ((double) y[n][e] * cs[c] - (double) x[d + half] * sn[c]);
-                        else if (d < a.n_dims) y[n][e] = (float) ((double) x[d - half] * sn[c] + (double) y[n][e] * cs[c]);
+                        if (d < half) y[n][e] = turned(y[n][e], cs[c], x[d + half], -sn[c]);
+                        else if (d < a.n_dims) y[n][e] = turned(y[n][e], cs[c], x[d - half], sn[c]);
                     }
                 }
             }
@@ -96,20 +112,17 @@ __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
         const int64_t tile = on && !is_q ? paged_tile(a.p, s, pos, hk, D) : -1;
 #pragma unroll
         for (int n = 0; n < NP; n++) {
-#pragma clang fp contract(off)
             int code[2];
             float d[2];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                float w = y[n][e];
-                w = w == w ? fminf(fmaxf(w, -kPagedMax), kPagedMax) : 0.0f;
+                const float w = held(y[n][e]);
                 const float m = wave_max<32>(fabsf(w));
                 const uint64_t at = __ballot(fabsf(w) == m), neg = __ballot(w < 0.0f);
                 const uint32_t at32 = (uint32_t) (lane < 32 ? at : at >> 32), neg32 = (uint32_t) (lane < 32 ? neg : neg >> 32);
                 const bool minus = neg32 >> __builtin_ctz(at32) & 1;  // the first of the largest
-                d[e] = (minus ? m : -m) * 0.125f;
-                const float id = d[e] != 0.0f ? __fdiv_rn(1.0f, d[e]) : 0.0f;
-                code[e] = max(min((int) (w * id + 8.5f), 15), 0);
+                d[e] = block_scale(m, minus);
+                code[e] = code_of(w, block_inverse(d[e]));
             }
             if (tile >= 0) {
                 const int i = il + 64 * n;
@@ -123,6 +136,151 @@ __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
                     }
             }
         }
+    }
+}
+
+// Many rows of a sequence: a workgroup takes one tile of the cache (32 positions) for one KV head, and the tile's rows of q
+// heads hk, hk + Hkv, .. A thread has four pairs of one row for all of those heads, their sines in registers; the tile is put
+// together in LDS and leaves as 16-byte pieces, where a row at a time writes V's bytes one by one.
+template <int D, bool FULL>
+__global__ __launch_bounds__(4 * D) void k_paged_append_tile(const AppendArgs a) {
+    constexpr int L = D / 8, QB = FULL ? 4 : 1;  // threads of a row; q heads under way at a time, as the registers allow
+    __shared__ __align__(16) uint8_t image[36 * D];
+    const int tid = threadIdx.x, lane = tid & 63, slot = tid / L, i = 4 * (tid % L), hk = blockIdx.x % a.p.Hkv;
+    PagedSpan w;
+    if (!paged_find(a.p, blockIdx.x / a.p.Hkv, w)) return;
+    const int64_t pos = w.tile * 32 + slot, j = pos - w.past;
+    const bool on = j >= 0 && j < w.rows;
+    const int64_t r = w.r0 + (on ? j : 0);
+    const int half = a.n_dims / 2;
+
+    // of dims i .. i + 3 and i + D / 2 ..: values, and partners (FULL: each other)
+    typedef float f4_t __attribute__((ext_vector_type(4)));
+    struct Four {
+        f4_t x[2], p[FULL ? 1 : 2];
+    };
+    const auto fetch = [&](const float * x, bool turn) {
+        Four f{};
+        if (!on) return f;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int d = i + e * (D / 2);
+            f.x[e] = *reinterpret_cast<const f4_t *>(x + d);
+            if constexpr (!FULL)
+                if (turn && d < a.n_dims) f.p[e] = *reinterpret_cast<const f4_t *>(x + (d < half ? d + half : d - half));
+        }
+        return f;
+    };
+    const auto q_at = [&](int h) { return a.q + r * a.q_r + min(h, a.H - 1) * a.q_h; };
+    Four k = fetch(a.k + r * a.k_r + hk * a.k_h, true), v = fetch(a.v + r * a.v_r + hk * a.v_h, false), q[QB];
+    if (a.q)
+#pragma unroll
+        for (int n = 0; n < QB; n++) q[n] = fetch(q_at(hk + n * a.p.Hkv), true);
+
+    constexpr int NC = FULL ? 1 : 2;
+    double cs[NC][4], sn[NC][4];
+    if (a.freqs) {
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int d = i + e + c * (D / 2);
+                cs[c][e] = 1.0;
+                sn[c][e] = 0.0;
+                if (FULL || d < a.n_dims) {
+                    sincos((double) pos * (double) a.freqs[!FULL && d >= half ? d - half : d], &sn[c][e], &cs[c][e]);
+                    cs[c][e] *= (double) a.attn_factor;
+                    sn[c][e] *= !FULL && d < half ? -(double) a.attn_factor : (double) a.attn_factor;
+                }
+            }
+    }
+    const auto turn = [&](Four & f) {
+        if (!a.freqs) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float x0 = f.x[0][e], x1 = f.x[1][e];
+            if (FULL || i < a.n_dims) f.x[0][e] = FULL ? turned(x0, cs[0][e], x1, -sn[0][e]) : turned(x0, cs[0][e], f.p[0][e], sn[0][e]);
+            if (FULL || i + D / 2 < a.n_dims) f.x[1][e] = FULL ? turned(x1, cs[0][e], x0, sn[0][e]) : turned(x1, cs[NC - 1][e], f.p[FULL ? 0 : 1][e], sn[NC - 1][e]);
+        }
+    };
+    const int64_t tile = paged_tile(a.p, w.s, w.tile * 32, hk, D);  // (-1 for all of its positions or none)
+    turn(k);
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        int code[2][4];
+        float d[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            f4_t y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = held((c ? v : k).x[h][e]);
+            float m = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+            m = fmaxf(m, lane_pair<1>(m));  // over the block's 8 lanes
+            m = fmaxf(m, lane_pair<2>(m));
+            m = fmaxf(m, lane_pair<4>(m));
+            bool at = false, neg = false;  // the first of the largest
+#pragma unroll
+            for (int e = 3; e >= 0; e--)
+                if (fabsf(y[e]) == m) at = true, neg = y[e] < 0.0f;
+            const uint32_t ats = (uint32_t) (__ballot(at) >> (lane & 56)) & 255, negs = (uint32_t) (__ballot(neg) >> (lane & 56));
+            d[h] = block_scale(m, negs >> __builtin_ctz(ats) & 1);
+            const float id = block_inverse(d[h]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) code[h][e] = code_of(y[e], id);
+        }
+        if (c == 0) {
+            uint32_t bytes = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) bytes |= (uint32_t) (code[0][e] | code[1][e] << 4) << (8 * e);
+            *reinterpret_cast<uint32_t *>(image + paged_k_byte<D>(slot, i)) = bytes;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) image[paged_v_byte<D>(slot, i + e)] = (uint8_t) (code[0][e] | code[1][e] << 4);
+        }
+        if ((lane & 7) == 0)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int b = i / 32 + h * (D / 64);
+                *reinterpret_cast<uint16_t *>(image + (c ? paged_v_scale<D>(slot, b) : paged_k_scale<D>(slot, b))) = f2h_exact(d[h]);
+            }
+    }
+    if (a.q) {
+        typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+        for (int h0 = hk; h0 < a.H; h0 += QB * a.p.Hkv) {
+            if (h0 != hk)
+#pragma unroll
+                for (int n = 0; n < QB; n++) q[n] = fetch(q_at(h0 + n * a.p.Hkv), true);
+#pragma unroll
+            for (int n = 0; n < QB; n++) {
+                const int h = h0 + n * a.p.Hkv;
+                if (h >= a.H || !on) break;
+                turn(q[n]);
+                _Float16 * o = a.q_out + (r * a.H + h) * D + i;
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const f4_t y = q[n].x[e];
+                    const h4_t u = {(_Float16) y[0], (_Float16) y[1], (_Float16) y[2], (_Float16) y[3]};
+                    __builtin_memcpy(o + e * (D / 2), &u, 8);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (tile < 0 || tid >= 36 * D / 16) return;
+    // the tile's 16-byte pieces; in part where some of their tokens are not this batch's
+    const int64_t s0 = w.past - w.tile * 32, s1 = s0 + w.rows;
+    const uint32_t have = (s1 >= 32 ? ~0u : (1u << s1) - 1) & (s0 > 0 ? ~0u << s0 : ~0u);
+    uint8_t * o = a.p.data + tile + 16 * tid;
+    const uint8_t * from = image + 16 * tid;
+    const bool codes = tid < 2 * D;
+    const uint32_t m = tid < D ? (have >> tid / (D / 32) & 1) * 255 : have >> (codes ? tid >> 4 & 3 : tid & 3) * 8 & 255;
+    if (m == 255) *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<const uint4 *>(from);
+    else if (codes) {
+        for (int b = 0; b < 16; b++)
+            if (m >> (b & 7) & 1) o[b] = from[b];
+    } else {
+        for (int e = 0; e < 8; e++)
+            if (m >> paged_order(e) & 1) *reinterpret_cast<uint16_t *>(o + 2 * e) = *reinterpret_cast<const uint16_t *>(from + 2 * e);
     }
 }
 
@@ -160,6 +318,43 @@ __global__ __launch_bounds__(256) void k_paged_read(const ReadArgs a) {
             o[i] = lo;
             o[i + D / 2] = hi;
         }
+    }
+}
+
+// Many rows: a workgroup takes one tile for one KV head, by way of LDS; a thread gives four pairs of one row.
+template <int D>
+__global__ __launch_bounds__(4 * D) void k_paged_read_tile(const ReadArgs a) {
+    constexpr int L = D / 8;
+    __shared__ __align__(16) uint8_t image[36 * D];
+    const int tid = threadIdx.x, slot = tid / L, i = 4 * (tid % L), hk = blockIdx.x % a.p.Hkv;
+    PagedSpan w;
+    if (!paged_find(a.p, blockIdx.x / a.p.Hkv, w)) return;
+    const int64_t tile = paged_tile(a.p, w.s, w.tile * 32, hk, D);
+    if (tile >= 0 && tid < 36 * D / 16) *reinterpret_cast<uint4 *>(image + 16 * tid) = *reinterpret_cast<const uint4 *>(a.p.data + tile + 16 * tid);
+    __syncthreads();
+    const int64_t j = w.tile * 32 + slot - w.past;
+    if (j < 0 || j >= w.rows) return;
+    typedef float f4_t __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        f4_t y[2] = {};
+        if (tile >= 0) {
+            uint32_t b = 0;
+            if (c == 0) b = *reinterpret_cast<const uint32_t *>(image + paged_k_byte<D>(slot, i));
+            else
+#pragma unroll
+                for (int e = 0; e < 4; e++) b |= (uint32_t) image[paged_v_byte<D>(slot, i + e)] << (8 * e);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int blk = i / 32 + h * (D / 64);
+                const float d = h2f(*reinterpret_cast<const uint16_t *>(image + (c ? paged_v_scale<D>(slot, blk) : paged_k_scale<D>(slot, blk))));
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[h][e] = d * (float) ((int) (b >> (8 * e + 4 * h) & 15) - 8);
+            }
+        }
+        float * o = (c ? a.v : a.k) + ((w.r0 + j) * a.p.Hkv + hk) * D + i;
+        *reinterpret_cast<f4_t *>(o) = y[0];
+        *reinterpret_cast<f4_t *>(o + D / 2) = y[1];
     }
 }
 
@@ -206,11 +401,32 @@ unsigned blocks(int64_t waves) {
     return (unsigned) ((waves + 3) / 4);
 }
 
+// Whether rows are taken a tile at a time: a sequence has some of a tile's 32 at the least, on average.
+bool by_tiles(const Paged & p) { return p.n_rows >= kTileRows * std::min(p.n_seq, p.n_rows); }
+unsigned tile_blocks(const Paged & p) {  // a sequence's rows may begin and end inside a tile
+    const int64_t n = (p.n_rows / kPagedTile + 2 * (int64_t) std::min(p.n_seq, p.n_rows)) * p.Hkv;
+    require(n <= INT32_MAX, "paged: too many rows and heads");
+    return (unsigned) n;
+}
+bool vectors(const float * x, int64_t r, int64_t h) { return aligned(x, 16) && r % 4 == 0 && h % 4 == 0; }
+
 template <int D>
 void run_append(const AppendArgs & a, hipStream_t s) {
+    const bool full = !a.freqs || a.n_dims == D;
+    if (by_tiles(a.p) && a.n_dims % 8 == 0 && vectors(a.k, a.k_r, a.k_h) && vectors(a.v, a.v_r, a.v_h) &&
+        (!a.q || (vectors(a.q, a.q_r, a.q_h) && aligned(a.q_out, 8)))) {
+        if (full) k_paged_append_tile<D, true><<<tile_blocks(a.p), 4 * D, 0, s>>>(a);
+        else k_paged_append_tile<D, false><<<tile_blocks(a.p), 4 * D, 0, s>>>(a);
+        return;
+    }
     const unsigned grid = blocks((int64_t) a.p.n_rows * a.parts);
-    if (!a.freqs || a.n_dims == D) k_paged_append<D, true><<<grid, 256, 0, s>>>(a);
+    if (full) k_paged_append<D, true><<<grid, 256, 0, s>>>(a);
     else k_paged_append<D, false><<<grid, 256, 0, s>>>(a);
+}
+template <int D>
+void run_read(const ReadArgs & a, hipStream_t s) {
+    if (by_tiles(a.p) && aligned(a.k, 16) && aligned(a.v, 16)) k_paged_read_tile<D><<<tile_blocks(a.p), 4 * D, 0, s>>>(a);
+    else k_paged_read<D><<<blocks((int64_t) a.p.n_rows * a.p.Hkv), 256, 0, s>>>(a);
 }
 
 }  // namespace
@@ -275,10 +491,9 @@ int gcq_paged_read(const gcq_paged_cache * cache, const gcq_paged_batch * batch,
         need(k, "k", 4);
         need(v, "v", 4);
         hipStream_t s = as_stream(stream);
-        const unsigned grid = blocks(n_rows * a.p.Hkv);
-        if (cache->head_dim == 64) k_paged_read<64><<<grid, 256, 0, s>>>(a);
-        else if (cache->head_dim == 128) k_paged_read<128><<<grid, 256, 0, s>>>(a);
-        else k_paged_read<256><<<grid, 256, 0, s>>>(a);
+        if (cache->head_dim == 64) run_read<64>(a, s);
+        else if (cache->head_dim == 128) run_read<128>(a, s);
+        else run_read<256>(a, s);
         check_launch("paged read");
     });
 }

@@ -74,17 +74,6 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs & a, int s) {
 }
 __device__ __forceinline__ int splits(int tiles, int chunk) { return max(1, (tiles + chunk - 1) / chunk); }
 
-// Inclusive prefix sum over the wavefront.
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15 into the next row, then 31 into the upper half
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
-
 // The plan, the same in every wavefront: tiles per split, and a sequence's first item. Items of a sequence: [KV
 // head][row tile, the last, which sees most, first][split]. The batch's arrays are read once where the sequences fit the lanes.
 template <int ROWS>

@@ -545,3 +545,66 @@ def test_refusals_on_the_device(gops):
         gops.paged_attn(cache, batch, q, 0.1, out=torch.zeros((4, 4, 128), device="cuda")[..., ::2])
     assert gops.paged_attn(cache, batch, q[:0], 0.1).shape == (0, 4, 64)
     assert gops.paged_read(cache, batch, 0)[0].shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("D,n_dims,H,Hkv", [(64, 64, 9, 3), (128, 128, 3, 4), (128, 72, 24, 2), (256, 256, 10, 2), (256, 64, 4, 1)])
+@pytest.mark.parametrize("rows,past", [([8], [0]), ([8, 9], [28, 31]), ([7, 9], [1, 2]), ([32, 64, 1, 31], [0, 32, 95, 33]),
+                                       ([3, 200, 0, 95], [62, 33, 4, 1])])
+def test_rows_by_tiles_equal_rows_one_by_one(gops, D, n_dims, H, Hkv, rows, past):
+    """A call that goes a tile at a time and calls of a few rows each (strides that no 16-byte load takes among them) leave
+    the same bytes, queries and rows read back; the rest of the pool stays as it is."""
+    c = Case(gops, rows, past, Hkv, D, 64, seed=31, extra_rows=2, fill=0xA5)
+    x = torch.from_numpy(c.rng.standard_normal((c.n, H + 2 * Hkv, D)).astype(np.float32)).cuda()
+    freqs = gops.rope_freqs(n_dims, 10000.0)
+    odd = torch.zeros((c.n, H + 2 * Hkv, D + 1), device="cuda")
+    odd[..., :D] = x
+    q, k, v = x[:, :H], x[:, H:H + Hkv], x[:, H + Hkv:]
+    q16 = torch.full((c.n, H, D), 5.0, dtype=torch.float16, device="cuda")
+    gops.paged_append(c.cache, c.batch(), k, v, q=q, freqs=freqs, q_out=q16)
+    once = c.cache.data.clone()
+    c.cache.data.fill_(0xA5)
+    o16 = torch.full_like(q16, 5.0)
+    gops.paged_append(c.cache, c.batch(), odd[:, H:H + Hkv, :D], odd[:, H + Hkv:, :D], q=odd[:, :H, :D], freqs=freqs, q_out=o16)
+    assert torch.equal(once, c.cache.data) and torch.equal(q16, o16)
+    c.cache.data.fill_(0xA5)
+    b = c.batch()
+    got_k, got_v = gops.paged_read(gops.PagedCache(c.n_pages, 64, Hkv, D, once), b, c.n, *(torch.full_like(k, 3.0) for _ in range(2)))
+    for s, (r, p) in enumerate(zip(rows, past)):
+        for j in range(0, r, 5):
+            m, at = min(5, r - j), int(c.starts[s]) + j
+            one = gops.PagedBatch(b.pages[s:s + 1], torch.tensor([0, m], dtype=torch.int32).cuda(),
+                                  torch.tensor([p + j], dtype=torch.int32).cuda())
+            few = gops.paged_append(c.cache, one, k[at:at + m], v[at:at + m], q=q[at:at + m], freqs=freqs)
+            assert torch.equal(few, q16[at:at + m])
+            for y, w in zip(gops.paged_read(c.cache, one, m), (got_k, got_v)):
+                assert torch.equal(y, w[at:at + m])
+    assert torch.equal(once, c.cache.data)
+    assert (got_k[-2:] == 3.0).all() and (got_v[-2:] == 3.0).all() and (q16[-2:] == 5.0).all()
+
+
+def test_append_by_tiles_special_values(gops):
+    """Ties of either sign, zeros of either sign, NaNs, infinities and subnormal scales: a tile at a time as one by one."""
+    D = 64
+    x = torch.zeros((32, 1, D), device="cuda")
+    x[1, 0, 5], x[1, 0, 9] = -2.0, 2.0
+    x[2, 0, 5], x[2, 0, 9] = 2.0, -2.0
+    x[3, 0, 31], x[3, 0, 32], x[3, 0, 63] = 1.0, -1.0, 1.0
+    x[4] = -0.0
+    x[5, 0, 3], x[5, 0, 40] = float("nan"), float("nan")
+    x[6, 0, 3], x[6, 0, 4], x[6, 0, 40] = float("inf"), 1.0, -float("inf")
+    x[7] = 3e-7
+    x[8, 0, ::3] = 1e-40
+    x[9] = 3e38
+    x[10, 0, :4], x[10, 0, 4:8] = 1.0, -1.0
+    x[11, 0, 3], x[11, 0, 4] = -1.0, 1.0
+    x[12, 0, 7], x[12, 0, 8] = 1.0, -1.0
+    i32 = dict(dtype=torch.int32, device="cuda")
+    a, b = (gops.PagedCache.new(1, 32, 1, D) for _ in range(2))
+    page = torch.zeros((1, 1), **i32)
+    whole = gops.PagedBatch(page, torch.tensor([0, 32], **i32), torch.tensor([0], **i32))
+    q = gops.paged_append(a, whole, x, x, q=x)
+    for r in range(32):
+        one = gops.PagedBatch(page, torch.tensor([0, 1], **i32), torch.tensor([r], **i32))
+        o = gops.paged_append(b, one, x[r:r + 1], x[r:r + 1], q=x[r:r + 1])
+        assert torch.equal(o.view(torch.int16), q[r:r + 1].view(torch.int16))
+    assert torch.equal(a.data, b.data)
