@@ -54,11 +54,11 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
-// Tile `id` of those that the batch's new rows touch, a sequence's after the one's before: the sequence, its rows and the tile's
-// number in it (uniform; all lanes together).
+// Eight `id` (8 positions, a quarter of a tile) of those that the batch's new rows touch, a sequence's after the one's before:
+// the sequence, its rows and the eight's number in it (uniform; all lanes together).
 struct PagedSpan {
     int s, r0, rows;
-    int64_t past, tile;
+    int64_t past, eight;
 };
 __device__ __forceinline__ bool paged_find(const Paged & a, int id, PagedSpan & w) {
     const int lane = threadIdx.x & 63;
@@ -69,7 +69,7 @@ __device__ __forceinline__ bool paged_find(const Paged & a, int id, PagedSpan & 
             r0 = a.starts[s0 + lane];
             rows = r0 < 0 ? 0 : max(min(a.starts[s0 + lane + 1], a.n_rows) - r0, 0);
             past = a.past[s0 + lane];
-            n = rows ? (int) ((((int64_t) past + rows - 1) >> 5) - (past >> 5)) + 1 : 0;
+            n = rows ? (int) ((((int64_t) past + rows - 1) >> 3) - (past >> 3)) + 1 : 0;
         }
         const int sum = wave_scan(n);
         const uint64_t at = __ballot(base + sum > id);
@@ -79,7 +79,7 @@ __device__ __forceinline__ bool paged_find(const Paged & a, int id, PagedSpan & 
             w.r0 = __builtin_amdgcn_readlane(r0, l);
             w.rows = __builtin_amdgcn_readlane(rows, l);
             w.past = __builtin_amdgcn_readlane(past, l);
-            w.tile = (w.past >> 5) + id - base - __builtin_amdgcn_readlane(sum - n, l);
+            w.eight = (w.past >> 3) + id - base - __builtin_amdgcn_readlane(sum - n, l);
             return true;
         }
         base += __builtin_amdgcn_readlane(sum, 63);

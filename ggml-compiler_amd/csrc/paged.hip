@@ -11,8 +11,6 @@ namespace gcq {
 
 namespace {
 
-constexpr int kTileRows = 8;
-
 struct AppendArgs {
     Paged p;
     const float * k, * v, * q;
@@ -139,17 +137,31 @@ __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
     }
 }
 
-// Many rows of a sequence: a workgroup takes one tile of the cache (32 positions) for one KV head, and the tile's rows of q
-// heads hk, hk + Hkv, .. A thread has four pairs of one row for all of those heads, their sines in registers; the tile is put
-// together in LDS and leaves as 16-byte pieces, where a row at a time writes V's bytes one by one.
+// Eight tokens of a tile (one of its four parts) put side by side: 9 D bytes, and where their 16-byte pieces belong in the tile.
+template <int D>
+struct Eight {
+    static constexpr int kPieces = 9 * D / 16;  // D / 4 of K's codes (D / 32 to a token), D / 4 of V's, one of scales for each block
+    static __device__ __forceinline__ int k_byte(int m, int i) { return paged_k_byte<D>(m, i); }
+    static __device__ __forceinline__ int v_byte(int m, int i) { return 4 * D + (i >> 5) * 256 + (i & 15) * 16 + (i >> 4 & 1) * 8 + m; }
+    static __device__ __forceinline__ int scale(int m, int b, int v) { return 8 * D + 16 * (b + v * (D / 32)) + 2 * paged_order(m); }
+    static __device__ __forceinline__ int piece(int c, int g) {
+        if (c < D / 4) return 4 * D * g + 16 * c;
+        if (c < D / 2) return 16 * D + ((c - D / 4) >> 4) * 1024 + g * 256 + (c & 15) * 16;
+        return 32 * D + (c - D / 2) * 64 + g * 16;
+    }
+};
+
+// Many rows of a sequence: a workgroup takes eight positions of a tile for one KV head, and their rows of q heads hk,
+// hk + Hkv, .. A thread has four pairs of one row for all of those heads, their sines in registers; the eight tokens' bytes are
+// put together in LDS and leave as 16-byte pieces, where a row at a time writes V's one by one.
 template <int D, bool FULL>
-__global__ __launch_bounds__(4 * D) void k_paged_append_tile(const AppendArgs a) {
-    constexpr int L = D / 8, QB = FULL ? 4 : 1;  // threads of a row; q heads under way at a time, as the registers allow
-    __shared__ __align__(16) uint8_t image[36 * D];
-    const int tid = threadIdx.x, lane = tid & 63, slot = tid / L, i = 4 * (tid % L), hk = blockIdx.x % a.p.Hkv;
+__global__ __launch_bounds__(D) void k_paged_append_eight(const AppendArgs a) {
+    constexpr int L = D / 8, QB = FULL ? 2 : 1;  // threads of a row; q heads under way at a time, as the registers allow
+    __shared__ __align__(16) uint8_t image[9 * D];
+    const int tid = threadIdx.x, lane = tid & 63, m8 = tid / L, i = 4 * (tid % L), hk = blockIdx.x % a.p.Hkv;
     PagedSpan w;
     if (!paged_find(a.p, blockIdx.x / a.p.Hkv, w)) return;
-    const int64_t pos = w.tile * 32 + slot, j = pos - w.past;
+    const int64_t pos = w.eight * 8 + m8, j = pos - w.past;
     const bool on = j >= 0 && j < w.rows;
     const int64_t r = w.r0 + (on ? j : 0);
     const int half = a.n_dims / 2;
@@ -203,7 +215,7 @@ __global__ __launch_bounds__(4 * D) void k_paged_append_tile(const AppendArgs a)
             if (FULL || i + D / 2 < a.n_dims) f.x[1][e] = FULL ? turned(x1, cs[0][e], x0, sn[0][e]) : turned(x1, cs[NC - 1][e], f.p[FULL ? 0 : 1][e], sn[NC - 1][e]);
         }
     };
-    const int64_t tile = paged_tile(a.p, w.s, w.tile * 32, hk, D);  // (-1 for all of its positions or none)
+    const int64_t tile = paged_tile(a.p, w.s, w.eight * 8, hk, D);  // (-1 for all eight or none)
     turn(k);
 #pragma unroll
     for (int c = 0; c < 2; c++) {
@@ -232,16 +244,16 @@ __global__ __launch_bounds__(4 * D) void k_paged_append_tile(const AppendArgs a)
             uint32_t bytes = 0;
 #pragma unroll
             for (int e = 0; e < 4; e++) bytes |= (uint32_t) (code[0][e] | code[1][e] << 4) << (8 * e);
-            *reinterpret_cast<uint32_t *>(image + paged_k_byte<D>(slot, i)) = bytes;
+            *reinterpret_cast<uint32_t *>(image + Eight<D>::k_byte(m8, i)) = bytes;
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) image[paged_v_byte<D>(slot, i + e)] = (uint8_t) (code[0][e] | code[1][e] << 4);
+            for (int e = 0; e < 4; e++) image[Eight<D>::v_byte(m8, i + e)] = (uint8_t) (code[0][e] | code[1][e] << 4);
         }
         if ((lane & 7) == 0)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int b = i / 32 + h * (D / 64);
-                *reinterpret_cast<uint16_t *>(image + (c ? paged_v_scale<D>(slot, b) : paged_k_scale<D>(slot, b))) = f2h_exact(d[h]);
+                *reinterpret_cast<uint16_t *>(image + Eight<D>::scale(m8, b, c)) = f2h_exact(d[h]);
             }
     }
     if (a.q) {
@@ -266,21 +278,20 @@ __global__ __launch_bounds__(4 * D) void k_paged_append_tile(const AppendArgs a)
         }
     }
     __syncthreads();
-    if (tile < 0 || tid >= 36 * D / 16) return;
-    // the tile's 16-byte pieces; in part where some of their tokens are not this batch's
-    const int64_t s0 = w.past - w.tile * 32, s1 = s0 + w.rows;
-    const uint32_t have = (s1 >= 32 ? ~0u : (1u << s1) - 1) & (s0 > 0 ? ~0u << s0 : ~0u);
-    uint8_t * o = a.p.data + tile + 16 * tid;
+    if (tile < 0 || tid >= Eight<D>::kPieces) return;
+    // in part where some of the eight are not this batch's
+    const int64_t s0 = w.past - w.eight * 8, s1 = s0 + w.rows;
+    const uint32_t have = (s1 >= 8 ? 255 : (1u << s1) - 1) & (s0 > 0 ? 255u << s0 : 255);
+    uint8_t * o = a.p.data + tile + Eight<D>::piece(tid, (int) w.eight & 3);
     const uint8_t * from = image + 16 * tid;
-    const bool codes = tid < 2 * D;
-    const uint32_t m = tid < D ? (have >> tid / (D / 32) & 1) * 255 : have >> (codes ? tid >> 4 & 3 : tid & 3) * 8 & 255;
-    if (m == 255) *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<const uint4 *>(from);
-    else if (codes) {
+    if (have == 255 || (tid < D / 4 && have >> tid / (D / 32) & 1)) *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<const uint4 *>(from);
+    else if (tid < D / 4) return;
+    else if (tid < D / 2) {
         for (int b = 0; b < 16; b++)
-            if (m >> (b & 7) & 1) o[b] = from[b];
+            if (have >> (b & 7) & 1) o[b] = from[b];
     } else {
         for (int e = 0; e < 8; e++)
-            if (m >> paged_order(e) & 1) *reinterpret_cast<uint16_t *>(o + 2 * e) = *reinterpret_cast<const uint16_t *>(from + 2 * e);
+            if (have >> paged_order(e) & 1) *reinterpret_cast<uint16_t *>(o + 2 * e) = *reinterpret_cast<const uint16_t *>(from + 2 * e);
     }
 }
 
@@ -291,48 +302,19 @@ struct ReadArgs {
     float * k, * v;
 };
 
-// A wavefront takes one row of one KV head, keys and values.
+// A workgroup takes eight positions for one KV head, by way of LDS; a thread gives four pairs of one row.
 template <int D>
-__global__ __launch_bounds__(256) void k_paged_read(const ReadArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int r = (int) (unit / a.p.Hkv), h = (int) (unit % a.p.Hkv);
-    if (r >= a.p.n_rows) return;
-    const int s = paged_seq(a.p, r);
-    if (s < 0) return;
-    const int64_t pos = (int64_t) a.p.past[s] + (r - a.p.starts[s]);
-    const int slot = (int) pos & 31;
-    const int64_t tile = paged_tile(a.p, s, pos, h, D);
-#pragma unroll
-    for (int c = 0; c < 2; c++) {
-        float * o = (c ? a.v : a.k) + unit * D;
-        for (int i = lane; i < D / 2; i += 64) {
-            float lo = 0.0f, hi = 0.0f;
-            if (tile >= 0) {
-                const uint8_t * t = a.p.data + tile;
-                const int b = t[c ? paged_v_byte<D>(slot, i) : paged_k_byte<D>(slot, i)];
-                const auto scale = [&](int blk) { return h2f(*(const uint16_t *) (t + (c ? paged_v_scale<D>(slot, blk) : paged_k_scale<D>(slot, blk)))); };
-                lo = scale(i / 32) * (float) ((b & 15) - 8);
-                hi = scale(i / 32 + D / 64) * (float) ((b >> 4) - 8);
-            }
-            o[i] = lo;
-            o[i + D / 2] = hi;
-        }
-    }
-}
-
-// Many rows: a workgroup takes one tile for one KV head, by way of LDS; a thread gives four pairs of one row.
-template <int D>
-__global__ __launch_bounds__(4 * D) void k_paged_read_tile(const ReadArgs a) {
+__global__ __launch_bounds__(D) void k_paged_read(const ReadArgs a) {
     constexpr int L = D / 8;
-    __shared__ __align__(16) uint8_t image[36 * D];
-    const int tid = threadIdx.x, slot = tid / L, i = 4 * (tid % L), hk = blockIdx.x % a.p.Hkv;
+    __shared__ __align__(16) uint8_t image[9 * D];
+    const int tid = threadIdx.x, m8 = tid / L, i = 4 * (tid % L), hk = blockIdx.x % a.p.Hkv;
     PagedSpan w;
     if (!paged_find(a.p, blockIdx.x / a.p.Hkv, w)) return;
-    const int64_t tile = paged_tile(a.p, w.s, w.tile * 32, hk, D);
-    if (tile >= 0 && tid < 36 * D / 16) *reinterpret_cast<uint4 *>(image + 16 * tid) = *reinterpret_cast<const uint4 *>(a.p.data + tile + 16 * tid);
+    const int64_t tile = paged_tile(a.p, w.s, w.eight * 8, hk, D);
+    if (tile >= 0 && tid < Eight<D>::kPieces)
+        *reinterpret_cast<uint4 *>(image + 16 * tid) = *reinterpret_cast<const uint4 *>(a.p.data + tile + Eight<D>::piece(tid, (int) w.eight & 3));
     __syncthreads();
-    const int64_t j = w.tile * 32 + slot - w.past;
+    const int64_t j = w.eight * 8 + m8 - w.past;
     if (j < 0 || j >= w.rows) return;
     typedef float f4_t __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -340,14 +322,14 @@ __global__ __launch_bounds__(4 * D) void k_paged_read_tile(const ReadArgs a) {
         f4_t y[2] = {};
         if (tile >= 0) {
             uint32_t b = 0;
-            if (c == 0) b = *reinterpret_cast<const uint32_t *>(image + paged_k_byte<D>(slot, i));
+            if (c == 0) b = *reinterpret_cast<const uint32_t *>(image + Eight<D>::k_byte(m8, i));
             else
 #pragma unroll
-                for (int e = 0; e < 4; e++) b |= (uint32_t) image[paged_v_byte<D>(slot, i + e)] << (8 * e);
+                for (int e = 0; e < 4; e++) b |= (uint32_t) image[Eight<D>::v_byte(m8, i + e)] << (8 * e);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int blk = i / 32 + h * (D / 64);
-                const float d = h2f(*reinterpret_cast<const uint16_t *>(image + (c ? paged_v_scale<D>(slot, blk) : paged_k_scale<D>(slot, blk))));
+                const float d = h2f(*reinterpret_cast<const uint16_t *>(image + Eight<D>::scale(m8, blk, c)));
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[h][e] = d * (float) ((int) (b >> (8 * e + 4 * h) & 15) - 8);
             }
@@ -401,10 +383,15 @@ unsigned blocks(int64_t waves) {
     return (unsigned) ((waves + 3) / 4);
 }
 
-// Whether rows are taken a tile at a time: a sequence has some of a tile's 32 at the least, on average.
-bool by_tiles(const Paged & p) { return p.n_rows >= kTileRows * std::min(p.n_seq, p.n_rows); }
-unsigned tile_blocks(const Paged & p) {  // a sequence's rows may begin and end inside a tile
-    const int64_t n = (p.n_rows / kPagedTile + 2 * (int64_t) std::min(p.n_seq, p.n_rows)) * p.Hkv;
+// Whether rows are appended eight positions at a time: a sequence fills half an eight at the least, and there are 2^20 values,
+// enough to pay for a workgroup's longer way. (64 sequences, 32 heads and 8 KV heads of 128, rows one by one and by
+// eights: 2 rows each 6.9 and 7.9 us, 4 rows 8.7 and 8.0, 16 rows 21.1 and 10.6; one sequence: 32 rows 4.4 and 6.3, 128 rows
+// 6.7 and 6.4.)
+bool by_eights(const AppendArgs & a, int D) {
+    return a.p.n_rows >= 4 * std::min(a.p.n_seq, a.p.n_rows) && (int64_t) a.p.n_rows * (a.H + 2 * a.p.Hkv) * D >= 1 << 20;
+}
+unsigned eight_blocks(const Paged & p) {  // a sequence's rows may begin and end inside an eight
+    const int64_t n = (p.n_rows / 8 + 2 * (int64_t) std::min(p.n_seq, p.n_rows)) * p.Hkv;
     require(n <= INT32_MAX, "paged: too many rows and heads");
     return (unsigned) n;
 }
@@ -413,10 +400,10 @@ bool vectors(const float * x, int64_t r, int64_t h) { return aligned(x, 16) && r
 template <int D>
 void run_append(const AppendArgs & a, hipStream_t s) {
     const bool full = !a.freqs || a.n_dims == D;
-    if (by_tiles(a.p) && a.n_dims % 8 == 0 && vectors(a.k, a.k_r, a.k_h) && vectors(a.v, a.v_r, a.v_h) &&
+    if (by_eights(a, D) && a.n_dims % 8 == 0 && vectors(a.k, a.k_r, a.k_h) && vectors(a.v, a.v_r, a.v_h) &&
         (!a.q || (vectors(a.q, a.q_r, a.q_h) && aligned(a.q_out, 8)))) {
-        if (full) k_paged_append_tile<D, true><<<tile_blocks(a.p), 4 * D, 0, s>>>(a);
-        else k_paged_append_tile<D, false><<<tile_blocks(a.p), 4 * D, 0, s>>>(a);
+        if (full) k_paged_append_eight<D, true><<<eight_blocks(a.p), D, 0, s>>>(a);
+        else k_paged_append_eight<D, false><<<eight_blocks(a.p), D, 0, s>>>(a);
         return;
     }
     const unsigned grid = blocks((int64_t) a.p.n_rows * a.parts);
@@ -425,8 +412,7 @@ void run_append(const AppendArgs & a, hipStream_t s) {
 }
 template <int D>
 void run_read(const ReadArgs & a, hipStream_t s) {
-    if (by_tiles(a.p) && aligned(a.k, 16) && aligned(a.v, 16)) k_paged_read_tile<D><<<tile_blocks(a.p), 4 * D, 0, s>>>(a);
-    else k_paged_read<D><<<blocks((int64_t) a.p.n_rows * a.p.Hkv), 256, 0, s>>>(a);
+    k_paged_read<D><<<eight_blocks(a.p), D, 0, s>>>(a);
 }
 
 }  // namespace
@@ -488,8 +474,8 @@ int gcq_paged_read(const gcq_paged_cache * cache, const gcq_paged_batch * batch,
     return guarded([&] {
         ReadArgs a{view(cache, batch, n_rows), k, v};
         if (n_rows == 0) return;
-        need(k, "k", 4);
-        need(v, "v", 4);
+        need(k, "k", 16);
+        need(v, "v", 16);
         hipStream_t s = as_stream(stream);
         if (cache->head_dim == 64) run_read<64>(a, s);
         else if (cache->head_dim == 128) run_read<128>(a, s);

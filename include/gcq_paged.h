@@ -62,7 +62,7 @@ GCQ_API int gcq_paged_append(const gcq_paged_cache * cache, const gcq_paged_batc
                              const float * q, int64_t q_r, int64_t q_h, int n_head, void * q_out, const float * freqs,
                              int n_dims, float attn_factor, void * stream);
 
-/* The values that the cache holds for the batch's rows: k, v [n_rows][n_head_kv][D] f32. past = 0 and all of a
+/* The values that the cache holds for the batch's rows: k, v [n_rows][n_head_kv][D] f32, 16-byte aligned. past = 0 and all of a
  * sequence's tokens as rows reads the sequence. */
 GCQ_API int gcq_paged_read(const gcq_paged_cache * cache, const gcq_paged_batch * batch, int64_t n_rows, float * k,
                            float * v, void * stream);

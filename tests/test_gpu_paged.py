@@ -547,12 +547,13 @@ def test_refusals_on_the_device(gops):
     assert gops.paged_read(cache, batch, 0)[0].shape == (0, 2, 64)
 
 
-@pytest.mark.parametrize("D,n_dims,H,Hkv", [(64, 64, 9, 3), (128, 128, 3, 4), (128, 72, 24, 2), (256, 256, 10, 2), (256, 64, 4, 1)])
-@pytest.mark.parametrize("rows,past", [([8], [0]), ([8, 9], [28, 31]), ([7, 9], [1, 2]), ([32, 64, 1, 31], [0, 32, 95, 33]),
-                                       ([3, 200, 0, 95], [62, 33, 4, 1])])
-def test_rows_by_tiles_equal_rows_one_by_one(gops, D, n_dims, H, Hkv, rows, past):
-    """A call that goes a tile at a time and calls of a few rows each (strides that no 16-byte load takes among them) leave
-    the same bytes, queries and rows read back; the rest of the pool stays as it is."""
+@pytest.mark.parametrize("D,n_dims,Hkv", [(64, 64, 3), (128, 128, 4), (128, 72, 2), (256, 256, 2), (256, 64, 1)])
+@pytest.mark.parametrize("rows,past", [([8], [0]), ([4], [30]), ([8, 9], [28, 31]), ([7, 9], [1, 2]),
+                                       ([32, 64, 1, 31], [0, 32, 95, 33]), ([3, 200, 0, 95], [62, 33, 4, 1])])
+def test_rows_by_eights_equal_rows_one_by_one(gops, D, n_dims, Hkv, rows, past):
+    """A call that goes eight positions at a time and calls of a few rows each (strides that no 16-byte load takes among
+    them) leave the same bytes, queries and rows read back; the rest of the pool stays as it is."""
+    H = (1 << 20) // (D * sum(rows)) + 2  # (fewer values go row by row)
     c = Case(gops, rows, past, Hkv, D, 64, seed=31, extra_rows=2, fill=0xA5)
     x = torch.from_numpy(c.rng.standard_normal((c.n, H + 2 * Hkv, D)).astype(np.float32)).cuda()
     freqs = gops.rope_freqs(n_dims, 10000.0)
@@ -582,8 +583,8 @@ def test_rows_by_tiles_equal_rows_one_by_one(gops, D, n_dims, H, Hkv, rows, past
     assert (got_k[-2:] == 3.0).all() and (got_v[-2:] == 3.0).all() and (q16[-2:] == 5.0).all()
 
 
-def test_append_by_tiles_special_values(gops):
-    """Ties of either sign, zeros of either sign, NaNs, infinities and subnormal scales: a tile at a time as one by one."""
+def test_append_by_eights_special_values(gops):
+    """Ties of either sign, zeros of either sign, NaNs, infinities and subnormal scales: by eights as one by one."""
     D = 64
     x = torch.zeros((32, 1, D), device="cuda")
     x[1, 0, 5], x[1, 0, 9] = -2.0, 2.0
@@ -602,9 +603,10 @@ def test_append_by_tiles_special_values(gops):
     a, b = (gops.PagedCache.new(1, 32, 1, D) for _ in range(2))
     page = torch.zeros((1, 1), **i32)
     whole = gops.PagedBatch(page, torch.tensor([0, 32], **i32), torch.tensor([0], **i32))
-    q = gops.paged_append(a, whole, x, x, q=x)
+    q = gops.paged_append(a, whole, x, x, q=x.expand(32, 512, D))  # (512 heads: enough values to go by eights)
+    assert torch.equal(q[:, 0].view(torch.int16), q[:, 511].view(torch.int16))
     for r in range(32):
         one = gops.PagedBatch(page, torch.tensor([0, 1], **i32), torch.tensor([r], **i32))
         o = gops.paged_append(b, one, x[r:r + 1], x[r:r + 1], q=x[r:r + 1])
-        assert torch.equal(o.view(torch.int16), q[r:r + 1].view(torch.int16))
+        assert torch.equal(o[:, 0].view(torch.int16), q[r:r + 1, 0].view(torch.int16))
     assert torch.equal(a.data, b.data)

@@ -102,7 +102,7 @@ def test_append_refusals():
 
 def test_read_refusals():
     _refused(_read(k=None), "k is NULL")
-    _refused(_read(v=P + 1), "4-byte aligned")
+    _refused(_read(v=P + 8), "16-byte aligned")
 
 
 def test_attn_refusals():
