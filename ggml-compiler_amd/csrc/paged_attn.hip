@@ -186,6 +186,8 @@ template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // Wavefronts per SIMD that the registers (and, heads of 256, LDS) hold; and of a workgroup.
+// (Eight wavefronts to a workgroup, heads of 128: 32 sequences' step 32.1 us for 25.3 with four, four prompts 134 for 86; heads of
+// 256 with 32 rows, whose four wavefronts would fill half the LDS: 52.6 us with eight, 80.3 with four.)
 constexpr int per_simd(int D, int RT) { return D * RT <= 128 ? 4 : D * RT == 256 && RT == 2 ? 3 : 2; }
 constexpr int waves(int D, int rows) { return D == 256 && rows == 32 ? 8 : 4; }
 
@@ -614,25 +616,36 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a) {
     }
 }
 
-// How a call is run: row tiles of `rows` rows, `waves` wavefronts to each, splits that aim at `target` workgroups, those
-// resident at once.
+// How a call is run: row tiles of `rows` rows, splits that aim at `target` workgroups, those resident at once.
 struct Shape {
-    int rows, waves, target;
+    int rows, target;
     int64_t tiles, items, most;  // row tiles and workgroups that may have work; splits of a sequence
 };
-Shape shape_for(const Paged & p, int D, int G, int64_t max_rows) {
+Shape shape_of(const Paged & p, int D, int G, int64_t max_rows, int window, int rows) {
     Shape s{};
-    const int64_t per_seq = std::min<int64_t>(max_rows, p.n_rows) * G;  // rows of a KV head
-    s.rows = per_seq <= 16 ? 16 : 32;
-    s.waves = waves(D, s.rows);
-    s.target = 256 * 4 * per_simd(D, s.rows / 16) / s.waves;
+    s.rows = rows;
+    s.target = 256 * 4 * per_simd(D, rows / 16) / waves(D, rows);
     // row tiles: the rows' whole tiles and one more for each sequence
-    s.tiles = p.Hkv * std::min<int64_t>((int64_t) p.n_rows * G / s.rows + std::min<int64_t>(p.n_seq, p.n_rows),
-                                        p.n_seq * ((per_seq + s.rows - 1) / s.rows));
-    const int64_t longest = ((int64_t) p.max_pages << p.shift) / kPagedTile;  // tiles
+    const int64_t per_seq = std::min<int64_t>(max_rows, p.n_rows) * G;
+    s.tiles = p.Hkv * std::min<int64_t>((int64_t) p.n_rows * G / rows + std::min<int64_t>(p.n_seq, p.n_rows),
+                                        p.n_seq * ((per_seq + rows - 1) / rows));
+    int64_t longest = ((int64_t) p.max_pages << p.shift) / kPagedTile;  // tiles that a sequence's rows can see
+    if (window) longest = std::min(longest, (window + std::min<int64_t>(max_rows, p.n_rows) - 2) / kPagedTile + 2);
     s.most = longest <= 2 * kMinChunk ? 1 : (longest + kMinChunk - 1) / kMinChunk;
     s.items = std::min(s.tiles + s.target, s.tiles * s.most);
     return s;
+}
+// Tiles of 32 rows halve the work on K and V; tiles of 16 are more workgroups, of half the length. The larger ones if they
+// can still keep six wavefronts on every CU. (Heads of 128, 8 KV heads, tiles of 16 and of 32: 2000 keys, 20 rows of a KV
+// head 12.9 and 17.1 us, 256 rows 22.0 and 24.8; 32000 keys, 20 rows 28.9 and 25.0, 256 rows 125 and 100; 16 sequences of
+// 1000 keys, 64 rows 22.9 and 22.9, 256 rows 67.9 and 59.4.)
+Shape shape_for(const Paged & p, int D, int G, int64_t max_rows, int window) {
+    const Shape few = shape_of(p, D, G, max_rows, window, 16), many = shape_of(p, D, G, max_rows, window, 32);
+    const bool wide = std::min<int64_t>(max_rows, p.n_rows) * G > 16 && many.tiles * many.most * waves(D, 32) >= 6 * 256;
+    return wide ? many : few;
+}
+size_t workspace_of(const Shape & w, int D) {
+    return w.most == 1 ? 0 : (size_t) w.items * (w.rows * (D * sizeof(float) + sizeof(float2)) + sizeof(Part));
 }
 
 template <int D, int RT>
@@ -652,10 +665,11 @@ void run(const AttnArgs & a, const Shape & w, hipStream_t s) {
 
 }  // namespace
 
+// (for any window: a window only takes splits away)
 size_t paged_attn_workspace(const Paged & p, int D, int H, int64_t max_rows) {
     if (p.n_rows == 0) return 0;
-    const Shape w = shape_for(p, D, H / p.Hkv, max_rows);
-    return w.most == 1 ? 0 : (size_t) w.items * (w.rows * (D * sizeof(float) + sizeof(float2)) + sizeof(Part));
+    const int G = H / p.Hkv;
+    return std::max(workspace_of(shape_of(p, D, G, max_rows, 0, 16), D), workspace_of(shape_of(p, D, G, max_rows, 0, 32), D));
 }
 
 void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int64_t q_h, int H, int64_t max_rows, int window,
@@ -667,7 +681,7 @@ void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int6
     a.c2 = (float) (std::max(fabs((double) scale), 0x1p-100) * 1.4426950408889634074);
     a.negate = scale < 0.0f;
     a.out = out;
-    const Shape w = shape_for(p, D, a.G, max_rows);
+    const Shape w = shape_for(p, D, a.G, max_rows, window);
     if (w.items >= INT32_MAX) fail("paged_attn: too many rows and heads");
     a.items = (int) w.items, a.target = w.target;
     a.min_chunk = w.most == 1 ? 1 << 30 : kMinChunk;
