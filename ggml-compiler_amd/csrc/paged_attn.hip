@@ -409,6 +409,8 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
                     sh[i] = mine ? kP : shift[i];
                 }
             }
+            float minus = -1.0f;  // (unknown to the compiler: one v_fma_mix_f32 and not a conversion and a subtraction)
+            asm("" : "+s"(minus));
             h8_t ph[RA], pl[RA];
 #pragma unroll
             for (int i = 0; i < RA; i++)
@@ -416,7 +418,7 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
                 for (int e = 0; e < 8; e += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(fmaf(S[i][e], c[i], sh[i])), p1 = __builtin_amdgcn_exp2f(fmaf(S[i][e + 1], c[i], sh[i]));
                     const h2_t w = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-                    const h2_t u = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) w.x, -1.0f, p0), fmaf((float) w.y, -1.0f, p1)));
+                    const h2_t u = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) w.x, minus, p0), fmaf((float) w.y, minus, p1)));
                     ph[i][e] = w.x, ph[i][e + 1] = w.y, pl[i][e] = u.x, pl[i][e + 1] = u.y;
                 }
             // P V: 16 dims' MFMAs, then the next 16 dims' operands and the last ones' sums while they run; a row of ones at the
