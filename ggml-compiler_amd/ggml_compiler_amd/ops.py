@@ -315,15 +315,14 @@ def _paged_device(cache: PagedCache, batch: PagedBatch) -> int:
 
 def _paged_rows(x: torch.Tensor, dtype: torch.dtype, name: str, shape: tuple, d: int) -> tuple[int, int]:
     """x's strides, checked. (One test on the way through: these wrappers cost as much as a single token's kernels.)"""
-    s = x.stride()
-    if x.dtype != dtype or x.shape != shape or s[2] != 1 or x.get_device() != d:
+    if x.dtype != dtype or x.shape != shape or x.stride(2) != 1 or x.get_device() != d:
         _cuda(x, dtype, name)
         if x.shape != shape:
             raise ValueError(f"{name} must be {list(shape)}, got {list(x.shape)}")
-        if s[2] != 1:
+        if x.stride(2) != 1:
             raise ValueError(f"{name} needs a unit stride along the head dim")
         raise ValueError(f"{name} on {x.device}, the current device is {d}")
-    return s[0], s[1]
+    return x.stride(0), x.stride(1)
 
 
 def _paged_out(out: torch.Tensor | None, shape: tuple, dtype: torch.dtype, name: str, like: torch.Tensor) -> torch.Tensor:
@@ -337,8 +336,8 @@ def _paged_out(out: torch.Tensor | None, shape: tuple, dtype: torch.dtype, name:
     return out
 
 
-def _heads(x: torch.Tensor) -> int:
-    return x.shape[1] if x.dim() == 3 else 0
+def _rows_heads(x: torch.Tensor) -> tuple[int, int]:
+    return (x.shape[0], x.shape[1]) if x.dim() == 3 else (0, 0)
 
 
 def rope_freqs(n_dims: int, base: float, freq_scale: float = 1.0, ff: torch.Tensor | None = None,
@@ -357,12 +356,12 @@ def paged_append(cache: PagedCache, batch: PagedBatch, k: torch.Tensor, v: torch
     """Rows k, v f32 [n, Hkv, D] (strided allowed, unit inner stride) into the cache as Q4_0, the keys' NEOX pairs
     (i, i + len(freqs)) turned by position * freqs[i] (freqs None: unrotated). q f32 [n, H, D]: turned alike and
     returned as f16 [n, H, D], paged_attn's input (q_out: into it; rows of no sequence stay as they are)."""
-    d, n = _paged_device(cache, batch), k.shape[0]
+    d, (n, _) = _paged_device(cache, batch), _rows_heads(k)
     kv = (n, cache.Hkv, cache.D)
     ks, vs = _paged_rows(k, torch.float32, "k", kv, d), _paged_rows(v, torch.float32, "v", kv, d)
     H, q_at, out_at, qs, f_at, n_dims = 0, None, None, (0, 0), None, 0
     if q is not None:
-        H = _heads(q)
+        H = _rows_heads(q)[1]
         shape = (n, H, cache.D)
         qs = _paged_rows(q, torch.float32, "q", shape, d)
         q_out = _paged_out(q_out, shape, torch.float16, "q_out", q)
@@ -396,11 +395,13 @@ def paged_attn(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, scale: flo
     `window` of them if window > 0. q f16 [n, H, D] (strides multiples of 8, unit inner stride) -> f32 [n, H, D] (into
     out if given; rows of no sequence stay as they are; a row that sees no token gives zeros). max_rows: no sequence
     has more rows than this (default n); 1 for a decode step."""
-    d, n, H = _paged_device(cache, batch), q.shape[0], _heads(q)
+    d, (n, H) = _paged_device(cache, batch), _rows_heads(q)
     shape = (n, H, cache.D)
     qs = _paged_rows(q, torch.float16, "q", shape, d)
     out = _paged_out(out, shape, torch.float32, "out", q)
-    max_rows = max(n, 1) if max_rows is None else max_rows
+    max_rows = max(n, 1) if max_rows is None else min(max_rows, max(n, 1))
+    if not 0 <= window < 1 << 31:
+        raise ValueError(f"window {window} is not in 0 .. 2^31 - 1")
     lib = load()
     ws_n = lib.gcq_paged_attn_workspace(cache._at, batch._at, n, H, max_rows)
     if ws_n == 0:

@@ -537,8 +537,20 @@ def test_refusals_on_the_device(gops):
         gops.paged_attn(cache, batch, q[:, :3], 0.1)
     with pytest.raises(ValueError, match="torch.float16"):
         gops.paged_attn(cache, batch, q.float(), 0.1)
-    with pytest.raises(gops.GcqError, match="window"):
-        gops.paged_attn(cache, batch, q, 0.1, window=-1)
+    for window in (-1, 1 << 31, 1 << 32):
+        with pytest.raises(ValueError, match="window"):
+            gops.paged_attn(cache, batch, q, 0.1, window=window)
+    for bad in (x[0, 0, 0], x[0], x[None]):
+        with pytest.raises(ValueError, match="must be"):
+            gops.paged_append(cache, batch, bad, bad)
+        with pytest.raises(ValueError, match="must be"):
+            gops.paged_append(cache, batch, x, x, q=bad)
+        with pytest.raises(ValueError, match="must be"):
+            gops.paged_attn(cache, batch, bad.half(), 0.1)
+    with pytest.raises(AttributeError):  # (its address is in the C structure)
+        batch.past = batch.starts
+    with pytest.raises(gops.GcqError, match="16-byte aligned"):
+        gops.paged_read(cache, batch, 4, k=torch.zeros(4 * 2 * 64 + 1, device="cuda")[1:].view(4, 2, 64))
     with pytest.raises(gops.GcqError, match="max_rows"):
         gops.paged_attn(cache, batch, q, 0.1, max_rows=0)
     with pytest.raises(ValueError, match="contiguous"):
@@ -610,3 +622,20 @@ def test_append_by_eights_special_values(gops):
         o = gops.paged_append(b, one, x[r:r + 1], x[r:r + 1], q=x[r:r + 1])
         assert torch.equal(o[:, 0].view(torch.int16), q[r:r + 1, 0].view(torch.int16))
     assert torch.equal(a.data, b.data)
+
+
+@pytest.mark.parametrize("rows", [[1, 2], [9, 90]])
+def test_attention_largest_scale(gops, rows):
+    """scale log2(e) past f32: queries of zeros still weigh all keys alike."""
+    c = Case(gops, rows, [70, 3], 1, 64, 32, seed=33)
+    run_attn(gops, c, 4, scale=3e38, q_scale=0.0)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows,past,window,G", [([8] * 9, [500 * s for s in range(9)], 0, 4), ([8] * 9, [500 * s for s in range(9)], 700, 4),
+                                                ([40] * 6 + [1], [9000, 0, 33, 64, 4000, 1, 7000], 0, 2),
+                                                ([3, 1], [40000, 60000], 0, 8), ([3, 1], [40000, 60000], 2000, 8)])
+def test_attention_both_row_tiles(gops, D, rows, past, window, G):
+    """Sizes on either side of the choice between tiles of 16 and of 32 rows, in one and in several splits, the window
+    moving it."""
+    run_attn(gops, Case(gops, rows, past, 1 if max(past) > 30000 else 2, D, 64, seed=34), G, window=window, max_rows=max(rows))
