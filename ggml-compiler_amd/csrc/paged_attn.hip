@@ -85,6 +85,8 @@ struct Plan {
     __device__ __forceinline__ Plan(const AttnArgs & args) : a(args) {
         const int lane = threadIdx.x & 63;
         w = seq_work<ROWS>(a, lane);
+        chunk = a.min_chunk;
+        if (!a.parts) return;  // one split each
         double u = (double) w.rts * w.tiles, n = w.rts;
         for (int s0 = 64; s0 < a.p.n_seq; s0 += 64) {
             const SeqWork x = seq_work<ROWS>(a, s0 + lane);
