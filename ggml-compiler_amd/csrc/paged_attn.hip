@@ -1,20 +1,29 @@
 // paged_attn.hip - attention over the paged 4-bit cache (include/gcq_paged.h; layout in paged.h).
 //
-// k_paged_attn: a wavefront takes 16 rows, a row being a (query, head) pair of one KV head (row j G + g), and tiles of 32
-// keys, straight from memory into the matrix cores' operands:
+// A row is a (query, head) pair of one KV head (row j G + g of a sequence, G query heads to a KV head). k_paged_attn gives a
+// workgroup a row tile of 16 RT rows and a run of key tiles, which its NW wavefronts take in turn, each over all the rows:
+//   - a tile comes straight from memory into the wavefront's two slots of LDS (36 D bytes, the next tile under way);
 //   - scores S^T[key][row] = K Q^T, one v_mfma_f32_16x16x32_f16 per Q4_0 block of 32 dims and 16 keys, on the codes c - 8
-//     themselves (exact in f16); a block's sum is scaled by its d in f32.
+//     themselves (exact in f16); a block's sum is scaled by its d in f32;
 //   - lane (row, g) is left with the scores of keys 8 g .. 8 g + 7, in the order that P V's operand wants them;
 //   - O^T[dim][row] += V^T P^T, V's values d (c - 8) as two f16 parts (15 bits: exact), P as two of 11 bits, cut off; the
 //     sum of weights goes through the same two parts (a row of ones), so that numerator and denominator see the same.
 // The softmax runs in powers of two against an integer reference R that follows the maximum in steps: it moves when a score
 // passes it by 4, which is rare, and moving it scales by an exact power of two. Chains inside the MFMAs (whose sums are
-// cut off, not rounded) start from zero for each tile; tiles are added in f32.
+// cut off, not rounded) start from zero for each tile; tiles are added in f32. Against 64 bits the outputs are off by 2e-7 to
+// 5e-7 (2-norm).
 //
-// Work: a sequence's tiles are cut into splits of `chunk` tiles, the same for all sequences, chosen so that all splits of all
-// sequences make about kTarget workgroups. Every workgroup computes that plan from the batch's arrays by itself (no planning
-// launch, and a captured graph follows the arrays), finds its split by a prefix sum over the sequences, deals its
-// tiles to its wavefronts in turn and joins their sums in LDS. Sequences of several splits are joined by k_paged_merge.
+// Work: a sequence's tiles are cut into even splits of about `chunk` tiles, one chunk for all sequences, chosen so that all splits of
+// all row tiles come to Shape::target workgroups. Every workgroup computes that plan from the batch's arrays by itself (no planning
+// launch, and a captured graph follows the arrays), finds its split by a prefix sum over the sequences and joins its wavefronts'
+// sums in LDS. Row tiles of several splits are joined by k_paged_merge, from notes (Part) that the workgroups leave.
+//
+// What bounds it: the vector ALU. A tile of heads of 128 costs a wavefront some 335 operations at 16 rows: 216 to make its 4-bit
+// codes into MFMA operands, whatever the rows, the others for 16 rows' scaling, softmax and sums. Reads alone, all
+// arithmetic left out, took 25 us of 131071 keys' 39 (one row of 32 heads, 8 KV heads, 151 MB: 3.9 TB/s) and 15 us of 27 for 32
+// sequences of 200 to 8191 keys. 512 rows over 4096 keys take 95 us (339 TFLOP/s of 4 D flops a key and row; the MFMAs do twice
+// those, for the parts). That is also why a wavefront has all of its rows' dims: shared between wavefronts by way of LDS, the
+// operands of a tile took longer to write there (34 cycles a KiB of a CU's) than to make again.
 #include "paged.h"
 
 #include <algorithm>
@@ -30,7 +39,7 @@ typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kMinChunk = 16;    // tiles: a shorter split costs more in the merge than it saves
+constexpr int kMinChunk = 16;    // tiles of a split: four to a wavefront (32 sequences' step: 25.3 us, with 32 tiles 28.6)
 constexpr float kSlack = 4.0f;   // how far a score's exponent may pass R
 constexpr float kBig = 0x1p20f;  // exponents from here on are no longer exact to 2^-4
 constexpr float kP = 4.0f;       // the exponent of P's scale: with kSlack at most 2^8; parts down to 2^-28 of 2^R
@@ -540,6 +549,7 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
 
 // A row tile of several splits: their sums, weighted by 2^(R - the largest R). The splits' workgroups share its rows, row y to
 // split y % ns's; a row's splits are read by the workgroup's four wavefronts together if they are more than one has under way.
+// (4.8 us for 131071 keys' 125 splits, 8.6 with a wavefront to a row; 4.6 us for 16 sequences' 35 rows in 3 splits, 24.5 with four.)
 template <int D, int ROWS>
 __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a) {
     constexpr int L = D / 4, N1 = 64 / L, N4 = 4 * N1;  // lanes of a split; splits at a time, a wavefront's and all four's
@@ -644,6 +654,7 @@ Shape shape_of(const Paged & p, int D, int G, int64_t max_rows, int window, int 
                                         p.n_seq * ((per_seq + rows - 1) / rows));
     int64_t longest = ((int64_t) p.max_pages << p.shift) / kPagedTile;  // tiles that a sequence's rows can see
     if (window) longest = std::min(longest, (window + std::min<int64_t>(max_rows, p.n_rows) - 2) / kPagedTile + 2);
+    // (two splits of the least size gain nothing and need the join: 501 keys 9.5 us as one split, 10.7 + 3.7 as two)
     s.most = longest <= 2 * kMinChunk ? 1 : (longest + kMinChunk - 1) / kMinChunk;
     s.items = std::min(s.tiles + s.target, s.tiles * s.most);
     return s;
