@@ -288,6 +288,9 @@ class PagedBatch:
         if self.pages.dim() != 2 or self.pages.stride(1) != 1:
             raise ValueError("pages must be [sequences, pages] with contiguous rows")
         S, n = self.pages.shape
+        ld = self.pages.stride(0) if S > 1 else n
+        if ld < n:
+            raise ValueError(f"pages' rows overlap: stride {ld} for {n} pages")
         if self.starts.shape != (S + 1,) or self.past.shape != (S,):
             raise ValueError(f"{S} sequences need starts [{S + 1}] and past [{S}], got {tuple(self.starts.shape)} and "
                              f"{tuple(self.past.shape)}")
@@ -295,7 +298,7 @@ class PagedBatch:
             raise ValueError("starts and past must be contiguous")
         if self.starts.get_device() != self.pages.get_device() or self.past.get_device() != self.pages.get_device():
             raise ValueError("pages, starts and past must be on one device")
-        _paged_handle(self, _lib.PagedBatch(self.pages.data_ptr(), max(self.pages.stride(0), n), self.starts.data_ptr(),
+        _paged_handle(self, _lib.PagedBatch(self.pages.data_ptr(), ld, self.starts.data_ptr(),
                                             self.past.data_ptr(), S, n), self.pages)
 
 

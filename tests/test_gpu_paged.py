@@ -522,6 +522,8 @@ def test_refusals_on_the_device(gops):
         gops.PagedCache(4, 32, 2, 64, cache.data[:-1])
     with pytest.raises(ValueError, match="2 sequences need"):
         gops.PagedBatch(torch.zeros((2, 2), **i32), torch.zeros(2, **i32), torch.zeros(2, **i32))
+    with pytest.raises(ValueError, match="rows overlap"):
+        gops.PagedBatch(torch.zeros((1, 2), **i32).expand(2, 2), torch.zeros(3, **i32), torch.zeros(2, **i32))
     with pytest.raises(ValueError, match="torch.int32"):
         gops.PagedBatch(torch.zeros((2, 2), device="cuda", dtype=torch.int64), torch.zeros(3, **i32), torch.zeros(2, **i32))
     for bad in (x[:, :1], x[..., :32], x.half(), x.cpu(), x.transpose(1, 2).contiguous().transpose(1, 2)):
@@ -639,3 +641,46 @@ def test_attention_both_row_tiles(gops, D, rows, past, window, G):
     """Sizes on either side of the choice between tiles of 16 and of 32 rows, in one and in several splits, the window
     moving it."""
     run_attn(gops, Case(gops, rows, past, 1 if max(past) > 30000 else 2, D, 64, seed=34), G, window=window, max_rows=max(rows))
+
+
+def test_captured_long_step_follows_the_batch(gops):
+    """As above where keys are split, rows go by eights and are read back: one captured append, attention and read."""
+    Hkv, H, D, page, S, n = 2, 14, 128, 256, 3, 600
+    rng = np.random.default_rng(41)
+    table = torch.from_numpy(rng.permutation(80)[:72].reshape(S, 24).astype(np.int32)).cuda()
+    starts, past = torch.zeros(S + 1, dtype=torch.int32, device="cuda"), torch.zeros(S, dtype=torch.int32, device="cuda")
+    batch = gops.PagedBatch(table, starts, past)
+    cache, other = (gops.PagedCache.new(80, page, Hkv, D) for _ in range(2))
+    x = torch.randn((3 * 5000, Hkv, D), device="cuda")
+    full = gops.PagedBatch(table, torch.arange(0, 15001, 5000, dtype=torch.int32, device="cuda"), torch.zeros_like(past))
+    for c in (cache, other):
+        gops.paged_append(c, full, x, x)
+    qkv = torch.zeros((n, H + 2 * Hkv, D), device="cuda")
+    freqs = gops.rope_freqs(D, 10000.0)
+    q16 = torch.zeros((n, H, D), dtype=torch.float16, device="cuda")
+    outs = [torch.zeros((n, H, D), device="cuda"), *(torch.zeros((n, Hkv, D), device="cuda") for _ in range(2))]
+
+    def step(c, q16, out, k, v):
+        gops.paged_append(c, batch, qkv[:, H:H + Hkv], qkv[:, H + Hkv:], q=qkv[:, :H], freqs=freqs, q_out=q16)
+        gops.paged_attn(c, batch, q16, D ** -0.5, out=out)
+        gops.paged_read(c, batch, n, k, v)
+
+    step(cache, q16, *outs)  # (starts of zeros: nobody's rows)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(cache, q16, *outs)
+    for rows, at in (([1, 1, 1], [4999, 10, 700]), ([600, 0, 0], [4300, 1, 2]), ([1, 0, 400], [5000, 0, 33]),
+                     ([0, 2, 1], [0, 5100, 701]), ([100, 250, 250], [4950, 0, 3000]), ([1, 1, 1], [5050, 250, 3250])):
+        qkv.copy_(torch.randn((n, H + 2 * Hkv, D), device="cuda"))
+        starts.copy_(torch.tensor(np.concatenate([[0], np.cumsum(rows)]), dtype=torch.int32))
+        past.copy_(torch.tensor(at, dtype=torch.int32))
+        for t in (q16, *outs):
+            t.fill_(7.0)
+        want = [t.clone() for t in (q16, *outs)]
+        graph.replay()
+        step(other, *want)
+        torch.cuda.synchronize()
+        for w, t in zip(want, (q16, *outs)):
+            assert torch.equal(w, t)
+        assert torch.equal(cache.data, other.data)
+        assert not bool((outs[0][:sum(rows)] == 7.0).all()) and bool((outs[0][sum(rows):] == 7.0).all())
