@@ -6,12 +6,13 @@
 //   - scores S^T[key][row] = K Q^T, one v_mfma_f32_16x16x32_f16 per Q4_0 block of 32 dims and 16 keys, on the codes c - 8
 //     themselves (exact in f16); a block's sum is scaled by its d in f32;
 //   - lane (row, g) is left with the scores of keys 8 g .. 8 g + 7, in the order that P V's operand wants them;
-//   - O^T[dim][row] += V^T P^T, V's values d (c - 8) as two f16 parts (15 bits: exact), P as two of 11 bits, cut off; the
-//     sum of weights goes through the same two parts (a row of ones), so that numerator and denominator see the same.
+//   - O^T[dim][row] += V^T P^T, V's values d (c - 8) as two f16 parts (15 bits: exact), P as two of 11 bits, the second one
+//     rounded: 2^-23 of a weight, or 2^-36 of 2^R where that is more; the sum of weights goes through the same two parts (a row
+//     of ones), so that numerator and denominator see the same.
 // The softmax runs in powers of two against an integer reference R that follows the maximum in steps: it moves when a score
 // passes it by 4, which is rare, and moving it scales by an exact power of two. Chains inside the MFMAs (whose sums are
-// cut off, not rounded) start from zero for each tile; tiles are added in f32. Against 64 bits the outputs are off by 2e-7 to
-// 5e-7 (2-norm).
+// cut off, not rounded) start from zero for each tile; tiles are added in f32. Against 64 bits the outputs are off by 1e-7 to
+// 7e-7 (2-norm; the more where one key is far ahead of up to 65535 others that together still count).
 //
 // Work: a sequence's tiles are cut into even splits of about `chunk` tiles, one chunk for all sequences, chosen so that all splits of
 // all row tiles come to Shape::target workgroups. Every workgroup computes that plan from the batch's arrays by itself (no planning
@@ -36,12 +37,13 @@ typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kMinChunk = 16;    // tiles of a split: four to a wavefront (32 sequences' step: 25.3 us, with 32 tiles 28.6)
 constexpr float kSlack = 4.0f;   // how far a score's exponent may pass R
 constexpr float kBig = 0x1p20f;  // exponents from here on are no longer exact to 2^-4
-constexpr float kP = 4.0f;       // the exponent of P's scale: with kSlack at most 2^8; parts down to 2^-28 of 2^R
+constexpr float kP = 11.0f;      // the exponent of P's scale: with kSlack at most 2^15, f16's largest power; parts down to 2^-35 of 2^R
 
 struct AttnArgs {
     Paged p;
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
     const auto body = [&](auto ra) {
         constexpr int RA = decltype(ra)::value;
         f4_t O[RA][NT];
-        float R[RA], l[RA], top[RA], shift[RA];  // the reference exponent; R + kSlack; kP - R
+        float R[RA], l[RA], top[RA], shift[RA];  // the reference exponent; where it moves; kP - R
 #pragma unroll
         for (int i = 0; i < RA; i++) {
             R[i] = top[i] = -INFINITY;
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
                     const float m = xor16_max(mx[i]), Rn = m > top[i] ? ceilf(m) : R[i];  // (a row's R goes by its own scores)
                     const float al = R[i] == Rn ? 1.0f : __builtin_amdgcn_exp2f(R[i] - Rn);
                     R[i] = Rn;
-                    top[i] = Rn + kSlack;
+                    top[i] = fabsf(Rn) >= kBig ? Rn : Rn + kSlack;  // (from 2^26 on R + 4 may be R + 8, more than P has room for)
                     shift[i] = kP - (Rn == -INFINITY ? 0.0f : Rn);
                     l[i] *= al;
 #pragma unroll
@@ -436,7 +438,8 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
                 for (int e = 0; e < 8; e += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(fmaf(S[i][e], c[i], sh[i])), p1 = __builtin_amdgcn_exp2f(fmaf(S[i][e + 1], c[i], sh[i]));
                     const h2_t w = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-                    const h2_t u = __builtin_bit_cast(h2_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) w.x, minus, p0), fmaf((float) w.y, minus, p1)));
+                    // (rounded: cut off, many small weights beside a large one would all lose)
+                    const h2_t u = __builtin_convertvector(f2_t{fmaf((float) w.x, minus, p0), fmaf((float) w.y, minus, p1)}, h2_t);
                     ph[i][e] = w.x, ph[i][e + 1] = w.y, pl[i][e] = u.x, pl[i][e + 1] = u.y;
                 }
             // P V: 16 dims' MFMAs, then the next 16 dims' operands and the last ones' sums while they run; a row of ones at the

@@ -684,3 +684,46 @@ def test_captured_long_step_follows_the_batch(gops):
             assert torch.equal(w, t)
         assert torch.equal(cache.data, other.data)
         assert not bool((outs[0][:sum(rows)] == 7.0).all()) and bool((outs[0][sum(rows):] == 7.0).all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("above", [10, 14, 17, 20, 24])
+@pytest.mark.parametrize("keys,rows,S,G", [(1024, 1, 160, 4), (4096, 1, 160, 4), (16384, 1, 160, 1), (4096, 768, 1, 8), (16384, 384, 2, 8),
+                                           (65536, 1, 1, 4)])
+def test_attention_sink(gops, D, above, keys, rows, S, G):
+    """One key `above` powers of two ahead of each other one, whose weights are log-normal, and values whose mean the first key's
+    is far from: what the small weights lose together shows. Mostly one split (the sequences share their pages), all row tiles."""
+    Hkv = 8 if rows == 1 else 2
+    c = Case(gops, [keys], [0], Hkv, D, 256, seed=above + D)
+    k = torch.from_numpy(c.rng.standard_normal((keys, Hkv, D)).astype(np.float32)).cuda() * 0.5
+    v = torch.from_numpy(c.rng.standard_normal((keys, Hkv, D)).astype(np.float32)).cuda() + 1.0
+    k[0], v[0] = above / (1.4426950408889634 * D ** 0.5), v[0] - 2.0  # (q's mean is 1: scale q K[0] = above ln 2)
+    b = c.batch()
+    gops.paged_append(c.cache, b, k, v)
+    c.k, c.v = (x.double() for x in gops.paged_read(c.cache, b, keys))
+    q = torch.from_numpy(c.rng.standard_normal((S * rows, G * Hkv, D)).astype(np.float32)).cuda().mul(0.5).add(1.0).half()
+    out = gops.paged_attn(c.cache, c.batch([rows] * S, [keys - rows] * S, np.repeat(c.table, S, 0)), q, D ** -0.5, max_rows=rows)
+    unseen = torch.arange(keys, device="cuda")[None] > torch.arange(keys - rows, keys, device="cuda").repeat(S)[:, None]
+    want, bound = torch.empty(q.shape, dtype=torch.float64, device="cuda"), 0.0
+    for h in range(G * Hkv):
+        x, kh = q[:, h].double(), c.k[:, h // G]
+        want[:, h] = torch.softmax((x @ kh.T * D ** -0.5).masked_fill(unseen, -torch.inf), -1) @ c.v[:, h // G]
+        bound = max(bound, float((x.abs() @ kh.abs().T).max()) * D ** -0.5)
+    check_attn(c, out, want, bound, keys)
+
+
+def test_attention_scores_one_step_apart(gops):
+    """Scores of 2^26 .. 2^27, whose f32 steps are 8: a later tile's key one step ahead of the first takes nearly all the weight."""
+    D, n = 64, 160
+    k, v = (torch.zeros((n, 1, D), device="cuda") for _ in range(2))
+    k[0, 0, 0] = k[128, 0, 0] = 1.0
+    k[128, 0, 32] = 2.0 ** -10
+    v[0], v[128] = 1.0, -1.0
+    c = Case(gops, [n], [0], 1, D, 32, seed=44)
+    gops.paged_append(c.cache, c.batch(), k, v)
+    q = torch.zeros((1, 1, D), dtype=torch.float16, device="cuda")
+    q[0, 0, 0], q[0, 0, 32] = 2.0 ** 13, 1.0  # q K: 2^13, and 2^-23 of it more
+    for i in range(24):
+        got = gops.paged_attn(c.cache, c.batch([1], [n - 1]), q, 2.0 ** 13 / 1.4426950408889634 * (1 + i / 26))
+        # 8 or more powers of two: at least 255 / 257 of the way, the weights' sums and product in f32
+        assert bool(((got <= -253.0 / 257.0) & (got >= -1.0 - 2.0 ** -20)).all()), (i, got)
