@@ -255,6 +255,9 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
         const int y = 16 * i + lr, x = x0 + min(y, nr - 1);
         h8_t v = *reinterpret_cast<const h8_t *>(a.q + (int64_t) (sw.r0 + x / a.G) * a.q_r + (int64_t) (hk * a.G + x % a.G) * a.q_h + 32 * b + 8 * g);
         if (y >= nr) v = h8_t{};
+        // An infinity becomes a NaN, as softmax makes of every key's score with it: scores of -inf alone would leave R at -inf, and
+        // the row would count as one without keys.
+        v = __builtin_elementwise_fma(v, h8_t{}, v);
         if (a.negate) v = -v;
         return h8_t{v[0], v[2], v[1], v[3], v[4], v[6], v[5], v[7]};
     };

@@ -73,9 +73,10 @@ GCQ_API size_t gcq_paged_attn_workspace(const gcq_paged_cache * cache, const gcq
 /* out[r][h] = sum over the keys j that row r sees of softmax_j(scale q[r][h] . K[j]) V[j], its rows appended before:
  * a row at position p sees the keys 0 .. p of its sequence, with window > 0 the last `window` of them; no key: zeros.
  * q f16 [r][h][D] at element strides (q_r, q_h), multiples of 8; out f32 [n_rows][n_head][D]; n_head a multiple of
- * n_head_kv, KV head h * n_head_kv / n_head. Scores, sums and outputs are f32's; a weight is held to 2^-23 of itself, but no finer
- * than 2^-35 of the row's largest (smaller ones come to 0). max_rows: no sequence has more rows than this (rows past it are left as
- * they are); n_rows where nothing is known. ws: gcq_paged_attn_workspace bytes, 256-byte aligned, any contents; calls
+ * n_head_kv, KV head h * n_head_kv / n_head. Scores, sums and outputs are f32's; a weight is held to 2^-23 of itself,
+ * but no finer than 2^-35 of the row's largest (smaller ones come to 0). A query with a NaN or an infinity gives NaNs
+ * where it sees a key. max_rows: no sequence has more rows than this (rows past it are left as they are); n_rows where
+ * nothing is known. ws: gcq_paged_attn_workspace bytes, 256-byte aligned, any contents; calls
  * that can overlap need one each. */
 GCQ_API int gcq_paged_attn(const gcq_paged_cache * cache, const gcq_paged_batch * batch, int64_t n_rows, const void * q,
                            int64_t q_r, int64_t q_h, int n_head, int64_t max_rows, int window, float scale, float * out,

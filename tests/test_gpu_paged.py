@@ -727,3 +727,34 @@ def test_attention_scores_one_step_apart(gops):
         got = gops.paged_attn(c.cache, c.batch([1], [n - 1]), q, 2.0 ** 13 / 1.4426950408889634 * (1 + i / 26))
         # 8 or more powers of two: at least 255 / 257 of the way, the weights' sums and product in f32
         assert bool(((got <= -253.0 / 257.0) & (got >= -1.0 - 2.0 ** -20)).all()), (i, got)
+
+
+@pytest.mark.parametrize("D,G", [(64, 4), (128, 1), (256, 8)])
+@pytest.mark.parametrize("rows,past,window", [([1, 1], [40, 0], 0), ([1], [40000], 0), ([3, 90], [700, 0], 0), ([40], [300], 33)])
+def test_a_query_with_an_infinity_gives_nans(gops, D, G, rows, past, window):
+    """softmax of scores among which are infinities is NaN, also where all of them are -inf; a row without keys gives zeros."""
+    c = Case(gops, rows, past, 1, D, 32, seed=45)
+    n_keys = [p + r for r, p in zip(rows, past)]
+    b = c.batch(n_keys, [0] * len(rows))
+    k = torch.rand((sum(n_keys), 1, D), device="cuda") + 0.5  # (positive, and no code stands for 0)
+    gops.paged_append(c.cache, b, k, k)
+    assert (gops.paged_read(c.cache, b, sum(n_keys))[0] > 0).all()
+    q = torch.randn((c.n, G, D), device="cuda").half()
+    table = c.table.copy()
+    if len(rows) == 2:
+        table[1] = -1
+    b = c.batch(table=table)
+    clean = gops.paged_attn(c.cache, b, q, 0.1, window=window)
+    assert torch.isfinite(clean).all()
+    bad = torch.zeros((c.n, G), dtype=torch.bool, device="cuda")
+    for i, (r, h) in enumerate([(0, 0), (c.n - 1, G - 1), (c.n // 2, G // 2)]):
+        bad[r, h] = True
+        q[r, h, 7 * i + 5] = [-torch.inf, torch.inf, -torch.inf][i]
+    keyless = torch.arange(c.n, device="cuda") >= rows[0] if len(rows) == 2 else torch.zeros(c.n, dtype=torch.bool, device="cuda")
+    for scale in (0.1, -0.1, 0.0):
+        want = clean if scale == 0.1 else gops.paged_attn(c.cache, b, q.masked_fill(bad[..., None], 0.0), scale, window=window)
+        got = gops.paged_attn(c.cache, b, q, scale, window=window)
+        assert torch.isnan(got[bad & ~keyless[:, None]]).all()
+        assert (got[keyless] == 0).all()
+        keep = ~bad & ~keyless[:, None]
+        assert torch.equal(got[keep], want[keep])
