@@ -706,8 +706,9 @@ void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int6
     AttnArgs a{};
     a.p = p, a.q = (const _Float16 *) q, a.q_r = q_r, a.q_h = q_h, a.H = H, a.G = H / p.Hkv, a.window = window;
     a.max_rows = (int) std::min<int64_t>(max_rows, p.n_rows);
-    // (from 0 up to 2^-100: scores of 0 either way, but -inf for a hidden key; no more than f32 holds: 0 for a score of 0)
-    a.c2 = (float) std::min(std::max(fabs((double) scale), 0x1p-100) * 1.4426950408889634074, 0x1.fffffep127);
+    // (from 0 up to 2^-100: scores of 0 either way, but -inf for a hidden key. Down to 2^86: q K is at most 2^40, all exponents
+    // stay within f32, and two scores q K that differ, by 2^-48 at the least, are 2^38 powers of two apart already.)
+    a.c2 = (float) (std::min(std::max(fabs((double) scale), 0x1p-100), 0x1p86) * 1.4426950408889634074);
     a.negate = scale < 0.0f;
     a.out = out;
     const Shape w = shape_for(p, D, a.G, max_rows, window);

@@ -758,3 +758,22 @@ def test_a_query_with_an_infinity_gives_nans(gops, D, G, rows, past, window):
         assert (got[keyless] == 0).all()
         keep = ~bad & ~keyless[:, None]
         assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("scale", [1e25, 1e32, -1e36, 3e38, -3e38])
+@pytest.mark.parametrize("D,G,rows,past", [(64, 4, [1, 1], [60, 0]), (128, 1, [70], [0]), (256, 8, [3, 20], [500, 0])])
+def test_attention_scores_past_f32(gops, D, G, rows, past, scale):
+    """Scores that f32 has no room for: still the largest key's values (of keys within 2^-20 of it, some mean), a single key's
+    whatever its sign."""
+    c = Case(gops, rows, past, 1, D, 32, seed=46)
+    c.fill_past()
+    q = torch.randn((c.n, G, D), device="cuda").half()
+    got = gops.paged_attn(c.cache, c.batch(), q, scale).double()
+    for s, (n, p) in enumerate(zip(rows, past)):
+        k, v = c.k[c.key0[s]:c.key0[s + 1], 0], c.v[c.key0[s]:c.key0[s + 1], 0]
+        for r in range(n):
+            x = k[:p + r + 1] @ q[c.starts[s] + r].double().T * scale
+            for h in range(G):
+                near = x[:, h] >= x[:, h].max() - x[:, h].abs().max() * 2.0 ** -20
+                o, u = got[c.starts[s] + r, h], v[:len(x)][near]
+                assert ((o >= u.amin(0) - 1e-5) & (o <= u.amax(0) + 1e-5)).all()
