@@ -175,12 +175,20 @@ __device__ __forceinline__ h8_t code_frag(u2_t w) {
 }
 
 // A tile from memory into LDS, without registers in between: 1 KiB per instruction, 16 bytes per lane, the last one partly.
-// (As inline code, m0 set and used in one piece, since the compiler has a builtin's loads waited for, all of them, before any LDS read.)
+// (As inline code, m0 set and used in one piece, since the compiler has a builtin's loads waited for, all of them, before any LDS read.
+// The base may come from a v_readlane just before: five wait states to a memory access that reads it, which the compiler leaves between
+// its own instructions only.)
 template <int D> constexpr int kTileLoads = (36 * D + 1023) / 1024;
-template <int OFF>
-__device__ __forceinline__ void lds_load(const uint8_t * base, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" ::"v"(voff), "s"(base), "s"(lds), "n"(OFF) : "memory");
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is a reserved register: it is said all the same that it changes)
+template <int N>
+__device__ __forceinline__ void lds_load(const uint8_t * base, uint32_t voff, uint32_t lds) {  // N KiB
+    static_assert(N >= 1 && N <= 3, "the offset has 13 bits, signed");
+    if constexpr (N == 1) asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
+    if constexpr (N == 2) asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1\n\tglobal_load_lds_dwordx4 %0, %1 offset:1024" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
+    if constexpr (N == 3) asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1\n\tglobal_load_lds_dwordx4 %0, %1 offset:1024\n\tglobal_load_lds_dwordx4 %0, %1 offset:2048" ::"v"(voff), "s"(base), "s"(lds) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <int D>
 __device__ __forceinline__ void tile_load(const uint8_t * t, uint32_t lds, int lane) {  // (t, lds: uniform)
     constexpr int full = 36 * D / 1024, rest = (36 * D % 1024) / 16;
@@ -188,11 +196,11 @@ __device__ __forceinline__ void tile_load(const uint8_t * t, uint32_t lds, int l
 #pragma unroll
     for (int i = 0; i < full; i += 3) {
         const uint32_t v = 16 * lane + 1024 * i;
-        lds_load<0>(t, v, lds + 1024 * i);
-        if (i + 1 < full) lds_load<1024>(t, v, lds + 1024 * i);
-        if (i + 2 < full) lds_load<2048>(t, v, lds + 1024 * i);
+        if (i + 2 < full) lds_load<3>(t, v, lds + 1024 * i);
+        else if (i + 1 < full) lds_load<2>(t, v, lds + 1024 * i);
+        else lds_load<1>(t, v, lds + 1024 * i);
     }
-    if (rest && lane < rest) lds_load<0>(t, 16 * lane + 1024 * full, lds + 1024 * full);
+    if (rest && lane < rest) lds_load<1>(t, 16 * lane + 1024 * full, lds + 1024 * full);
 }
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }

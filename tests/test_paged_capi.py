@@ -140,3 +140,22 @@ def test_rope_freqs():
     f = ops.rope_freqs(8, 10000.0, 0.5, torch.tensor([1.0, 2.0, 4.0, 8.0]), device="cpu")
     want = [0.5 * 10000.0 ** (-i / 4) / 2 ** i for i in range(4)]
     assert f.dtype == torch.float32 and torch.equal(f, torch.tensor(want, dtype=torch.float64).float())
+
+
+def test_hand_written_loads_declare_what_they_change():
+    """An asm statement that sets m0 says so, and leaves the five wait states that a vector memory access needs behind a v_readlane
+    which may have written its scalar base just before (the compiler counts none of them inside asm)."""
+    found = 0
+    for path in sorted((_lib.LIBRARY.parents[1] / "csrc").glob("*.h*")):
+        text = path.read_text()
+        for m in re.finditer(r"\basm\b(?:\s+volatile)?\s*\(((?:[^()\"]|\"(?:[^\"\\]|\\.)*\"|\([^()]*\))*)\)\s*;", text):
+            code, *operands = re.split(r"(?<!:):(?!:)|::", m.group(1))
+            if "m0" not in code:
+                continue
+            found += 1
+            assert operands and '"m0"' in operands[-1], (path.name, m.group(0))
+            assert "load" in code
+            before = code[:code.index("load")].split("\\n\\t")
+            states = sum(1 + int(i.split()[-1]) if "s_nop" in i else 1 for i in before[:-1])
+            assert states >= 5, (path.name, m.group(0))
+    assert found
