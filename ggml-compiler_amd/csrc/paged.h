@@ -99,6 +99,12 @@ template <int D> __device__ __forceinline__ int paged_k_scale(int t, int b) {
 }
 template <int D> __device__ __forceinline__ int paged_v_scale(int t, int b) { return paged_k_scale<D>(t, b) + 2 * D; }
 
+// A launch's grid: it may hold fewer than 2^32 threads.
+inline unsigned paged_grid(int64_t blocks, int threads) {
+    if (blocks * threads > (int64_t) UINT32_MAX) fail("paged: too many rows and heads");
+    return (unsigned) blocks;
+}
+
 size_t paged_attn_workspace(const Paged & p, int D, int H, int64_t max_rows);
 void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int64_t q_h, int H, int64_t max_rows, int window,
                        float scale, float * out, void * ws, hipStream_t s);

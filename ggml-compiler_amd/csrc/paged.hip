@@ -383,11 +383,6 @@ Paged view(const gcq_paged_cache * c, const gcq_paged_batch * b, int64_t n_rows,
     return p;
 }
 
-unsigned blocks(int64_t waves) {
-    require(waves <= (int64_t) 4 * INT32_MAX, "paged: too many rows and heads");
-    return (unsigned) ((waves + 3) / 4);
-}
-
 // Whether rows are appended eight positions at a time: a sequence fills half an eight at the least, and there are 2^20 values,
 // enough to pay for a workgroup's longer way. (64 sequences, 32 heads and 8 KV heads of 128, rows one by one and by
 // eights: 2 rows each 6.9 and 7.9 us, 4 rows 8.7 and 8.0, 16 rows 21.1 and 10.6; one sequence: 32 rows 4.4 and 6.3, 128 rows
@@ -395,10 +390,8 @@ unsigned blocks(int64_t waves) {
 bool by_eights(const AppendArgs & a, int D) {
     return a.p.n_rows >= 4 * std::min(a.p.n_seq, a.p.n_rows) && (int64_t) a.p.n_rows * (a.H + 2 * a.p.Hkv) * D >= 1 << 20;
 }
-unsigned eight_blocks(const Paged & p) {  // a sequence's rows may begin and end inside an eight
-    const int64_t n = (p.n_rows / 8 + 2 * (int64_t) std::min(p.n_seq, p.n_rows)) * p.Hkv;
-    require(n <= INT32_MAX, "paged: too many rows and heads");
-    return (unsigned) n;
+unsigned eight_blocks(const Paged & p, int threads) {  // a sequence's rows may begin and end inside an eight
+    return paged_grid((p.n_rows / 8 + 2 * (int64_t) std::min(p.n_seq, p.n_rows)) * p.Hkv, threads);
 }
 bool vectors(const float * x, int64_t r, int64_t h) { return aligned(x, 16) && r % 4 == 0 && h % 4 == 0; }
 
@@ -407,17 +400,17 @@ void run_append(const AppendArgs & a, hipStream_t s) {
     const bool full = !a.freqs || a.n_dims == D;
     if (by_eights(a, D) && a.n_dims % 8 == 0 && vectors(a.k, a.k_r, a.k_h) && vectors(a.v, a.v_r, a.v_h) &&
         (!a.q || (vectors(a.q, a.q_r, a.q_h) && aligned(a.q_out, 8)))) {
-        if (full) k_paged_append_eight<D, true><<<eight_blocks(a.p), D, 0, s>>>(a);
-        else k_paged_append_eight<D, false><<<eight_blocks(a.p), D, 0, s>>>(a);
+        if (full) k_paged_append_eight<D, true><<<eight_blocks(a.p, D), D, 0, s>>>(a);
+        else k_paged_append_eight<D, false><<<eight_blocks(a.p, D), D, 0, s>>>(a);
         return;
     }
-    const unsigned grid = blocks((int64_t) a.p.n_rows * a.parts);
+    const unsigned grid = paged_grid(((int64_t) a.p.n_rows * a.parts + 3) / 4, 256);
     if (full) k_paged_append<D, true><<<grid, 256, 0, s>>>(a);
     else k_paged_append<D, false><<<grid, 256, 0, s>>>(a);
 }
 template <int D>
 void run_read(const ReadArgs & a, hipStream_t s) {
-    k_paged_read<D><<<eight_blocks(a.p), D, 0, s>>>(a);
+    k_paged_read<D><<<eight_blocks(a.p, D), D, 0, s>>>(a);
 }
 
 }  // namespace

@@ -688,10 +688,10 @@ size_t workspace_of(const Shape & w, int D) {
 template <int D, int RT>
 void launch(const AttnArgs & a, const Shape & w, hipStream_t s) {
     constexpr int ROWS = 16 * RT, NW = waves(D, ROWS);
-    k_paged_attn<D, RT, NW><<<(unsigned) a.items, 64 * NW, 0, s>>>(a);
+    k_paged_attn<D, RT, NW><<<paged_grid(a.items, 64 * NW), 64 * NW, 0, s>>>(a);
     check_launch("paged attn");
     if (w.most == 1) return;
-    k_paged_merge<D, ROWS><<<(unsigned) a.items, 256, 0, s>>>(a);
+    k_paged_merge<D, ROWS><<<paged_grid(a.items, 256), 256, 0, s>>>(a);
     check_launch("paged attn merge");
 }
 template <int D>

@@ -159,3 +159,14 @@ def test_hand_written_loads_declare_what_they_change():
             states = sum(1 + int(i.split()[-1]) if "s_nop" in i else 1 for i in before[:-1])
             assert states >= 5, (path.name, m.group(0))
     assert found
+
+
+def test_more_threads_than_a_launch_takes():
+    """A launch of 2^32 threads or more is refused here, whatever the driver makes of it."""
+    many = "too many rows and heads"
+    _refused(_append(n_rows=1 << 27), many)                   # by eights
+    _refused(_append(n_rows=1 << 26, k_r=255), many)          # row by row
+    _refused(_read(n_rows=1 << 28), many)
+    _refused(_read(_cache(n_head_kv=65535), n_rows=1 << 13), many)
+    _refused(_attn(n_rows=1 << 28, max_rows=1 << 28, ws_size=1 << 62), many)
+    _refused(_attn(_cache(head_dim=256), n_rows=1 << 28, max_rows=1 << 28, ws_size=1 << 62), many)
