@@ -49,7 +49,7 @@ struct AttnArgs {
     Paged p;
     const _Float16 * q;
     int64_t q_r, q_h;
-    int H, G, window, max_rows, items, target, min_chunk;  // target: workgroups that the splits aim at
+    int H, G, window, max_rows, items, slots, target, min_chunk;  // slots: of part_o, part_ml; target: workgroups that the splits aim at
     float c2;     // |scale| log2(e)
     bool negate;  // the scale is negative
     float * out, * part_o;
@@ -59,7 +59,7 @@ struct AttnArgs {
 
 // What k_paged_merge has to know of a workgroup's row tile.
 struct __align__(32) Part {
-    int ns, split, nr, hk, r0, x0;  // ns 0: no work
+    int ns, split, nr, hk, r0, x0, slot;  // ns 0: no work; slot: where its sums are, if ns > 1
 };
 
 // A sequence's rows, and the tiles of the keys that any of them sees.
@@ -86,11 +86,14 @@ __device__ __forceinline__ int splits(int tiles, int chunk) { return max(1, (til
 
 // The plan, the same in every wavefront: tiles per split, and a sequence's first item. Items of a sequence: [KV
 // head][row tile, the last, which sees most, first][split]. The batch's arrays are read once where the sequences fit the lanes.
+// Items of split row tiles have a slot each for their sums. Those are fewer than 2 target: with u tiles in all items' and a chunk of more than
+// u / cut, a row tile has less than tiles cut / u splits more than one, all of them together less than cut <= target, and a split row tile has
+// at most twice as many splits as that.
 template <int ROWS>
 struct Plan {
     const AttnArgs & a;
     SeqWork w;  // of sequence s0 + lane
-    int chunk, s, base, lane_at;
+    int chunk, s, base, slot, lane_at;
 
     __device__ __forceinline__ Plan(const AttnArgs & args) : a(args) {
         const int lane = threadIdx.x & 63;
@@ -114,24 +117,28 @@ struct Plan {
         const int l = __builtin_amdgcn_readfirstlane(lane_at);
         const auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
         base = __builtin_amdgcn_readfirstlane(base);
+        slot = __builtin_amdgcn_readfirstlane(slot);
         s = __builtin_amdgcn_readfirstlane(s);
         return {pick(w.r0), pick(w.rows), pick(w.tile0), pick(w.tiles), pick(w.rts), pick(w.past)};
     }
-    // To the sequence of item `id`; base: its first.
+    // To the sequence of item `id`; base: its first, slot: that one's.
     __device__ __forceinline__ bool find(int id) {
         const int lane = threadIdx.x & 63;
-        base = 0;
+        base = slot = 0;
         for (int s0 = 0; s0 < a.p.n_seq; s0 += 64) {
             if (s0) w = seq_work<ROWS>(a, s0 + lane);
-            const int n = w.rts * a.p.Hkv * splits(w.tiles, chunk), sum = wave_scan(n);
+            const int ns = splits(w.tiles, chunk), n = w.rts * a.p.Hkv * ns, sum = wave_scan(n);
+            const int m = ns > 1 ? n : 0, sum_m = wave_scan(m);
             const uint64_t at = __ballot(base + sum > id);
             if (at) {
                 lane_at = __builtin_ctzll(at);
                 base += __builtin_amdgcn_readlane(sum - n, lane_at);
+                slot += __builtin_amdgcn_readlane(sum_m - m, lane_at);
                 s = s0 + lane_at;
                 return true;
             }
             base += __builtin_amdgcn_readlane(sum, 63);
+            slot += __builtin_amdgcn_readlane(sum_m, 63);
         }
         return false;
     }
@@ -228,10 +235,11 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
     }
     const SeqWork sw = plan.picked();
     const int ns = splits(sw.tiles, plan.chunk), chunk = (sw.tiles + ns - 1) / ns, id = blockIdx.x - plan.base;
-    const int split = id % ns, rt = sw.rts - 1 - id / ns % sw.rts, hk = id / ns / sw.rts;
+    const int split = id % ns, rt = sw.rts - 1 - id / ns % sw.rts, hk = id / ns / sw.rts, slot_of = plan.slot + id;
 
     const int rows = sw.rows * a.G, x0 = rt * ROWS, nr = min(ROWS, rows - x0);  // this tile's rows
-    if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = {ns, split, nr, hk, sw.r0, x0};
+    if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = {ns, split, nr, hk, sw.r0, x0, slot_of};
+    if (ns > 1 && slot_of >= a.slots) return;  // (arrays that change under the call: no sums outside the workspace)
     const int64_t pos0 = (int64_t) sw.past + x0 / a.G, pos1 = (int64_t) sw.past + (x0 + nr - 1) / a.G;
     // this row tile's keys within the split; tiles below e0 or from e1 on are not seen whole by every row
     const int64_t cap = (int64_t) a.p.max_pages << a.p.shift;
@@ -549,8 +557,8 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
                     *reinterpret_cast<f4_t *>(a.out + ((int64_t) (sw.r0 + xx / a.G) * a.H + hk * a.G + xx % a.G) * D + d) =
                         sum == 0.0f ? f4_t{} : o * inv;
                 } else {
-                    *reinterpret_cast<f4_t *>(a.part_o + ((int64_t) blockIdx.x * ROWS + y0 + y) * D + d) = o;
-                    if (d == 0) a.part_ml[(int64_t) blockIdx.x * ROWS + y0 + y] = make_float2(m, sum);
+                    *reinterpret_cast<f4_t *>(a.part_o + ((int64_t) slot_of * ROWS + y0 + y) * D + d) = o;
+                    if (d == 0) a.part_ml[(int64_t) slot_of * ROWS + y0 + y] = make_float2(m, sum);
                 }
             }
         }
@@ -568,8 +576,8 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a) {
     constexpr int L = D / 4, N1 = 64 / L, N4 = 4 * N1;  // lanes of a split; splits at a time, a wavefront's and all four's
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), d = lane % L;
     const Part w = a.parts[blockIdx.x];
-    const int ns = __builtin_amdgcn_readfirstlane(w.ns), split = __builtin_amdgcn_readfirstlane(w.split), item = blockIdx.x - split;
-    if (ns <= 1 || split >= w.nr || item + ns > a.items) return;  // (the last: starts that do not ascend)
+    const int ns = __builtin_amdgcn_readfirstlane(w.ns), split = __builtin_amdgcn_readfirstlane(w.split), item = __builtin_amdgcn_readfirstlane(w.slot) - split;
+    if (ns <= 1 || split >= w.nr || (int) blockIdx.x - split + ns > a.items || item < 0 || item + ns > a.slots) return;  // (starts that do not ascend)
     __shared__ f4_t so[N4][L];
     __shared__ float2 sml[N4];
     const auto weight = [](float from, float to) { return from == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(from - to); };
@@ -655,7 +663,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a) {
 // How a call is run: row tiles of `rows` rows, splits that aim at `target` workgroups, those resident at once.
 struct Shape {
     int rows, target;
-    int64_t tiles, items, most;  // row tiles and workgroups that may have work; splits of a sequence
+    int64_t tiles, items, slots, most;  // row tiles and workgroups that may have work; sums of splits; splits of a sequence
 };
 Shape shape_of(const Paged & p, int D, int G, int64_t max_rows, int window, int rows) {
     Shape s{};
@@ -670,6 +678,7 @@ Shape shape_of(const Paged & p, int D, int G, int64_t max_rows, int window, int 
     // (two splits of the least size gain nothing and need the join: 501 keys 9.5 us as one split, 10.7 + 3.7 as two)
     s.most = longest <= 2 * kMinChunk ? 1 : (longest + kMinChunk - 1) / kMinChunk;
     s.items = std::min(s.tiles + s.target, s.tiles * s.most);
+    s.slots = std::min<int64_t>(s.items, 2 * s.target);
     return s;
 }
 // Tiles of 32 rows halve the work on K and V; tiles of 16 are more workgroups, of half the length. The larger ones if they
@@ -682,7 +691,7 @@ Shape shape_for(const Paged & p, int D, int G, int64_t max_rows, int window) {
     return wide ? many : few;
 }
 size_t workspace_of(const Shape & w, int D) {
-    return w.most == 1 ? 0 : (size_t) w.items * (w.rows * (D * sizeof(float) + sizeof(float2)) + sizeof(Part));
+    return w.most == 1 ? 0 : (size_t) w.slots * w.rows * (D * sizeof(float) + sizeof(float2)) + (size_t) w.items * sizeof(Part);
 }
 
 template <int D, int RT>
@@ -721,11 +730,11 @@ void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int6
     a.out = out;
     const Shape w = shape_for(p, D, a.G, max_rows, window);
     if (w.items >= INT32_MAX) fail("paged_attn: too many rows and heads");
-    a.items = (int) w.items, a.target = w.target;
+    a.items = (int) w.items, a.slots = (int) w.slots, a.target = w.target;
     a.min_chunk = w.most == 1 ? 1 << 30 : kMinChunk;
     a.part_o = (float *) ws;
-    a.part_ml = (float2 *) (a.part_o + (size_t) w.items * w.rows * D);
-    a.parts = w.most == 1 ? nullptr : (Part *) (a.part_ml + (size_t) w.items * w.rows);
+    a.part_ml = (float2 *) (a.part_o + (size_t) w.slots * w.rows * D);
+    a.parts = w.most == 1 ? nullptr : (Part *) (a.part_ml + (size_t) w.slots * w.rows);
     if (D == 64) run<64>(a, w, s);
     else if (D == 128) run<128>(a, w, s);
     else run<256>(a, w, s);

@@ -777,3 +777,31 @@ def test_attention_scores_past_f32(gops, D, G, rows, past, scale):
                 near = x[:, h] >= x[:, h].max() - x[:, h].abs().max() * 2.0 ** -20
                 o, u = got[c.starts[s] + r, h], v[:len(x)][near]
                 assert ((o >= u.amin(0) - 1e-5) & (o <= u.amax(0) + 1e-5)).all()
+
+
+@pytest.mark.parametrize("rows,past", [
+    ([1] * 70 + [1, 2], [40 + s for s in range(70)] + [16000, 9000]),       # a few sequences split among many that are not
+    ([300, 1, 1, 5], [10, 20000, 17, 12000]), ([1, 1], [0, 24000]), ([1] * 130, [2000 + s for s in range(130)]),
+    ([17] * 40 + [1] * 3, [200] * 40 + [9000, 3, 15000]), ([1000, 700], [0, 9000])])
+@pytest.mark.parametrize("D,Hkv,G", [(64, 2, 3), (128, 8, 4), (256, 1, 2)])
+def test_attention_keeps_to_its_workspace(gops, D, Hkv, G, rows, past):
+    """The bytes asked for, holding NaNs before, and none beyond them: sums of split row tiles beside tiles that are not split."""
+    import ctypes
+
+    from ggml_compiler_amd import _lib
+
+    c = Case(gops, rows, past, Hkv, D, 256, seed=47)
+    c.fill_past()
+    q = torch.randn((c.n, G * Hkv, D), device="cuda").half()
+    lib, b, most = _lib.load(), c.batch(), max(rows)
+    wide = gops.PagedBatch(torch.nn.functional.pad(b.pages, (0, 1024), value=-1).contiguous(), b.starts, b.past)
+    for batch in (b, wide):  # (a wider table: more workgroups than have work)
+        at = ctypes.addressof(c.cache._c), ctypes.addressof(batch._c)
+        n = lib.gcq_paged_attn_workspace(*at, c.n, G * Hkv, most)
+        buf = torch.full(((n + 255) // 256 * 256 + 4096,), 0xFF, dtype=torch.uint8, device="cuda")
+        out = torch.full((c.n, G * Hkv, D), 77.0, device="cuda")
+        _lib.check(lib.gcq_paged_attn(*at, c.n, q.data_ptr(), q.stride(0), q.stride(1), G * Hkv, most, 0, D ** -0.5, out.data_ptr(),
+                                      buf.data_ptr(), n, torch.cuda.current_stream().cuda_stream))
+        assert bool((buf[n:] == 0xFF).all())
+        want, bound = attn_reference(c, q, D ** -0.5)
+        check_attn(c, out, want, bound, max(p + r for r, p in zip(rows, past)))

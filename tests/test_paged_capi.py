@@ -170,3 +170,13 @@ def test_more_threads_than_a_launch_takes():
     _refused(_read(_cache(n_head_kv=65535), n_rows=1 << 13), many)
     _refused(_attn(n_rows=1 << 28, max_rows=1 << 28, ws_size=1 << 62), many)
     _refused(_attn(_cache(head_dim=256), n_rows=1 << 28, max_rows=1 << 28, ws_size=1 << 62), many)
+
+
+def test_attn_workspace_does_not_grow_with_the_rows():
+    """Sums are kept of split row tiles alone, whose number the plan bounds; a note of 32 bytes for each workgroup besides."""
+    lib, c = _lib.load(), _cache(n_head_kv=8, n_pages=1 << 20)
+    b = _batch(max_pages=2048, ld_pages=2048, n_seq=1)
+    at = ctypes.addressof(c), ctypes.addressof(b)
+    for n in (8192, 65536):
+        # a workgroup to 16 rows of a KV head; two times 1024 sums of 16 rows, or 768 of 32
+        assert lib.gcq_paged_attn_workspace(*at, n, 32, n) <= n * 4 // 16 * 8 * 32 + 1024 * 32 + 2 * 768 * 32 * (128 * 4 + 8) + (1 << 20)
