@@ -805,3 +805,55 @@ def test_attention_keeps_to_its_workspace(gops, D, Hkv, G, rows, past):
         assert bool((buf[n:] == 0xFF).all())
         want, bound = attn_reference(c, q, D ** -0.5)
         check_attn(c, out, want, bound, max(p + r for r, p in zip(rows, past)))
+
+
+@pytest.mark.parametrize("S,most,H", [(65, 1, 4), (128, 1, 4), (200, 1, 4), (130, 9, 16), (70, 40, 16), (300, 5, 16)])
+@pytest.mark.parametrize("D,n_dims", [(64, 64), (128, 40)])
+def test_append_more_sequences_than_lanes(gops, orc, S, most, H, D, n_dims):
+    """Rows one by one and by eights, some sequences without any: all that is held and given against the encoder, all else as it was."""
+    rng = np.random.default_rng(S)
+    rows = [1 if most == 1 else int(r) for r in rng.integers(max(1, most - 2), most + 1, S)]
+    for s in (0, 3, 63, 64, S - 1):
+        rows[s] = 0 if s != 64 else most
+    past = [int(p) for p in rng.integers(0, 100, S)]
+    c = Case(gops, rows, past, 2, D, 32, seed=S + D, extra_rows=2, fill=0xA5)
+    x = c.rng.standard_normal((c.n, H + 4, D)).astype(np.float32)
+    t = torch.from_numpy(x).cuda()
+    freqs = gops.rope_freqs(n_dims, 10000.0)
+    q_out = torch.full((c.n, H, D), 5.0, dtype=torch.float16, device="cuda")
+    gops.paged_append(c.cache, c.batch(), t[:, H:H + 2], t[:, H + 2:], q=t[:, :H], freqs=freqs, q_out=q_out)
+    k, v = gops.paged_read(c.cache, c.batch(), c.n)
+    n, f = int(c.starts[-1]), freqs.cpu().numpy()
+    assert np.array_equal(q_out[:n].cpu().numpy(), rotated(x[:n, :H], positions(c), f).astype(np.float16))
+    assert (q_out[n:] == 5.0).all()
+    assert np.array_equal(k[:n].cpu().numpy(), q4_values(orc, rotated(x[:n, H:H + 2], positions(c), f)))
+    assert np.array_equal(v[:n].cpu().numpy(), q4_values(orc, np.ascontiguousarray(x[:n, H + 2:])))
+    got = c.cache.data.cpu().numpy()
+    rest = np.ones(got.shape, bool)
+    rest[layout_bytes(c, [(s, past[s] + j) for s in range(S) for j in range(rows[s])])] = False
+    assert (got[rest] == 0xA5).all()
+
+
+@pytest.mark.parametrize("window", [0, 40, 3000])
+def test_attention_of_rows_past_the_table(gops, window):
+    """Rows at positions that the page table has no entry for see the keys it has, as far as the window reaches them."""
+    Hkv, G, D, page, pages = 2, 4, 128, 32, 6
+    rows, past = [1, 5, 1, 40, 1], [pages * page, pages * page + 20, 2000000000, pages * page - 10, 2500]
+    c = Case(gops, [pages * page] * 5, [0] * 5, Hkv, D, page, seed=48, extra_cols=0)
+    c.fill_past()
+    q = torch.from_numpy(c.rng.standard_normal((sum(rows), G * Hkv, D)).astype(np.float32)).cuda().half()
+    got = gops.paged_attn(c.cache, c.batch(rows, past), q, D ** -0.5, max_rows=40, window=window)
+    at = 0
+    for s, (r, p) in enumerate(zip(rows, past)):
+        k, v = (x[c.key0[s]:c.key0[s + 1]] for x in (c.k, c.v))
+        for j in range(r):
+            pos = p + j
+            lo, hi = max(0, pos - window + 1) if window else 0, min(pos + 1, pages * page)
+            for h in range(G * Hkv):
+                if lo >= hi:
+                    assert (got[at, h] == 0).all()
+                    continue
+                w = torch.softmax(k[lo:hi, h // G] @ q[at, h].double() * D ** -0.5, 0)
+                want = w @ v[lo:hi, h // G]
+                assert ((got[at, h].double() - want).norm() <= 2.0 ** -18 * want.norm()).item()
+            at += 1
