@@ -156,8 +156,9 @@ struct Eight {
 // hk + Hkv, .. A thread has four pairs of one row for all of those heads, their sines in registers; the eight tokens' bytes are
 // put together in LDS and leave as 16-byte pieces, where a row at a time writes V's one by one. (By eights and not by whole tiles:
 // four times the workgroups, whose waits overlap; 8192 rows of 16 heads, 8 + 8 KV heads of 256: 85 us, by tiles 121.) 3998 rows of 32
-// heads, 8 + 8 KV heads of 128: 31 us for 140 MB, 4.5 TB/s, where a large copy reaches 5.1; 7 us of it are the rotation's 64-bit
-// operations.
+// heads, 8 + 8 KV heads of 128: 31 us for 136 MB, 4.4 TB/s, where a large copy reaches 5.1; 7 us of it are the rotation's 64-bit
+// operations. Of a part of the dims (FULL false) partners are loaded besides and there are sines for both: 64 of 128 dims 31 us as well,
+// 128 of 256 dims, 8192 rows of 16 heads, 98 us for 81.
 template <int D, bool FULL>
 __global__ __launch_bounds__(D) void k_paged_append_eight(const AppendArgs a) {
     constexpr int L = D / 8, QB = FULL ? 2 : 1;  // threads of a row; q heads under way at a time, as the registers allow

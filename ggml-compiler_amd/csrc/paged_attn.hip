@@ -19,12 +19,13 @@
 // launch, and a captured graph follows the arrays), finds its split by a prefix sum over the sequences and joins its wavefronts'
 // sums in LDS. Row tiles of several splits are joined by k_paged_merge, from notes (Part) that the workgroups leave.
 //
-// What bounds it: the vector ALU. A tile of heads of 128 costs a wavefront some 335 operations at 16 rows: 216 to make its 4-bit
-// codes into MFMA operands, whatever the rows, the others for 16 rows' scaling, softmax and sums. Reads alone, all
-// arithmetic left out, took 25 us of 131071 keys' 39 (one row of 32 heads, 8 KV heads, 151 MB: 3.9 TB/s) and 15 us of 27 for 32
-// sequences of 200 to 8191 keys. 512 rows over 4096 keys take 95 us (339 TFLOP/s of 4 D flops a key and row; the MFMAs do twice
-// those, for the parts). That is also why a wavefront has all of its rows' dims: shared between wavefronts by way of LDS, the
-// operands of a tile took longer to write there (34 cycles a KiB of a CU's) than to make again.
+// What bounds it: where wavefronts have many tiles the vector ALU. A tile of heads of 128 costs a wavefront some 335 operations at 16
+// rows: 216 to make its 4-bit codes into MFMA operands, whatever the rows, the others for 16 rows' scaling, softmax and sums.
+// Reads alone, all arithmetic left out, took 25 us of 131071 keys' 39 (one row of 32 heads, 8 KV heads, 151 MB: 3.8 TB/s). With few
+// tiles to a wavefront, plan, lookups, the first tile and the join weigh as much: 26 us for 32 sequences of 232 to 7611 keys, 15 of
+// them reads alone, 11 the tiles' operations. 512 rows over 4096 keys take 88 us (365 TFLOP/s of 4 D flops a key and row; the
+// MFMAs do twice those, for the parts). The ALU is also why a wavefront has all of its rows' dims: shared between wavefronts by
+// way of LDS, the operands of a tile took longer to write there (34 cycles a KiB of a CU's) than to make again.
 #include "paged.h"
 
 #include <algorithm>
@@ -618,7 +619,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a) {
     };
     f4_t acc;
     float R, l;
-    if (ns > 8 * N1) {  // (one or two rows: at most 32 of them)
+    if (ns > 8 * N1) {  // (one or two rows of the tile's 32 at most, heads of 256 up to four)
         for (int y = split; y < w.nr; y += ns) {
             row(y, tid / L, N4, acc, R, l);
             so[tid / L][d] = acc;

@@ -8,7 +8,7 @@ stands for and its reference call site are named per function.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 
 import torch
 

@@ -17,7 +17,7 @@
  * stands for tokens that are not there: append drops them, attention does not see them, read gives
  * zeros. These arrays live on the device and are read by the kernels: a captured graph follows their
  * contents from replay to replay. Sequences may share pages that a call only reads; two rows of one
- * call that append to the same slot leave either's codes there. A call that takes a launch of 2^32 threads or more (some 2^26 rows) is
+ * call that append to the same slot leave some of either's bytes there. A call that takes a launch of 2^32 threads or more (some 2^26 rows) is
  * refused.
  */
 #ifndef GCQ_PAGED_H
