@@ -12,6 +12,8 @@
 
 #include "gcq_common.h"
 
+#include "../../include/gcq_paged.h"
+
 namespace gcq {
 
 constexpr int kPagedTile = 32;
@@ -105,8 +107,20 @@ inline unsigned paged_grid(int64_t blocks, int threads) {
     return (unsigned) blocks;
 }
 
+// Checks (paged.hip): a message only where one fails; cache and batch, checked, as the kernels take them.
+void paged_require(bool ok, const char * message);
+void paged_need(const void * p, const char * what, size_t align = 1);
+Paged paged_view(const gcq_paged_cache * c, const gcq_paged_batch * b, int64_t n_rows, bool pointers = true);
+
+// What the rows of draft trees see of each other (include/gcq_draft.h); mask null: rows are lines of text.
+struct PagedTree {
+    const int32_t * positions;
+    const uint32_t * mask;
+    int ld;
+};
+
 size_t paged_attn_workspace(const Paged & p, int D, int H, int64_t max_rows);
 void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int64_t q_h, int H, int64_t max_rows, int window,
-                       float scale, float * out, void * ws, hipStream_t s);
+                       float scale, const PagedTree & tree, float * out, void * ws, hipStream_t s);
 
 }  // namespace gcq

@@ -1,11 +1,11 @@
 // paged.hip - the paged 4-bit key / value cache: append with rotation, read back, and the C ABI
-// (include/gcq_paged.h; layout in paged.h).
+// (include/gcq_paged.h, and include/gcq_draft.h's for rows of draft trees; layout in paged.h).
 #include "paged.h"
 
 #include <algorithm>
 #include <cmath>
 
-#include "../../include/gcq_paged.h"
+#include "../../include/gcq_draft.h"
 
 namespace gcq {
 
@@ -17,6 +17,7 @@ struct AppendArgs {
     int64_t k_r, k_h, v_r, v_h, q_r, q_h;
     _Float16 * q_out;
     const float * freqs;
+    const int32_t * positions;  // of the rows, null: their slots
     float attn_factor;
     int H, n_dims, per, parts;  // heads (of H + 2 Hkv) per wavefront, wavefronts per row
 };
@@ -51,7 +52,8 @@ __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
     if (r >= a.p.n_rows) return;  // whole wavefronts
     const int s = paged_seq(a.p, r);
     if (s < 0) return;
-    const int64_t pos = (int64_t) a.p.past[s] + (r - a.p.starts[s]);
+    const int64_t pos = (int64_t) a.p.past[s] + (r - a.p.starts[s]);  // the slot
+    const int64_t turn_pos = a.positions ? a.positions[r] : pos;
     const int h0 = (int) (unit % a.parts) * a.per, h1 = min(h0 + a.per, a.H + 2 * a.p.Hkv);
     const int slot = (int) pos & 31;
 
@@ -67,7 +69,7 @@ __global__ __launch_bounds__(256) void k_paged_append(const AppendArgs a) {
             cs[c] = 1.0;
             sn[c] = 0.0;
             if (FULL || e < a.n_dims) {
-                sincos((double) pos * (double) a.freqs[!FULL && e >= half ? e - half : e], &sn[c], &cs[c]);
+                sincos((double) turn_pos * (double) a.freqs[!FULL && e >= half ? e - half : e], &sn[c], &cs[c]);
                 cs[c] *= (double) a.attn_factor;
                 sn[c] *= (double) a.attn_factor;
             }
@@ -169,6 +171,7 @@ __global__ __launch_bounds__(D) void k_paged_append_eight(const AppendArgs a) {
     const int64_t pos = w.eight * 8 + m8, j = pos - w.past;
     const bool on = j >= 0 && j < w.rows;
     const int64_t r = w.r0 + (on ? j : 0);
+    const int64_t turn_pos = a.positions && on ? a.positions[r] : pos;
     const int half = a.n_dims / 2;
 
     // of dims i .. i + 3 and i + D / 2 ..: values, and partners (FULL: each other)
@@ -205,7 +208,7 @@ __global__ __launch_bounds__(D) void k_paged_append_eight(const AppendArgs a) {
                 cs[c][e] = 1.0;
                 sn[c][e] = 0.0;
                 if (FULL || d < a.n_dims) {
-                    sincos((double) pos * (double) a.freqs[!FULL && d >= half ? d - half : d], &sn[c][e], &cs[c][e]);
+                    sincos((double) turn_pos * (double) a.freqs[!FULL && d >= half ? d - half : d], &sn[c][e], &cs[c][e]);
                     cs[c][e] *= (double) a.attn_factor;
                     sn[c][e] *= !FULL && d < half ? -(double) a.attn_factor : (double) a.attn_factor;
                 }
@@ -348,33 +351,35 @@ __global__ __launch_bounds__(D) void k_paged_read(const ReadArgs a) {
 
 // ---------------------------------------------------------------------------------- checks
 
-// (messages are put together only where a check fails: a launch costs the host some 3 us, a call's strings were one more)
-void require(bool ok, const char * message) {
-    if (!ok) fail(message);
-}
-void need(const void * p, const char * what, size_t align = 1) {
-    if (!p) fail(std::string("paged: ") + what + " is NULL");
-    if (!aligned(p, align)) fail(std::string("paged: ") + what + " must be " + std::to_string(align) + "-byte aligned");
-}
-
 bool shape_ok(int n_pages, int page, int Hkv, int D) {
     return n_pages > 0 && Hkv > 0 && Hkv <= 65535 && (page == 32 || page == 64 || page == 128 || page == 256) &&
            (D == 64 || D == 128 || D == 256);
 }
 
-Paged view(const gcq_paged_cache * c, const gcq_paged_batch * b, int64_t n_rows, bool pointers = true) {
-    need(c, "cache");
-    need(b, "batch");
-    require(shape_ok(c->n_pages, c->page_size, c->n_head_kv, c->head_dim),
+}  // namespace
+
+// (messages are put together only where a check fails: a launch costs the host some 3 us, a call's strings were one more)
+void paged_require(bool ok, const char * message) {
+    if (!ok) fail(message);
+}
+void paged_need(const void * p, const char * what, size_t align) {
+    if (!p) fail(std::string("paged: ") + what + " is NULL");
+    if (!aligned(p, align)) fail(std::string("paged: ") + what + " must be " + std::to_string(align) + "-byte aligned");
+}
+
+Paged paged_view(const gcq_paged_cache * c, const gcq_paged_batch * b, int64_t n_rows, bool pointers) {
+    paged_need(c, "cache");
+    paged_need(b, "batch");
+    paged_require(shape_ok(c->n_pages, c->page_size, c->n_head_kv, c->head_dim),
             "paged: pages of 32, 64, 128 or 256 tokens, heads of 64, 128 or 256 values, at least one page and KV head");
-    require(b->n_seq > 0 && b->max_pages > 0 && b->ld_pages >= b->max_pages,
+    paged_require(b->n_seq > 0 && b->max_pages > 0 && b->ld_pages >= b->max_pages,
             "paged: a batch has at least one sequence and one page each, ld_pages >= max_pages");
-    require(n_rows >= 0 && n_rows < (1 << 30), "paged: n_rows out of range");
+    paged_require(n_rows >= 0 && n_rows < (1 << 30), "paged: n_rows out of range");
     if (pointers) {
-        need(c->data, "cache data", 16);
-        need(b->pages, "pages", 4);
-        need(b->starts, "starts", 4);
-        need(b->past, "past", 4);
+        paged_need(c->data, "cache data", 16);
+        paged_need(b->pages, "pages", 4);
+        paged_need(b->starts, "starts", 4);
+        paged_need(b->past, "past", 4);
     }
     Paged p{};
     p.data = (uint8_t *) c->data;
@@ -383,6 +388,8 @@ Paged view(const gcq_paged_cache * c, const gcq_paged_batch * b, int64_t n_rows,
     p.n_seq = b->n_seq, p.max_pages = b->max_pages, p.n_rows = (int) n_rows;
     return p;
 }
+
+namespace {
 
 // Whether rows are appended eight positions at a time: a sequence fills half an eight at the least, and there are 2^20 values,
 // enough to pay for a workgroup's longer way. (64 sequences, 32 heads and 8 KV heads of 128, rows one by one and by
@@ -414,6 +421,61 @@ void run_read(const ReadArgs & a, hipStream_t s) {
     k_paged_read<D><<<eight_blocks(a.p, D), D, 0, s>>>(a);
 }
 
+// (positions null: the rows' slots)
+void append(const gcq_paged_cache * cache, const gcq_paged_batch * batch, int64_t n_rows, const int32_t * positions,
+            const float * k, int64_t k_r, int64_t k_h, const float * v, int64_t v_r, int64_t v_h, const float * q,
+            int64_t q_r, int64_t q_h, int n_head, void * q_out, const float * freqs, int n_dims, float attn_factor,
+            void * stream) {
+    AppendArgs a{};
+    a.p = paged_view(cache, batch, n_rows);
+    if (n_rows == 0) return;
+    const int D = cache->head_dim;
+    paged_need(k, "k", 4);
+    paged_need(v, "v", 4);
+    paged_require(k_r >= 0 && k_h >= 0 && v_r >= 0 && v_h >= 0 && q_r >= 0 && q_h >= 0, "paged_append: negative strides");
+    if (q) {
+        paged_need(q, "q", 4);
+        paged_need(q_out, "q_out", 2);
+        paged_require(n_head > 0 && n_head <= 65535, "paged_append: n_head must be positive");
+    }
+    if (freqs) {
+        paged_need(freqs, "freqs", 4);
+        paged_require(n_dims > 0 && n_dims % 2 == 0 && n_dims <= D, "paged_append: n_dims must be even and <= head_dim");
+        paged_require(std::isfinite(attn_factor), "paged_append: attn_factor must be finite");
+    }
+    a.k = k, a.k_r = k_r, a.k_h = k_h, a.v = v, a.v_r = v_r, a.v_h = v_h;
+    a.q = q, a.q_r = q_r, a.q_h = q_h, a.H = q ? n_head : 0, a.q_out = (_Float16 *) q_out;
+    a.positions = positions, a.freqs = freqs, a.n_dims = freqs ? n_dims : D, a.attn_factor = attn_factor;
+    const int64_t heads = a.H + 2 * a.p.Hkv;
+    // wavefronts: about 4096, one per row at the least
+    a.per = (int) std::max<int64_t>(1, std::min(heads, heads * n_rows / 4096));
+    if (D == 64) a.per = (a.per + 1) / 2 * 2;
+    a.parts = (int) ((heads + a.per - 1) / a.per);
+    hipStream_t s = as_stream(stream);
+    if (D == 64) run_append<64>(a, s);
+    else if (D == 128) run_append<128>(a, s);
+    else run_append<256>(a, s);
+    check_launch("paged append");
+}
+
+void attn(const gcq_paged_cache * cache, const gcq_paged_batch * batch, int64_t n_rows, const PagedTree & tree, const void * q,
+          int64_t q_r, int64_t q_h, int n_head, int64_t max_rows, int window, float scale, float * out, void * ws, size_t ws_size,
+          void * stream) {
+    const Paged p = paged_view(cache, batch, n_rows);
+    if (n_rows == 0) return;
+    paged_need(q, "q", 16);
+    paged_need(out, "out", 16);
+    paged_need(ws, "workspace", 256);
+    paged_require(n_head > 0 && n_head <= 65535 && n_head % p.Hkv == 0, "paged_attn: n_head must be a multiple of n_head_kv");
+    paged_require(q_r >= 0 && q_h >= 0 && q_r % 8 == 0 && q_h % 8 == 0, "paged_attn: q strides must be multiples of 8");
+    paged_require(max_rows > 0, "paged_attn: max_rows must be positive");
+    paged_require(window >= 0, "paged_attn: window must not be negative");
+    paged_require(std::isfinite(scale), "paged_attn: scale must be finite");
+    const size_t need_ws = std::max<size_t>(256, paged_attn_workspace(p, cache->head_dim, n_head, max_rows));
+    if (ws_size < need_ws) fail("workspace of " + std::to_string(ws_size) + " bytes, need " + std::to_string(need_ws));
+    launch_paged_attn(p, cache->head_dim, q, q_r, q_h, n_head, max_rows, window, scale, tree, out, ws, as_stream(stream));
+}
+
 }  // namespace
 
 }  // namespace gcq
@@ -435,46 +497,27 @@ int gcq_paged_append(const gcq_paged_cache * cache, const gcq_paged_batch * batc
                      int64_t q_h, int n_head, void * q_out, const float * freqs, int n_dims, float attn_factor,
                      void * stream) {
     return guarded([&] {
-        AppendArgs a{};
-        a.p = view(cache, batch, n_rows);
-        if (n_rows == 0) return;
-        const int D = cache->head_dim;
-        need(k, "k", 4);
-        need(v, "v", 4);
-        require(k_r >= 0 && k_h >= 0 && v_r >= 0 && v_h >= 0 && q_r >= 0 && q_h >= 0, "paged_append: negative strides");
-        if (q) {
-            need(q, "q", 4);
-            need(q_out, "q_out", 2);
-            require(n_head > 0 && n_head <= 65535, "paged_append: n_head must be positive");
-        }
-        if (freqs) {
-            need(freqs, "freqs", 4);
-            require(n_dims > 0 && n_dims % 2 == 0 && n_dims <= D, "paged_append: n_dims must be even and <= head_dim");
-            require(std::isfinite(attn_factor), "paged_append: attn_factor must be finite");
-        }
-        a.k = k, a.k_r = k_r, a.k_h = k_h, a.v = v, a.v_r = v_r, a.v_h = v_h;
-        a.q = q, a.q_r = q_r, a.q_h = q_h, a.H = q ? n_head : 0, a.q_out = (_Float16 *) q_out;
-        a.freqs = freqs, a.n_dims = freqs ? n_dims : D, a.attn_factor = attn_factor;
-        const int64_t heads = a.H + 2 * a.p.Hkv;
-        // wavefronts: about 4096, one per row at the least
-        a.per = (int) std::max<int64_t>(1, std::min(heads, heads * n_rows / 4096));
-        if (D == 64) a.per = (a.per + 1) / 2 * 2;
-        a.parts = (int) ((heads + a.per - 1) / a.per);
-        hipStream_t s = as_stream(stream);
-        if (D == 64) run_append<64>(a, s);
-        else if (D == 128) run_append<128>(a, s);
-        else run_append<256>(a, s);
-        check_launch("paged append");
+        append(cache, batch, n_rows, nullptr, k, k_r, k_h, v, v_r, v_h, q, q_r, q_h, n_head, q_out, freqs, n_dims, attn_factor, stream);
+    });
+}
+
+int gcq_paged_append_at(const gcq_paged_cache * cache, const gcq_paged_batch * batch, int64_t n_rows,
+                        const int32_t * positions, const float * k, int64_t k_r, int64_t k_h, const float * v, int64_t v_r,
+                        int64_t v_h, const float * q, int64_t q_r, int64_t q_h, int n_head, void * q_out, const float * freqs,
+                        int n_dims, float attn_factor, void * stream) {
+    return guarded([&] {
+        if (n_rows) paged_need(positions, "positions", 4);
+        append(cache, batch, n_rows, positions, k, k_r, k_h, v, v_r, v_h, q, q_r, q_h, n_head, q_out, freqs, n_dims, attn_factor, stream);
     });
 }
 
 int gcq_paged_read(const gcq_paged_cache * cache, const gcq_paged_batch * batch, int64_t n_rows, float * k, float * v,
                    void * stream) {
     return guarded([&] {
-        ReadArgs a{view(cache, batch, n_rows), k, v};
+        ReadArgs a{paged_view(cache, batch, n_rows), k, v};
         if (n_rows == 0) return;
-        need(k, "k", 16);
-        need(v, "v", 16);
+        paged_need(k, "k", 16);
+        paged_need(v, "v", 16);
         hipStream_t s = as_stream(stream);
         if (cache->head_dim == 64) run_read<64>(a, s);
         else if (cache->head_dim == 128) run_read<128>(a, s);
@@ -487,9 +530,9 @@ size_t gcq_paged_attn_workspace(const gcq_paged_cache * cache, const gcq_paged_b
                                 int64_t max_rows) {
     size_t n = 0;
     guarded([&] {
-        const Paged p = view(cache, batch, n_rows, false);
-        require(n_head > 0 && n_head % p.Hkv == 0, "paged_attn: n_head must be a multiple of n_head_kv");
-        require(max_rows > 0, "paged_attn: max_rows must be positive");
+        const Paged p = paged_view(cache, batch, n_rows, false);
+        paged_require(n_head > 0 && n_head % p.Hkv == 0, "paged_attn: n_head must be a multiple of n_head_kv");
+        paged_require(max_rows > 0, "paged_attn: max_rows must be positive");
         n = std::max<size_t>(256, paged_attn_workspace(p, cache->head_dim, n_head, max_rows));
     });
     return n;
@@ -498,20 +541,19 @@ size_t gcq_paged_attn_workspace(const gcq_paged_cache * cache, const gcq_paged_b
 int gcq_paged_attn(const gcq_paged_cache * cache, const gcq_paged_batch * batch, int64_t n_rows, const void * q,
                    int64_t q_r, int64_t q_h, int n_head, int64_t max_rows, int window, float scale, float * out, void * ws,
                    size_t ws_size, void * stream) {
+    return guarded([&] { attn(cache, batch, n_rows, {}, q, q_r, q_h, n_head, max_rows, window, scale, out, ws, ws_size, stream); });
+}
+
+int gcq_paged_attn_tree(const gcq_paged_cache * cache, const gcq_paged_batch * batch, int64_t n_rows,
+                        const int32_t * positions, const uint32_t * mask, int64_t ld_mask, const void * q, int64_t q_r,
+                        int64_t q_h, int n_head, int64_t max_rows, int window, float scale, float * out, void * ws,
+                        size_t ws_size, void * stream) {
     return guarded([&] {
-        const Paged p = view(cache, batch, n_rows);
-        if (n_rows == 0) return;
-        need(q, "q", 16);
-        need(out, "out", 16);
-        need(ws, "workspace", 256);
-        require(n_head > 0 && n_head <= 65535 && n_head % p.Hkv == 0, "paged_attn: n_head must be a multiple of n_head_kv");
-        require(q_r >= 0 && q_h >= 0 && q_r % 8 == 0 && q_h % 8 == 0, "paged_attn: q strides must be multiples of 8");
-        require(max_rows > 0, "paged_attn: max_rows must be positive");
-        require(window >= 0, "paged_attn: window must not be negative");
-        require(std::isfinite(scale), "paged_attn: scale must be finite");
-        const size_t need_ws = std::max<size_t>(256, paged_attn_workspace(p, cache->head_dim, n_head, max_rows));
-        if (ws_size < need_ws) fail("workspace of " + std::to_string(ws_size) + " bytes, need " + std::to_string(need_ws));
-        launch_paged_attn(p, cache->head_dim, q, q_r, q_h, n_head, max_rows, window, scale, out, ws, as_stream(stream));
+        if (n_rows) paged_need(mask, "mask", 4);
+        if (n_rows && window) paged_need(positions, "positions", 4);
+        paged_require(ld_mask > 0 && ld_mask <= GCQ_DRAFT_MAX_ROWS / 32, "paged_attn_tree: ld_mask must be 1 .. 32");
+        paged_require(std::min(max_rows, n_rows) <= 32 * ld_mask, "paged_attn_tree: max_rows past the mask's bits");
+        attn(cache, batch, n_rows, {positions, mask, (int) ld_mask}, q, q_r, q_h, n_head, max_rows, window, scale, out, ws, ws_size, stream);
     });
 }
 

@@ -53,6 +53,7 @@ struct AttnArgs {
     int H, G, window, max_rows, items, slots, target, min_chunk;  // slots: of part_o, part_ml; target: workgroups that the splits aim at
     float c2;     // |scale| log2(e)
     bool negate;  // the scale is negative
+    PagedTree tree;
     float * out, * part_o;
     float2 * part_ml;
     struct Part * parts;  // one for each workgroup; null: nothing is split
@@ -219,7 +220,9 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 constexpr int per_simd(int D, int RT) { return D * RT <= 128 ? 4 : D * RT == 256 && RT == 2 ? 3 : 2; }
 constexpr int waves(int D, int rows) { return D == 256 && rows == 32 ? 8 : 4; }
 
-template <int D, int RT, int NW>
+// TREE: the rows see the slots below past (a window's part of them) and those new rows that their masks name. Tiles of slots below
+// past alone are any row's; of the others, the last few, a row's 32 keys come as a word of ones shifted into its mask's.
+template <int D, int RT, int NW, bool TREE>
 __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const AttnArgs a) {
     constexpr int ROWS = 16 * RT, NB = D / 32, NT = D / 16, RING = 2, NL = kTileLoads<D>, P = D + 4;
     // LDS: the wavefronts' rings (then their sums of 16 rows), and the row tile's Q as MFMA operands (from two times 16
@@ -241,12 +244,23 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
     const int rows = sw.rows * a.G, x0 = rt * ROWS, nr = min(ROWS, rows - x0);  // this tile's rows
     if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = {ns, split, nr, hk, sw.r0, x0, slot_of};
     if (ns > 1 && slot_of >= a.slots) return;  // (arrays that change under the call: no sums outside the workspace)
-    const int64_t pos0 = (int64_t) sw.past + x0 / a.G, pos1 = (int64_t) sw.past + (x0 + nr - 1) / a.G;
+    // the slots of its first and last row; of a tree, the last slot that any row may see, and the first and last row's positions as
+    // far as a window goes
+    const int64_t pos0 = TREE ? sw.past : (int64_t) sw.past + x0 / a.G, pos1 = TREE ? (int64_t) sw.past + sw.rows - 1 : (int64_t) sw.past + (x0 + nr - 1) / a.G;
+    const auto row_of = [&](int y) { return sw.r0 + (x0 + min(y, nr - 1)) / a.G; };
+    int64_t top_pos = pos1;
+    if (TREE && a.window) {
+        int m = sw.past;
+        for (int y = lane; y < ROWS; y += 64) m = max(m, a.tree.positions[row_of(y)]);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
+        top_pos = m;
+    }
     // this row tile's keys within the split; tiles below e0 or from e1 on are not seen whole by every row
     const int64_t cap = (int64_t) a.p.max_pages << a.p.shift;
     const int first = max(sw.tile0 + split * chunk, a.window && pos0 - a.window + 1 > 0 ? (int) ((pos0 - a.window + 1) >> 5) : 0);
     const int last = min(sw.tile0 + min(sw.tiles, (split + 1) * chunk), (int) ((min(pos1 + 1, cap) + 31) >> 5));
-    const int e0 = a.window ? (int) ((pos1 - a.window) >> 5) + 1 : 0, e1 = (int) ((pos0 + 1) >> 5);
+    const int e0 = a.window ? (int) ((top_pos - a.window) >> 5) + 1 : 0, e1 = (int) ((TREE ? pos0 : pos0 + 1) >> 5);
 
     // The tiles of this wavefront: first + wave, + NW, ..; lane i holds the address of tile k0 + i, 0 for one that is not there.
     const int n = first + wave < last ? (last - first - wave + NW - 1) / NW : 0;
@@ -383,6 +397,35 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
             }
 
             if (tile < e0 || tile >= e1) {  // keys that some row does not see
+                uint32_t any = 0;  // TREE: the tile's keys that some row sees
+                if constexpr (TREE) {
+                    const int64_t rel = 32 * (int64_t) tile - sw.past, left = min(pos1 + 1, cap) - 32 * (int64_t) tile;  // the first key's bit; keys
+                    const int w0 = (int) max(rel >> 5, (int64_t) -1), sh = (int) rel & 31;
+#pragma unroll
+                    for (int i = 0; i < RA; i++) {
+                        const int r = row_of(16 * i + lr);
+                        const uint32_t * m = a.tree.mask + (int64_t) r * a.tree.ld;
+                        uint32_t bits = ~0u;
+                        if (rel > -32) {
+                            const uint32_t u = w0 >= 0 ? (w0 < a.tree.ld ? m[w0] : 0) : ~0u, v = w0 + 1 < a.tree.ld ? m[w0 + 1] : 0;
+                            bits = (uint32_t) ((((uint64_t) v << 32) | u) >> sh);
+                            if (left < 32) bits &= left > 0 ? (1u << left) - 1 : 0;
+                        }
+                        if (a.window && rel < 0) {  // of the past
+                            const int64_t cut = min((int64_t) max(a.tree.positions[r], sw.past) - a.window + 1 - 32 * (int64_t) tile, -rel);
+                            if (cut > 0) bits &= cut < 32 ? ~0u << cut : 0;
+                        }
+                        any |= bits;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int key = (e & 4) | (e & 1) << 1 | (e >> 1 & 1);  // order(e)
+                            S[i][e] = bits >> (8 * g + key) & 1 ? S[i][e] : -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int o = 1; o < 16; o <<= 1) any |= __shfl_xor(any, o, 64);  // (all rows of the lane's g)
+                    any >>= 8 * g;
+                }
                 const int64_t k0 = 32 * (int64_t) tile + 8 * g;
                 // (the first of a lane's 8 keys that a row at `pos` sees, and how many from there on)
                 const auto seen = [&](int64_t first_pos, int64_t pos, int & low, int & span) {
@@ -390,6 +433,7 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
                     span = max((int) (min(pos + 1, cap) - k0) - low, 0);
                 };
                 int low, span;
+                if constexpr (!TREE)
 #pragma unroll
                 for (int i = 0; i < RA; i++) {
                     barrier();
@@ -409,7 +453,7 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         const int key = (e & 4) | (e & 1) << 1 | (e >> 1 & 1);
-                        z[e] = (unsigned) (key - low) < (unsigned) span ? z[e] : (_Float16) 0.0f;
+                        z[e] = (TREE ? (any >> key & 1) != 0 : (unsigned) (key - low) < (unsigned) span) ? z[e] : (_Float16) 0.0f;
                     }
                     *vd = z;
                 }
@@ -698,7 +742,8 @@ size_t workspace_of(const Shape & w, int D) {
 template <int D, int RT>
 void launch(const AttnArgs & a, const Shape & w, hipStream_t s) {
     constexpr int ROWS = 16 * RT, NW = waves(D, ROWS);
-    k_paged_attn<D, RT, NW><<<paged_grid(a.items, 64 * NW), 64 * NW, 0, s>>>(a);
+    if (a.tree.mask) k_paged_attn<D, RT, NW, true><<<paged_grid(a.items, 64 * NW), 64 * NW, 0, s>>>(a);
+    else k_paged_attn<D, RT, NW, false><<<paged_grid(a.items, 64 * NW), 64 * NW, 0, s>>>(a);
     check_launch("paged attn");
     if (w.most == 1) return;
     k_paged_merge<D, ROWS><<<paged_grid(a.items, 256), 256, 0, s>>>(a);
@@ -720,9 +765,9 @@ size_t paged_attn_workspace(const Paged & p, int D, int H, int64_t max_rows) {
 }
 
 void launch_paged_attn(const Paged & p, int D, const void * q, int64_t q_r, int64_t q_h, int H, int64_t max_rows, int window,
-                       float scale, float * out, void * ws, hipStream_t s) {
+                       float scale, const PagedTree & tree, float * out, void * ws, hipStream_t s) {
     AttnArgs a{};
-    a.p = p, a.q = (const _Float16 *) q, a.q_r = q_r, a.q_h = q_h, a.H = H, a.G = H / p.Hkv, a.window = window;
+    a.p = p, a.q = (const _Float16 *) q, a.q_r = q_r, a.q_h = q_h, a.H = H, a.G = H / p.Hkv, a.window = window, a.tree = tree;
     a.max_rows = (int) std::min<int64_t>(max_rows, p.n_rows);
     // (from 0 up to 2^-100: scores of 0 either way, but -inf for a hidden key. Down to 2^86: q K is at most 2^40, all exponents
     // stay within f32, and two scores q K that differ, by 2^-48 at the least, are 2^38 powers of two apart already.)

@@ -17,6 +17,7 @@ LIBRARY = _PKG.parent / "lib" / "libgcq.so"
 HEADERS = [_PKG.parents[1] / "include" / h for h in ("gcq.h", "ggml_compiler_rt.h", "ggml.h", "ggml-backend.h",
                                                      "ggml-alloc.h")]
 PAGED_HEADER = _PKG.parents[1] / "include" / "gcq_paged.h"
+DRAFT_HEADER = _PKG.parents[1] / "include" / "gcq_draft.h"
 
 
 class GcqError(RuntimeError):
@@ -117,6 +118,13 @@ SIGNATURES = {
     "gcq_paged_read": ([p, p, i64, p, p, p], i32),
     "gcq_paged_attn_workspace": ([p, p, i64, i32, i64], sz),
     "gcq_paged_attn": ([p, p, i64, p, i64, i64, i32, i64, i32, f32, p, p, sz, p], i32),
+    # gcq_draft.h
+    "gcq_draft_tree": ([p, i64, p, i64, i32, p, p, i64, p], i32),
+    "gcq_paged_append_at": ([p, p, i64, p, p, i64, i64, p, i64, i64, p, i64, i64, i32, p, p, i32, f32, p], i32),
+    "gcq_paged_attn_tree": ([p, p, i64, p, p, i64, p, i64, i64, i32, i64, i32, f32, p, p, sz, p], i32),
+    "gcq_draft_verify_workspace": ([i32, i64, i64, i64], sz),
+    "gcq_draft_verify": ([p, i32, i64, p, p, p, i64, p, i64, i64, p, p, i64, i32, p, p, p, p, sz, p], i32),
+    "gcq_paged_move": ([p, i32, p, p, p, i64, i32, p], i32),
     "gcq_llama_create": ([p, i32], p),
     "gcq_llama_free": ([p], None),
     "gcq_llama_init_random": ([p, u64, f32], i32),

@@ -339,6 +339,16 @@ def _paged_out(out: torch.Tensor | None, shape: tuple, dtype: torch.dtype, name:
     return out
 
 
+def _ints(x: torch.Tensor, name: str, shape: tuple, d: int, dtype: torch.dtype = torch.int32) -> int:
+    """x's address, checked: contiguous, of the shape, on the device."""
+    if x.dtype != dtype or x.shape != shape or not x.is_contiguous() or x.get_device() != d:
+        _cuda(x, dtype, name)
+        if x.shape != shape or not x.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {list(shape)}, got {list(x.shape)}")
+        raise ValueError(f"{name} on {x.device}, the current device is {d}")
+    return x.data_ptr()
+
+
 def _rows_heads(x: torch.Tensor) -> tuple[int, int]:
     return (x.shape[0], x.shape[1]) if x.dim() == 3 else (0, 0)
 
@@ -354,11 +364,12 @@ def rope_freqs(n_dims: int, base: float, freq_scale: float = 1.0, ff: torch.Tens
 
 
 def paged_append(cache: PagedCache, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
-                 freqs: torch.Tensor | None = None, attn_factor: float = 1.0,
-                 q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+                 freqs: torch.Tensor | None = None, attn_factor: float = 1.0, q_out: torch.Tensor | None = None,
+                 positions: torch.Tensor | None = None) -> torch.Tensor | None:
     """Rows k, v f32 [n, Hkv, D] (strided allowed, unit inner stride) into the cache as Q4_0, the keys' NEOX pairs
     (i, i + len(freqs)) turned by position * freqs[i] (freqs None: unrotated). q f32 [n, H, D]: turned alike and
-    returned as f16 [n, H, D], paged_attn's input (q_out: into it; rows of no sequence stay as they are)."""
+    returned as f16 [n, H, D], paged_attn's input (q_out: into it; rows of no sequence stay as they are). positions int32
+    [n]: the positions to turn by where they are not the rows' slots (a DraftTree's)."""
     d, (n, _) = _paged_device(cache, batch), _rows_heads(k)
     kv = (n, cache.Hkv, cache.D)
     ks, vs = _paged_rows(k, torch.float32, "k", kv, d), _paged_rows(v, torch.float32, "v", kv, d)
@@ -375,8 +386,13 @@ def paged_append(cache: PagedCache, batch: PagedBatch, k: torch.Tensor, v: torch
         if freqs.dtype != torch.float32 or freqs.get_device() != d or freqs.dim() != 1 or not freqs.is_contiguous():
             raise ValueError("freqs must be contiguous f32 on the rows' device, one value for each pair")
         f_at, n_dims = freqs.data_ptr(), 2 * freqs.numel()
-    check(load().gcq_paged_append(cache._at, batch._at, n, k.data_ptr(), *ks, v.data_ptr(), *vs, q_at, *qs, H, out_at,
-                                  f_at, n_dims, attn_factor, torch._C._cuda_getCurrentRawStream(d)))
+    rows = (k.data_ptr(), *ks, v.data_ptr(), *vs, q_at, *qs, H, out_at, f_at, n_dims, attn_factor,
+            torch._C._cuda_getCurrentRawStream(d))
+    if positions is None:
+        check(load().gcq_paged_append(cache._at, batch._at, n, *rows))
+    else:
+        _ints(positions, "positions", (n,), d)
+        check(load().gcq_paged_append_at(cache._at, batch._at, n, positions.data_ptr(), *rows))
     return q_out
 
 
@@ -393,11 +409,12 @@ def paged_read(cache: PagedCache, batch: PagedBatch, n: int, k: torch.Tensor | N
 
 
 def paged_attn(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, scale: float, max_rows: int | None = None,
-               window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+               window: int = 0, out: torch.Tensor | None = None, tree: DraftTree | None = None) -> torch.Tensor:
     """Causal attention of the batch's rows over their sequences' cached tokens (their own appended before), the last
     `window` of them if window > 0. q f16 [n, H, D] (strides multiples of 8, unit inner stride) -> f32 [n, H, D] (into
     out if given; rows of no sequence stay as they are; a row that sees no token gives zeros). max_rows: no sequence
-    has more rows than this (default n); 1 for a decode step."""
+    has more rows than this (default n); 1 for a decode step. tree: the rows are draft trees, each sees its sequence's past (of a window
+    the part that its position leaves) and those rows that the tree's mask names."""
     d, (n, H) = _paged_device(cache, batch), _rows_heads(q)
     shape = (n, H, cache.D)
     qs = _paged_rows(q, torch.float16, "q", shape, d)
@@ -410,9 +427,138 @@ def paged_attn(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, scale: flo
     if ws_n == 0:
         raise _lib.error()
     ws = cache.data.new_empty(ws_n)
-    check(lib.gcq_paged_attn(cache._at, batch._at, n, q.data_ptr(), *qs, H, max_rows, window, scale, out.data_ptr(),
-                             ws.data_ptr(), ws_n, torch._C._cuda_getCurrentRawStream(d)))
+    rows = (q.data_ptr(), *qs, H, max_rows, window, scale, out.data_ptr(), ws.data_ptr(), ws_n,
+            torch._C._cuda_getCurrentRawStream(d))
+    if tree is None:
+        check(lib.gcq_paged_attn(cache._at, batch._at, n, *rows))
+    else:
+        if tree._n != n or tree._device != d:
+            raise ValueError(f"a tree of {tree._n} rows on device {tree._device} for {n} rows, the current device is {d}")
+        check(lib.gcq_paged_attn_tree(cache._at, batch._at, n, *tree._c, *rows))
     return out
+
+
+# ------------------------------------------------------------- steps with drafted tokens over the paged cache
+
+
+@dataclass(frozen=True, eq=False)
+class DraftTree:
+    """The trees of a batch's rows (include/gcq_draft.h), int32 on the device: parents [n], the number within its sequence
+    of the earlier row that a row follows, -1 for none; positions [n]; mask [n, words], bit i % 32 of word i // 32: the row
+    sees row i of its sequence. From draft_tree, or of a program's own making. A captured graph follows their contents."""
+
+    parents: torch.Tensor
+    positions: torch.Tensor
+    mask: torch.Tensor
+
+    def __post_init__(self) -> None:
+        n, d = self.parents.numel(), self.parents.get_device()
+        _ints(self.parents, "parents", (n,), d)
+        _ints(self.positions, "positions", (n,), d)
+        words = self.mask.shape[-1]
+        _ints(self.mask, "mask", (n, words), d)
+        if not 1 <= words <= 32:
+            raise ValueError(f"masks of 1 to 32 words, got {words}")
+        for name, value in (("_n", n), ("_device", d), ("_c", (self.positions.data_ptr(), self.mask.data_ptr(), words))):
+            object.__setattr__(self, name, value)
+
+
+def draft_tree(batch: PagedBatch, parents: torch.Tensor, max_rows: int | None = None, window: int = 0,
+               out: DraftTree | None = None) -> DraftTree:
+    """The positions (past + depth) and masks (a row's ancestors and itself, of a window those less than `window` positions
+    back) of the batch's trees, once for all layers. parents int32 [n]. max_rows: no sequence has more rows than this
+    (default n, at most 1024). out: a tree with these parents to write into; rows of no sequence stay as they are."""
+    d, n = torch._C._cuda_getDevice(), parents.numel()
+    if batch._device != d:
+        raise ValueError(f"batch on device {batch._device}, the current device is {d}")
+    max_rows = max(n, 1) if max_rows is None else min(max_rows, max(n, 1))
+    if not 0 <= window < 1 << 31:
+        raise ValueError(f"window {window} is not in 0 .. 2^31 - 1")
+    if out is None:
+        if not 1 <= max_rows <= 1024:
+            raise ValueError(f"max_rows {max_rows} is not in 1 .. 1024")
+        _ints(parents, "parents", (n,), d)
+        out = DraftTree(parents, torch.empty_like(parents), parents.new_empty((n, (max_rows + 31) // 32)))
+    elif out.parents is not parents or out._device != d:
+        raise ValueError("out is a tree of other parents, or not on the current device")
+    positions, mask, words = out._c
+    check(load().gcq_draft_tree(batch._at, n, parents.data_ptr(), max_rows, window, positions, mask, words,
+                                torch._C._cuda_getCurrentRawStream(d)))
+    return out
+
+
+@dataclass(frozen=True, eq=False)
+class DraftPath:
+    """What draft_verify accepts, int32: count [S] rows of each sequence, rows [S, max_path] their numbers within it, tokens
+    [S, max_path] the token that follows each (the last one the next step's first row); -1 from count on."""
+
+    count: torch.Tensor
+    rows: torch.Tensor
+    tokens: torch.Tensor
+
+
+def draft_verify(starts: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, logits: torch.Tensor,
+                 coins: torch.Tensor, draft_logits: torch.Tensor | None = None, temperature: torch.Tensor | None = None,
+                 max_rows: int | None = None, max_path: int | None = None, out: DraftPath | None = None) -> DraftPath:
+    """Which drafts stand against the target, and the token after them (gcq_draft_verify): sequence s owns rows starts[s] ..
+    starts[s + 1] - 1 (int32 [S + 1]), trees by parents (int32 [n]). tokens int32 [n]; logits f32 [n, V], the target's for
+    what follows each row; coins f32 [n], uniform of [0, 1); draft_logits f32 [n, V]: a row's children were drawn from their
+    softmax (None: guesses that were not drawn); temperature f32 [S] (None: 1; 0: the largest logit). Rows of logits may be
+    strided, unit inner stride. max_rows: no sequence has more rows than this (default n, at most 1024); max_path: a
+    path's rows at most (default max_rows). out: into these."""
+    d, n, S = torch._C._cuda_getDevice(), parents.numel(), starts.numel() - 1
+    if S < 1:
+        raise ValueError("starts must hold at least two numbers")
+    shape = (n, logits.shape[-1])
+    at = [_ints(starts, "starts", (S + 1,), d), _ints(parents, "parents", (n,), d), _ints(tokens, "tokens", (n,), d)]
+    lds = [(None, 0), (None, 0)]
+    for i, (x, name) in enumerate(((logits, "logits"), (draft_logits, "draft_logits"))):
+        if x is not None:
+            _cuda(x, torch.float32, name)
+            if x.shape != shape or (shape[1] > 1 and x.stride(1) != 1) or x.get_device() != d:
+                raise ValueError(f"{name} must be {list(shape)} on device {d} with a unit stride along a row, got {list(x.shape)}")
+            lds[i] = (x.data_ptr(), x.stride(0) if n > 1 else shape[1])
+    t_at = None if temperature is None else _ints(temperature, "temperature", (S,), d, torch.float32)
+    c_at = _ints(coins, "coins", (n,), d, torch.float32)
+    max_rows = max(n, 1) if max_rows is None else min(max_rows, max(n, 1))
+    if out is None:
+        max_path = max_rows if max_path is None else max_path
+        if max_path < 1:
+            raise ValueError(f"max_path {max_path} is not positive")
+        out = DraftPath(starts.new_empty(S), starts.new_empty((S, max_path)), starts.new_empty((S, max_path)))
+    else:
+        max_path = out.rows.shape[-1]
+        _ints(out.count, "count", (S,), d), _ints(out.rows, "rows", (S, max_path), d), _ints(out.tokens, "tokens", (S, max_path), d)
+    lib = load()
+    ws_n = lib.gcq_draft_verify_workspace(S, n, shape[1], max_rows)
+    if ws_n == 0:
+        raise _lib.error()
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=starts.device)
+    check(lib.gcq_draft_verify(at[0], S, n, at[1], at[2], *lds[0], *lds[1], shape[1], t_at, c_at, max_rows, max_path,
+                               out.count.data_ptr(), out.rows.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(), ws_n,
+                               torch._C._cuda_getCurrentRawStream(d)))
+    return out
+
+
+def paged_move(caches: PagedCache | list[PagedCache], batch: PagedBatch, count: torch.Tensor, rows: torch.Tensor) -> None:
+    """The accepted rows together: in each cache (all layers', of one shape) slot past[s] + i takes what slot past[s] +
+    rows[s, i] holds, for i < count[s]. count int32 [S], rows int32 [S, m] (strided rows allowed), a DraftPath's. All sources as
+    before the call; an entry below its own number, or one whose slots are not there, moves nothing."""
+    caches = [caches] if isinstance(caches, PagedCache) else caches
+    d, S = torch._C._cuda_getDevice(), batch.past.numel()
+    if not caches:
+        raise ValueError("at least one cache")
+    for c in caches:
+        if c._device != d or batch._device != d:
+            raise ValueError(f"cache on device {c._device}, batch on {batch._device}, the current device is {d}")
+    _ints(count, "count", (S,), d)
+    _cuda(rows, torch.int32, "rows")
+    if rows.dim() != 2 or rows.shape[0] != S or (rows.shape[1] > 1 and rows.stride(1) != 1) or rows.get_device() != d:
+        raise ValueError(f"rows must be [{S}, entries] with contiguous rows on device {d}, got {list(rows.shape)}")
+    n = len(caches)
+    check(load().gcq_paged_move((ctypes.c_void_p * n)(*[c._at for c in caches]), n, batch._at, count.data_ptr(),
+                                rows.data_ptr(), rows.stride(0) if S > 1 else rows.shape[1], rows.shape[1],
+                                torch._C._cuda_getCurrentRawStream(d)))
 
 
 # ------------------------------------------------------------------------ norms and glue
