@@ -1,7 +1,6 @@
 // draft.hip - steps with drafted tokens: the trees' masks and positions, the drafts' verification, and moving the accepted rows
 // together in the caches (include/gcq_draft.h; append and attention of such rows are paged.hip's and paged_attn.hip's).
 #include <algorithm>
-#include <cmath>
 
 #include "paged.h"
 
@@ -97,37 +96,39 @@ __global__ __launch_bounds__(256) void k_draft_tree(const TreeArgs a) {
 
 // ------------------------------------------------------------------------------- verification
 //
-// Three launches. k_verify_begin puts the rows in order, the sequences' first rows first, then their second ones, .. k_verify_rows
-// takes each row's logits in parts, a workgroup to a part: the largest and the sum of exponentials, of the target's and, where a
-// row has children, the drafter's. Whichever of a row's workgroups ends last has the row's softmax and decides which child stands,
-// which depends on nothing but the row. Rows that an earlier decision has cut off from the path are passed over if it is
-// known by then: in this order, where rows are many, it mostly is (nobody waits for it, and no result depends on it).
-// k_verify_walk, some workgroups to a sequence, follows the decisions from the root on and draws the last row's token.
-//
-// r after k fallen drafts is w_k / c_k, w_k = max(p - C_k q, 0), c_k its sum, C_0 = 0 and C_k+1 = C_k + c_k, since
-// max(max(a, 0) - b, 0) = max(a - b, 0) for b >= 0: one sum over the vocabulary for each that falls, which the walk makes
-// for the rows on the path alone.
+// k_verify_begin puts the rows in order, the sequences' first rows first, then their second ones, .. k_verify_rows takes each row's logits
+// in parts, a workgroup to a part: the largest and the sum of exponentials, of the target's and, where a row has children, the
+// drafter's. Whichever of a row's workgroups ends last has the row's softmax and decides which child stands, which depends on
+// nothing but the row. Rows that an earlier decision has cut off from the path are passed over if it is known by then: in this
+// order, where rows are many, it mostly is (nobody waits for it, and no result depends on it). k_verify_walk follows the
+// decisions from the root on and draws the last row's token. Where a drawn child fell it is drawn from what is left:
+//   r after k fallen drafts is w_k / c_k, w_k = max(p - C_k q, 0), c_k its sum, C_0 = 0 and C_k+1 = C_k + c_k, since
+//   max(max(a, 0) - b, 0) = max(a - b, 0) for b >= 0: one sum over the vocabulary for each that falls, made for the rows on the
+//   path alone.
 //
 // In 64 bits: a token's border in the cumulative sum would be off by 2^-25 or so in 32, and 10^5 borders then put a drawn token wrong
 // once in some hundred draws.
 
-constexpr int kT = 256;
-constexpr int kDraw = 16;  // values of a thread in the walk
+typedef int i4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kT = 256, kStep = 4 * kT;  // threads, logits of a workgroup at a time
+constexpr int kSteps = 8;                // .. of a part at most
+constexpr int kRowGroups = 1024;         // workgroups at a time in k_verify_rows
+constexpr float kHuge = 3.402823466e38f;
 
 // What became of a row: the child that stands (>= 0), or
-enum : int { kNone = -1, kOpen = -2, kCut = -3, kFell = -16 };  // kFell - j: child j fell, others are left, r's sum is not known
+enum : int { kNone = -1, kOpen = -2, kFell = -16 };  // not known yet; kFell - j: child j fell, others are left, r's sum is not known
 
-struct __align__(64) RowState {
+struct __align__(16) RowState {
     double sum_p, sum_q, C;  // sums of exp((l - m) / t)
     float m_p, m_q;
-    int top, next, arrived;
+    int top, pad;
 };
 struct __align__(16) PartSums {
     double p, q;
     float m_p, m_q;
     int top, pad;
 };
-constexpr int kPartWords = sizeof(PartSums) / 8;
 struct SeqState {
     int arrived, done;
 };
@@ -137,70 +138,150 @@ struct __align__(16) Item {  // a row in its order
     float t;              // temperature
     int child;            // the first; n: none
 };
-struct __align__(16) Drawn {
-    double w, p;
-};
-constexpr int kDrawnWords = sizeof(Drawn) / 8;
 
 struct VerifyArgs {
     const int32_t * starts, * parents, * tokens;
     const float * logits, * draft, * temperature, * coins;
     int64_t ld, draft_ld;
-    int n_seq, n_rows, V, max_rows, max_path, parts, draws;
-    bool vec, last;  // rows of whole 16-byte pieces; the last walk
+    int n_seq, n_rows, V, max_rows, max_path;
+    int parts, steps, abreast, each;  // parts of a row and a part's steps; rows abreast in k_verify_rows; workgroups to a sequence in k_verify_walk
+    bool vec, last;             // rows of whole 16-byte pieces; the last walk
     int32_t * count, * rows, * out;
     int * n_items;
     Item * items;
     RowState * state;
+    int * next, * arrived;  // of the rows
     PartSums * sums;
     SeqState * seq;
-    Drawn * drawn;
-    double roots[16];  // 2^(i / 16)
+    double * drawn;
 };
 
+// 2^(i / 16)
+__constant__ double kRoots[16] = {
+    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.189207115002721, 1.241857812073484,
+    1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+    1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+
 // exp by a sixteenth of a power of two from LDS (a bank of its own each) and five terms of exp's series on what is left: |z| <= ln 2 / 32, the
-// sixth is 2^-43. 12 operations of 64 bits; the library's takes about twice as many.
+// sixth is 2^-43. 12 operations of 64 bits and 5 others in `weigh4`, where the kernels spend their arithmetic; the library's takes
+// some 30. (Loops are left as loops here, and code is written once: most of it runs once in a workgroup, and fetching 40 KB of it took
+// longer than what it did.)
+__device__ __forceinline__ double power(double r) {  // 2^(r / 16), |r| <= 1 / 2
+    constexpr double k = 0.043321698784996581;           // ln 2 / 16
+    double y = fma(r, k * k * k * k * k / 120, k * k * k * k / 24);
+    y = fma(r, y, k * k * k / 6);
+    y = fma(r, y, k * k / 2);
+    y = fma(r, y, k);
+    return fma(r, y, 1.0);
+}
+// 2^(n / 16)
+__device__ __forceinline__ double root(const double * roots, int n) {
+    const double y = roots[n & 15];
+    return __hiloint2double(__double2hiint(y) + ((n & ~15) << 16), __double2loint(y));
+}
 struct Soft {
     const double * roots;  // LDS
-    double scale, m, inv;  // 16 / (t ln 2), the row's largest logit, 1 / its sum
-    bool huge;             // some logit is infinite
+    double scale, m, inv;  // 16 / (t ln 2); a logit that weighs 1, the row's weights are below 2^512; 1 / their sum
+    // exp((l - m) / t), 0 from 2^-1000 on
     __device__ __forceinline__ double weight(float l) const {
-        if (huge) l = fminf(l, 3.402823466e38f);
-        const double x = ((double) l - m) * scale, t = x + 0x1.8p52, r = x - (t - 0x1.8p52);
-        const int n = (int) (uint32_t) __double_as_longlong(t);
-        constexpr double k = 0.043321698784996581;  // ln 2 / 16
-        double y = fma(r, k * k * k * k * k / 120, k * k * k * k / 24);
-        y = fma(r, y, k * k * k / 6);
-        y = fma(r, y, k * k / 2);
-        y = fma(r, y, k);
-        y = fma(r, y, 1.0) * roots[n & 15];
-        y = __hiloint2double(__double2hiint(y) + ((n >> 4) << 20), __double2loint(y));
+        if (l > kHuge) l = kHuge;
+        const double x = ((double) l - m) * scale, t = x + 0x1.8p52, y = power(x - (t - 0x1.8p52)) * root(roots, (int) (uint32_t) __double_as_longlong(t));
         return x > -16000.0 ? y : 0.0;  // (nor for -inf and NaN)
     }
     __device__ __forceinline__ double p(float l) const { return weight(l) * inv; }
 };
-__device__ __forceinline__ Soft soft(const double * roots, double inv_t, float m, double sum) {
-    return {roots, inv_t * 23.083120654223414, (double) m, sum > 0.0 ? 1.0 / sum : 0.0, m >= 3.402823466e38f};
+__device__ __forceinline__ double scale_of(float t) { return 23.083120654223414 / (double) t; }
+__device__ __forceinline__ Soft soft(const double * roots, double scale, float m, double sum) { return {roots, scale, (double) m, sum > 0.0 ? 1.0 / sum : 0.0}; }
+
+// Logits around m where the short form serves: those above `low` (2^-1000; what is below counts as that, no more than 2^-1000 each, NaN too),
+// and not above `high`, 2^500. odd: there is no such range in f32, or no such m.
+struct Range {
+    float low, high;
+    int odd;
+};
+__device__ __forceinline__ Range range_of(float m, double scale) {
+    const double d = 16000.0 / scale;
+    Range z{(float) ((double) m - d), (float) ((double) m + 0.5 * d), 0};
+    const double x = ((double) z.low - (double) m) * scale;
+    z.odd = !(fabsf(m) < 1e38f) || !(x > -16300.0 && x < -15700.0);  // (root's powers end at 2^-1022)
+    return z;
+}
+// The weights of four logits in that range (two, then two: more at a time than the registers hold).
+__device__ __forceinline__ void weigh4(const double * roots, double scale, double m, float low, const float (&l)[4], double (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+#pragma unroll
+        for (int i = e; i < e + 2; i++) {
+            const double d = (double) __builtin_amdgcn_fmed3f(l[i], low, kHuge) - m, t = fma(d, scale, 0x1.8p52), r = fma(d, scale, 0x1.8p52 - t);
+            v[i] = power(r) * root(roots, (int) (uint32_t) __double_as_longlong(t));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
-// N values x[i ..), those at V and beyond -inf.
-template <int N>
-__device__ __forceinline__ void values(const float * x, int i, int V, bool vec, float (&v)[N]) {
-#pragma unroll
-    for (int e = 0; e < N; e += 4) {
-        if (vec && i + e + 3 < V) *reinterpret_cast<float4 *>(v + e) = *reinterpret_cast<const float4 *>(x + i + e);
-        else
-#pragma unroll
-            for (int c = 0; c < 4; c++) v[e + c] = i + e + c < V ? x[i + e + c] : -INFINITY;
+// A sum of weights; m: the logit that weighs 1, -inf while there is none.
+struct Running {
+    float m;
+    double s;
+    // s2 times exp(m2 / t) more
+    __device__ __forceinline__ void take(const double * roots, double scale, float m2, double s2) {
+        const Soft z{roots, scale, (double) fmaxf(m, m2), 0.0};
+        s = s * z.weight(m) + s2 * z.weight(m2);
+        m = fmaxf(m, m2);
     }
+    __device__ __forceinline__ void take4(const double * roots, double scale, Range & in, const float (&l)[4]) {
+        const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+        if (__any(m == -INFINITY && top > -INFINITY))
+            if (m == -INFINITY && top > -INFINITY) {
+                m = fminf(top, kHuge), s = 0.0;
+                const Range z = range_of(m, scale);
+                in.low = z.low, in.high = z.high, in.odd = z.odd;
+            }
+        if (__any(top > in.high || in.odd)) {
+            const float to = fminf(fmaxf(m, top), kHuge);
+            if (to > -INFINITY) {
+                const Soft z{roots, scale, (double) to, 0.0};
+                s *= z.weight(m);
+                m = to;
+                const Range w = range_of(m, scale);
+                in.low = w.low, in.high = w.high, in.odd = w.odd;
+                float x = l[0], y = l[1], u = l[2], v = l[3];
+#pragma unroll 1
+                for (int e = 0; e < 4; e++) {
+                    s += z.weight(x);
+                    x = y, y = u, u = v;
+                }
+            }
+            return;
+        }
+        double v[4];
+        weigh4(roots, scale, m > -INFINITY ? (double) m : 0.0, in.low, l, v);
+        s += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    __device__ __forceinline__ void wave(const double * roots, double scale) {
+        const float top = wave_max(m);
+        s = wave_sum_d(m > -INFINITY ? s * Soft{roots, scale, (double) top, 0.0}.weight(m) : 0.0);
+        m = top;
+    }
+};
+
+// Four values x[i ..), those at V and beyond -inf; whole: there are none of those, and 16-byte pieces.
+__device__ __forceinline__ void values4(const float * x, int i, int V, bool whole, float (&v)[4]) {
+    if (whole) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(x + i);
+    else
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            v[c] = -INFINITY;
+            if (i + c < V) v[c] = x[i + c];
+        }
 }
 
 template <class T>
 __device__ __forceinline__ T agent_load(const T * p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <class T>
 __device__ __forceinline__ void agent_store(T * p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-// What workgroups tell each other within a launch goes past the XCDs' L2s, word by word: a fence would write back and drop a whole L2, some
-// 40 ns each and one after the other (5120 workgroups 220 us; so 60).
+// What workgroups tell each other within a launch goes past the XCDs' L2s, word by word, and a store that others go by follows once what came
+// before has reached memory: a fence would write back and drop a whole L2, some 40 ns each and one after the other.
 template <class T>
 __device__ __forceinline__ void share(T * to, const T & v) {
     static_assert(sizeof(T) % 8 == 0, "words of 8 bytes");
@@ -218,11 +299,11 @@ __device__ __forceinline__ T shared(const T * from) {
     __builtin_memcpy(&v, w, sizeof(T));
     return v;
 }
-// Whether this workgroup is the last of n to arrive, after thread 0 has shared what it has (all threads together). The stores have reached
-// memory before the count is raised; who reads the last count reads them there.
+__device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Whether this workgroup is the last of n to arrive, after thread 0 has shared what it has (all threads together).
 __device__ __forceinline__ bool last_of(int * arrived, int n, int * flag) {
     if (threadIdx.x == 0) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        stores_done();
         *flag = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
     }
     __syncthreads();
@@ -242,9 +323,15 @@ __device__ __forceinline__ int child_after(const int32_t * parents, const Rows &
 // A wavefront to a row: its place in the order, and its state.
 __global__ __launch_bounds__(kT) void k_verify_begin(const VerifyArgs a) {
     const int lane = threadIdx.x & 63, r = blockIdx.x * (kT / 64) + (threadIdx.x >> 6);
-    for (int s = blockIdx.x * kT + threadIdx.x; s < a.n_seq; s += gridDim.x * kT) a.seq[s] = SeqState{};
+    for (int s = blockIdx.x * kT + threadIdx.x; s < a.n_seq; s += gridDim.x * kT) {
+        a.seq[s] = SeqState{};
+        const Rows w = rows_of(a.starts, s, a.n_rows, a.max_rows);
+        if (w.n) continue;
+        a.count[s] = 0, a.seq[s].done = 1;
+        for (int i = 0; i < a.max_path; i++) a.rows[(int64_t) s * a.max_path + i] = a.out[(int64_t) s * a.max_path + i] = -1;
+    }
     if (r >= a.n_rows) return;
-    if (lane == 0) a.state[r] = {0.0, 0.0, 0.0, -INFINITY, -INFINITY, 0x7fffffff, kOpen, 0};
+    if (lane == 0) a.next[r] = kOpen, a.arrived[r] = 0;
     const auto load = [&](int s0) { return s0 + lane < a.n_seq ? rows_of(a.starts, s0 + lane, a.n_rows, a.max_rows) : Rows{}; };
     const Rows first = load(0);
     Rows w{}, x = first;
@@ -267,7 +354,7 @@ __global__ __launch_bounds__(kT) void k_verify_begin(const VerifyArgs a) {
     before = wave_isum(before);
     if (r == 0) {
         all = wave_isum(all);
-        if (lane == 0) *a.n_items = all;
+        if (lane == 0) *a.n_items = min(all, a.n_rows);
     }
     if (s < 0 || before >= a.n_rows) return;
     const int parent = a.parents[r], child = child_after(a.parents, w, j, j);
@@ -296,373 +383,452 @@ __device__ __forceinline__ Children children(const VerifyArgs & a, const Rows & 
     }
     return c;
 }
-// The next child of a drawn row, row `from` having fallen last and r's sum c being known; k: the children from row j0 on.
-__device__ __forceinline__ void decide_drawn(const VerifyArgs & a, const Rows & w, int u, int from, double c, const Soft & p, const Soft & q,
-                                             Children k, int j0, RowState & z) {
-    z.next = kNone;
-    for (; j0 < w.n; k = children(a, w, u, j0 += 64)) {
-        const uint64_t left = from < j0 ? k.at : from - j0 >= 63 ? 0 : k.at >> (from - j0 + 1) << (from - j0 + 1);
-        if (!left) {
-            if (j0 + 64 >= w.n) return;
-            continue;
-        }
-        const int l = __builtin_ctzll(left), token = __builtin_amdgcn_readlane(k.token, l);
-        const double pt = p.p(readlane_f(k.x, l)), qt = q.p(readlane_f(k.y, l));
-        if (token >= 0 && token < a.V && (double) readlane_f(k.coin, l) * c * qt < fmax(pt - z.C * qt, 0.0)) {
-            z.next = j0 + l;
-            return;
-        }
-        z.C += c;
-        if (left & (left - 1) || child_after(a.parents, w, u, j0 + 63) < w.n) z.next = kFell - (j0 + l);
-        return;
-    }
-}
-// All children of a row whose drafts were not drawn.
-__device__ __forceinline__ int decide_guessed(const VerifyArgs & a, const Rows & w, int u, const Soft & p, Children k) {
+// Whether the child at bit l of k, the children from row j0 on, has the token of an earlier one.
+__device__ __forceinline__ bool again(const VerifyArgs & a, const Rows & w, int u, const Children & k, int j0, int l, int token) {
     const int lane = threadIdx.x & 63;
-    double left = 1.0;  // what the fallen leave
-    for (int j0 = u + 1; j0 < w.n;) {
-        const double pt = p.p(k.x);
-        for (uint64_t at = k.at; at; at &= at - 1) {
-            const int l = __builtin_ctzll(at), t = __builtin_amdgcn_readlane(k.token, l);
+    bool before = (k.at >> lane & 1) && lane < l && k.token == token;
+    for (int i = u + 1 + lane; i < j0; i += 64) before = before || (a.parents[w.r0 + i] == u && a.tokens[w.r0 + i] == token);
+    return __any(before);
+}
+// Which of row u's children after row `from` stands (a wavefront; k: its children from row j0 on): the first with the largest logit's token
+// (top >= 0); of drawn ones the next, c being r's sum; of guesses the first that stands, c what is left of p.
+__device__ __forceinline__ int decide(const VerifyArgs & a, const Rows & w, int u, int from, int top, double c, const Soft & p, const Soft & q,
+                                      Children k, int j0, double & C) {
+    for (;;) {
+        const int lane = threadIdx.x & 63;
+        uint64_t at = __ballot((k.at >> lane & 1) && j0 + lane > from && (top < 0 || k.token == top));
+        if (top >= 0 && at) return j0 + __builtin_ctzll(at);
+        const double pt = p.p(k.x), qt = a.draft ? q.p(k.y) : 1.0;  // (0 of a token that there is not)
+        for (; at; at &= at - 1) {
+            const int l = __builtin_ctzll(at);
+            const double ql = readlane_d(qt, l);
             double v = readlane_d(pt, l);
-            bool before = (k.at >> lane & 1) && lane < l && k.token == t;  // (fell already)
-            for (int i = u + 1 + lane; i < j0; i += 64) before = before || (a.parents[w.r0 + i] == u && a.tokens[w.r0 + i] == t);
-            if (__any(before)) v = 0.0;
-            if ((double) readlane_f(k.coin, l) * left < v) return j0 + l;
-            left -= v;
-        }
-        if ((j0 += 64) < w.n) k = children(a, w, u, j0);
-    }
-    return kNone;
-}
-
-template <int NV>
-__global__ __launch_bounds__(kT) void k_verify_rows(const VerifyArgs a) {
-    __shared__ double roots[16], red[2][kT / 64];
-    __shared__ float redm[2][kT / 64];
-    __shared__ int redt[kT / 64], flag;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x % a.parts, at = blockIdx.x / a.parts;
-    const Item it = a.items[at];  // (of n_rows there may be)
-    if (at >= *a.n_items) return;
-    if ((unsigned) it.r >= (unsigned) a.n_rows || it.r0 < 0 || it.j < 0 || it.r0 + it.j != it.r || it.j >= it.n || it.r0 > a.n_rows - it.n || it.n > kMaxRows) return;
-    RowState * const state = a.state + it.r;
-    if (it.j > 0) {
-        bool cut = it.parent < 0 || it.parent >= it.j;
-        if (!cut) {
-            const int next = agent_load(&a.state[it.r0 + it.parent].next);
-            cut = next == kNone || next == kCut || (next >= 0 && next != it.j) || (next <= kFell && it.j <= kFell - next);
-        }
-        if (cut) {
-            if (tid == 0) agent_store(&state->next, (int) kCut);
-            return;
-        }
-    }
-    const Rows w{it.r0, it.n};
-    const bool greedy = !(it.t > 0.0f);
-    const double inv_t = greedy ? 1.0 : 1.0 / (double) it.t;
-    constexpr int E = NV * 4 * kT;
-    const int i0 = part * E + 4 * tid;
-    float x[NV][4], y[NV][4];
-#pragma unroll
-    for (int k = 0; k < NV; k++) values<4>(a.logits + it.r * a.ld, i0 + 4 * kT * k, a.V, a.vec, x[k]);
-    const bool drawn = a.draft && !greedy && it.child < w.n;
-    if (drawn)
-#pragma unroll
-        for (int k = 0; k < NV; k++) values<4>(a.draft + it.r * a.draft_ld, i0 + 4 * kT * k, a.V, a.vec, y[k]);
-    Children kids{};
-    if (wave == 0 && it.child < w.n) kids = children(a, w, it.j, it.j + 1);
-    if (tid < 16) roots[tid] = a.roots[tid];
-    float mp = -INFINITY, mq = -INFINITY;
-    int top = 0x7fffffff;
-    if (greedy) {
-#pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) argmax_take(mp, top, x[k][e] > 3.402823466e38f ? 3.402823466e38f : x[k][e], i0 + 4 * kT * k + e);
-        for (int o = 32; o > 0; o >>= 1) argmax_take(mp, top, __shfl_xor(mp, o, 64), __shfl_xor(top, o, 64));
-    } else {
-#pragma unroll
-        for (int k = 0; k < NV; k++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) mp = fmaxf(mp, x[k][e]);
-        mp = wave_max(mp);
-        if (drawn) {
-#pragma unroll
-            for (int k = 0; k < NV; k++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) mq = fmaxf(mq, y[k][e]);
-            mq = wave_max(mq);
-        }
-    }
-    if (lane == 0) redm[0][wave] = mp, redm[1][wave] = mq, redt[wave] = top;
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < kT / 64; v++) {
-        if (greedy) argmax_take(mp, top, redm[0][v], redt[v]);
-        else mp = fmaxf(mp, redm[0][v]), mq = fmaxf(mq, redm[1][v]);
-    }
-    mp = fminf(mp, 3.402823466e38f);
-    mq = fminf(mq, 3.402823466e38f);
-    double sp = 0.0, sq = 0.0;
-    if (!greedy) {
-        const Soft p = soft(roots, inv_t, mp, 0.0), q = soft(roots, inv_t, mq, 0.0);
-        if (mp > -INFINITY)
-#pragma unroll
-            for (int k = 0; k < NV; k++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) sp += p.weight(x[k][e]);
-        if (drawn && mq > -INFINITY)
-#pragma unroll
-            for (int k = 0; k < NV; k++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) sq += q.weight(y[k][e]);
-        sp = wave_sum_d(sp);
-        sq = wave_sum_d(sq);
-        if (lane == 0) red[0][wave] = sp, red[1][wave] = sq;
-        __syncthreads();
-        sp = sq = 0.0;
-#pragma unroll
-        for (int v = 0; v < kT / 64; v++) sp += red[0][v], sq += red[1][v];
-    }
-    PartSums * const sums = a.sums + (int64_t) it.r * a.parts;
-    if (tid == 0) share(sums + part, PartSums{sp, sq, mp, mq, top, 0});
-    if (!last_of(&state->arrived, a.parts, &flag) || wave) return;
-
-    RowState z{0.0, 0.0, 0.0, -INFINITY, -INFINITY, 0x7fffffff, kNone, 0};
-    const PartSums mine = lane < a.parts ? shared(sums + lane) : PartSums{0.0, 0.0, -INFINITY, -INFINITY, 0x7fffffff, 0};
-    const auto each = [&](auto && f) {
-        f(mine);
-        for (int i = lane + 64; i < a.parts; i += 64) f(shared(sums + i));
-    };
-    each([&](const PartSums & x) {
-        argmax_take(z.m_p, z.top, x.m_p, x.top);
-        z.m_q = fmaxf(z.m_q, x.m_q);
-    });
-    for (int o = 32; o > 0; o >>= 1) argmax_take(z.m_p, z.top, __shfl_xor(z.m_p, o, 64), __shfl_xor(z.top, o, 64));
-    z.m_q = wave_max(z.m_q);
-    Soft p = soft(roots, inv_t, z.m_p, 0.0), q = soft(roots, inv_t, z.m_q, 0.0);
-    if (!greedy) {
-        each([&](const PartSums & x) {
-            if (x.p > 0.0) z.sum_p += x.p * p.weight(x.m_p);
-            if (x.q > 0.0) z.sum_q += x.q * q.weight(x.m_q);
-        });
-        z.sum_p = wave_sum_d(z.sum_p);
-        z.sum_q = wave_sum_d(z.sum_q);
-        p = soft(roots, inv_t, z.m_p, z.sum_p);
-        q = soft(roots, inv_t, z.m_q, z.sum_q);
-    }
-    if (z.m_p > -INFINITY && it.child < w.n) {
-        if (greedy) {
-            for (int j0 = it.j + 1; j0 < w.n; kids = children(a, w, it.j, j0)) {
-                const uint64_t hit = __ballot((kids.at >> lane & 1) && kids.token == z.top);
-                if (hit) z.next = j0 + __builtin_ctzll(hit);
-                if (hit || (j0 += 64) >= w.n) break;
+            if (a.draft) v = fmax(v - C * ql, 0.0);
+            else if (again(a, w, u, k, j0, l, __builtin_amdgcn_readlane(k.token, l))) v = 0.0;
+            if ((double) readlane_f(k.coin, l) * c * ql < v) return j0 + l;
+            if (a.draft) {
+                C += c;
+                return at & (at - 1) || child_after(a.parents, w, u, j0 + 63) < w.n ? kFell - (j0 + l) : (int) kNone;
             }
-        } else if (drawn) decide_drawn(a, w, it.j, it.j, 1.0, p, q, kids, it.j + 1, z);
-        else z.next = decide_guessed(a, w, it.j, p, kids);
-    }
-    if (lane == 0) {
-        state->sum_p = z.sum_p, state->sum_q = z.sum_q, state->C = z.C, state->m_p = z.m_p, state->m_q = z.m_q, state->top = z.top;
-        agent_store(&state->next, z.next);
+            c -= v;
+        }
+        if ((j0 += 64) >= w.n) return kNone;
+        k = children(a, w, u, j0);
     }
 }
 
-// The walk of one sequence. A part of the last row's weights w_k is a workgroup's, their sum for the draw or for the next child; the last
-// workgroup to end goes on, in the last launch alone to the end.
+// What a workgroup keeps in LDS of the path and of a draw.
+struct PathLds {
+    double roots[16], seg[4 * kSteps];  // sums of a part's runs of 256 tokens
+    int next[kMaxRows], path[kMaxRows];
+    uint32_t gone[kSteps * kStep / 32];
+    int flag, said;
+};
+
+// The path from the root as far as it is known: the number of its rows and the last one.
+__device__ __forceinline__ int find_path(const VerifyArgs & a, const Rows & w, PathLds & m, int & last) {
+    for (int j = threadIdx.x; j < w.n; j += kT) m.next[j] = agent_load(&a.next[w.r0 + j]);
+    __syncthreads();
+    int n = 0;
+    last = 0;
+    for (int u = 0; w.n > 0 && n < a.max_path;) {
+        if (threadIdx.x == 0) m.path[n] = u;
+        n++;
+        last = u;
+        const int v = __builtin_amdgcn_readfirstlane(m.next[u]);
+        if (v <= u || v >= w.n) break;
+        u = v;
+    }
+    return n;
+}
+
+// A lane's value and those of the lanes before.
+__device__ __forceinline__ double upto(double v) {
+#pragma unroll 1
+    for (int o = 1; o < 64; o <<= 1) {
+        const double b = __shfl_up(v, o, 64);
+        if ((threadIdx.x & 63) >= (unsigned) o) v += b;
+    }
+    return v;
+}
+
+// A row that a token is drawn from: its r, max(p - C q, 0) if C > 0, else p without the guesses that fell.
+struct Source {
+    Rows w;
+    int s, u;
+    double C;
+    Soft p, q;
+    float p_low, q_low;  // Range's
+    bool odd;
+};
+__device__ __forceinline__ Source source(const Rows & w, int s, int u, const RowState & st, const double * roots, double scale) {
+    const Range p = range_of(st.m_p, scale), q = st.C > 0.0 ? range_of(st.m_q, scale) : p;
+    return {w, s, u, st.C, soft(roots, scale, st.m_p, st.sum_p), soft(roots, scale, st.m_q, st.sum_q), p.low, q.low, p.odd || q.odd};
+}
+// The weights of the tokens whose logits are l (the drafter's d), from token i of a part on, of r or (all) of p.
+__device__ __forceinline__ void weights4(const VerifyArgs & a, const Source & z, const PathLds & m, int i, bool all, const float (&l)[4], const float (&d)[4], double (&v)[4]) {
+    const bool fell = z.C > 0.0 && !all;
+    double q[4];
+    if (z.odd) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[e] = z.p.weight(l[e]);
+            if (fell) q[e] = z.q.weight(d[e]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+        weigh4(z.p.roots, z.p.scale, z.p.m, z.p_low, l, v);
+        if (fell) weigh4(z.q.roots, z.q.scale, z.q.m, z.q_low, d, q);
+    }
+    const uint32_t out = a.draft || all ? 0 : m.gone[i / 32] >> (i % 32);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        v[e] = out >> e & 1 ? 0.0 : v[e] * z.p.inv;
+        if (fell) v[e] = fmax(v[e] - z.C * (q[e] * z.q.inv), 0.0);
+    }
+}
+__device__ __forceinline__ void logits4(const VerifyArgs & a, const Source & z, int part, int i, bool all, float (&l)[4], float (&d)[4]) {
+    const int at = part * a.steps * kStep + i;
+    const bool whole = a.vec && at + 3 < a.V;
+    values4(a.logits + (z.w.r0 + z.u) * a.ld, at, a.V, whole, l);
+    if (z.C > 0.0 && !all) values4(a.draft + (z.w.r0 + z.u) * a.draft_ld, at, a.V, whole, d);
+}
+// The sums of a part's runs of 256 tokens, and of the part (all threads).
+__device__ __forceinline__ double runs(const VerifyArgs & a, const Source & z, PathLds & m, int part, bool all) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (!a.draft && !all) {
+        m.gone[tid] = 0;
+        __syncthreads();
+        for (int j = z.u + 1 + tid; j < z.w.n; j += kT)
+            if (a.parents[z.w.r0 + j] == z.u) {
+                const unsigned e = (unsigned) a.tokens[z.w.r0 + j] - (unsigned) (part * a.steps * kStep);
+                if (e < (unsigned) (a.steps * kStep)) atomicOr(&m.gone[e / 32], 1u << (e % 32));
+            }
+        __syncthreads();
+    }
+    float l[4], d[4], l1[4], d1[4];
+    logits4(a, z, part, 4 * tid, all, l, d);
+#pragma unroll 1
+    for (int k = 0; k < a.steps; k++) {
+        if (k + 1 < a.steps) logits4(a, z, part, (k + 1) * kStep + 4 * tid, all, l1, d1);
+        double v[4];
+        weights4(a, z, m, k * kStep + 4 * tid, all, l, d, v);
+#pragma unroll
+        for (int e = 0; e < 4; e++) l[e] = l1[e], d[e] = d1[e];
+        const double sum = wave_sum_d((v[0] + v[1]) + (v[2] + v[3]));
+        if ((tid & 63) == 0) m.seg[4 * k + (tid >> 6)] = sum;
+    }
+    __syncthreads();
+    return wave_sum_d((tid & 63) < 4 * a.steps ? m.seg[tid & 63] : 0.0);
+}
+static_assert(kSteps * kStep / 32 == kT && 4 * kSteps <= 64, "a word of gone to a thread, a run to a lane");
+
+// The sum of a lane's part, of those from i0 on: what fell of drawn ones was summed for this draw, others are k_verify_rows's, less what fell.
+__device__ __forceinline__ double part_sum(const VerifyArgs & a, const Source & z, int i0, bool all) {
+    const int lane = threadIdx.x & 63, part = i0 + lane;
+    if (z.C > 0.0 && !all) return part < a.parts ? shared(a.drawn + (int64_t) z.s * a.parts + part) : 0.0;
+    double v = 0.0;
+    if (part < a.parts) {
+        const PartSums x = shared(a.sums + (int64_t) (z.w.r0 + z.u) * a.parts + part);
+        v = x.p * z.p.p(x.m_p);
+    }
+    if (all || a.draft) return v;
+    for (int j0 = z.u + 1; j0 < z.w.n; j0 += 64) {
+        const Children k = children(a, z.w, z.u, j0);
+        const double pt = z.p.p(k.x);
+        for (uint64_t at = k.at; at; at &= at - 1) {
+            const int l = __builtin_ctzll(at), token = __builtin_amdgcn_readlane(k.token, l);
+            if (token >= 0 && token / (a.steps * kStep) == part && !again(a, z.w, z.u, k, j0, l, token)) v -= readlane_d(pt, l);
+        }
+    }
+    return fmax(v, 0.0);
+}
+constexpr double kNothing = 0x1p-900;  // no token's weight
+// Of 64 lanes' values, the one where the sum passes `want`, the last above nothing if rounding leaves none, -1 if all are 0; below grows by those before
+// it, or by all.
+__device__ __forceinline__ int pass(double d, double want, double & below, bool & hit) {
+    const double sum = upto(d);
+    const uint64_t some = __ballot(d > kNothing), at = __ballot(d > kNothing && below + sum > want);
+    hit = at != 0;
+    const int l = hit ? __builtin_ctzll(at) : some ? 63 - __builtin_clzll(some) : -1;
+    below += hit ? (l ? readlane_d(sum, l - 1) : 0.0) : readlane_d(sum, 63);
+    return l;
+}
+// The token where the cumulative sum passes the coin's share of it: the part, the run, the lane, the token. From p if r has nothing.
+__device__ __forceinline__ int draw(const VerifyArgs & a, const Source & z, PathLds & m) {
+    const int lane = threadIdx.x & 63;
+    const float coin = a.coins[z.w.r0];
+    const double portion = coin > 0.0f ? fmin((double) coin, 1.0 - 0x1p-24) : 0.0;
+#pragma unroll 1
+    for (int all = 0; all < 2; all++) {
+        double first = 0.0, want = INFINITY, base = 0.0, rest = 0.0;
+        int part = -1;
+        bool hit = false;
+#pragma unroll 1
+        for (int find = 0; find < 2; find++) {  // the total, then the part
+            double below = 0.0;
+            for (int i0 = 0; i0 < a.parts && !hit; i0 += 64) {
+                const double d = find && i0 == 0 ? first : part_sum(a, z, i0, all), before = below;
+                if (i0 == 0) first = d;
+                const int l = pass(d, want, below, hit);
+                if (find && l >= 0) part = i0 + l, base = hit ? below : before, rest = hit ? want : INFINITY;
+            }
+            want = portion * below;
+        }
+        if (part < 0) continue;
+        want = rest;  // (no part passes it, by rounding: the last token of the last)
+        runs(a, z, m, part, all);
+        if (threadIdx.x < 64) {
+            const int run = pass(lane < 4 * a.steps ? m.seg[lane] : 0.0, want, base, hit);
+            int token = -1;
+            if (run >= 0) {
+                if (!hit) want = INFINITY;
+                float l[4], d[4];
+                double v[4];
+                logits4(a, z, part, run * 256 + 4 * lane, all, l, d);
+                weights4(a, z, m, run * 256 + 4 * lane, all, l, d, v);
+                const int who = pass((v[0] + v[1]) + (v[2] + v[3]), want, base, hit);
+                if (who >= 0) {
+                    if (!hit) want = INFINITY;
+                    int e = -1;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const double x = readlane_d(v[i], who);
+                        if (x > kNothing && (e < 0 || !(base > want))) e = i;
+                        base += x;
+                    }
+                    token = part * a.steps * kStep + run * 256 + 4 * who + e;
+                }
+            }
+            if (lane == 0) m.said = token;
+        }
+        __syncthreads();
+        if (m.said >= 0) return m.said;
+    }
+    return -1;
+}
+__device__ __forceinline__ void put_path(const VerifyArgs & a, const Rows & w, int s, int n, int token, const PathLds & m) {
+    int32_t * const rows = a.rows + (int64_t) s * a.max_path, * const out = a.out + (int64_t) s * a.max_path;
+    for (int i = threadIdx.x; i < a.max_path; i += kT) {
+        rows[i] = i < n ? m.path[i] : -1;
+        out[i] = i + 1 < n ? a.tokens[w.r0 + m.path[i + 1]] : i < n ? token : -1;
+    }
+    if (threadIdx.x == 0) a.count[s] = n, a.seq[s].done = 1;
+}
+
+// A workgroup has one part of every abreast-th row: those in work at a time are the next of the order that are not cut off. The workgroup meets
+// once for a part, where its wavefronts' sums come together: wavefront 1 has then looked up the next row, wavefront 0 goes on to
+// share the part's sums and to decide the row while the others are at the next.
+__global__ __launch_bounds__(kT, 4) void k_verify_rows(const VerifyArgs a) {
+    struct Met {
+        Running p[kT / 64], q[kT / 64];
+        int top[kT / 64];
+        Item next;
+    };
+    __shared__ double roots[16];
+    __shared__ Met met[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = blockIdx.x % a.parts;
+    if (tid < 16) roots[tid] = kRoots[tid];
+    int rank = blockIdx.x / a.parts;
+    Item it = a.items[rank];
+    const int n_items = min(*a.n_items, a.n_rows);
+    if (rank >= n_items) return;
+    __syncthreads();
+    for (int turn = 0;; turn ^= 1) {
+        // (starts that do not ascend)
+        if ((unsigned) it.s >= (unsigned) a.n_seq || it.r0 < 0 || it.j < 0 || it.n < 0 || it.r0 + it.j != it.r || it.j >= it.n || it.r0 > a.n_rows - it.n || it.n > kMaxRows) return;
+        Met & now = met[turn];
+        const Rows w{it.r0, it.n};
+        const bool greedy = !(it.t > 0.0f), drawn = a.draft && !greedy && it.child < w.n;
+        const double scale = greedy ? 1.0 : scale_of(it.t);
+        const float * const x = a.logits + it.r * a.ld, * const y = drawn ? a.draft + it.r * a.draft_ld : x;
+        Running p{-INFINITY, 0.0}, q{-INFINITY, 0.0};
+        Range p_in{0.0f, INFINITY, 0}, q_in{0.0f, INFINITY, 0};
+        int top = 0x7fffffff, i0 = part * a.steps * kStep + 4 * tid;
+        asm("" : "+v"(i0));  // (or every comparison with it is kept over the loop)
+        const auto load = [&](int k, float (&l)[4], float (&d)[4]) {
+            const bool whole = a.vec && (part * a.steps + k + 1) * kStep <= a.V;
+            values4(x, i0 + k * kStep, a.V, whole, l);
+            if (drawn) values4(y, i0 + k * kStep, a.V, whole, d);
+        };
+        float l[4], d[4], l1[4], d1[4];
+        load(0, l, d);
+        load(1, l1, d1);
+        Children kids{};
+        if (wave == 0 && it.child < w.n) kids = children(a, w, it.j, it.j + 1);
+#pragma unroll 1
+        for (int k = 0; k < a.steps; k++) {
+            float l2[4], d2[4];
+            if (k + 2 < a.steps) load(k + 2, l2, d2);
+            if (greedy) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) argmax_take(p.m, top, l[e] > kHuge ? kHuge : l[e], i0 + k * kStep + e);
+            } else {
+                p.take4(roots, scale, p_in, l);
+                if (drawn) q.take4(roots, scale, q_in, d);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) l[e] = l1[e], l1[e] = l2[e], d[e] = d1[e], d1[e] = d2[e];
+        }
+        const auto join = [&] {
+            if (greedy) {
+#pragma unroll 1
+                for (int o = 32; o > 0; o >>= 1) argmax_take(p.m, top, __shfl_xor(p.m, o, 64), __shfl_xor(top, o, 64));
+            } else {
+                p.wave(roots, scale);
+                if (drawn) q.wave(roots, scale);
+            }
+        };
+        if (wave == 1) {  // the next row that no decision so far cuts off, 64 at a time
+            for (rank += a.abreast; rank < n_items; rank += 64 * a.abreast) {
+                const int mine = rank + lane * a.abreast;
+                // (as two vectors: an Item goes by way of an address, which is made from the launch packet, in the host's memory:
+                // 2 us, 15 where a thousand workgroups do so)
+                bool on = mine >= rank && mine < n_items;
+                i4_t x = {}, y = {};  // r, s, j, parent; r0, n, t, child
+                if (on) {
+                    x = reinterpret_cast<const i4_t *>(a.items + mine)[0], y = reinterpret_cast<const i4_t *>(a.items + mine)[1];
+                    on = x.z == 0 || x.w >= 0;
+                    for (int c = x.z, u = x.w; on && u >= 0 && u < c && y.x >= 0 && y.x + c < a.n_rows;) {
+                        const int next = agent_load(&a.next[y.x + u]), up = a.parents[y.x + u];
+                        on = next == kOpen || next == c || (next <= kFell && c > kFell - next);
+                        c = u, u = up;
+                    }
+                }
+                const uint64_t at = __ballot(on);
+                if (at) {
+                    const int l = __builtin_ctzll(at);
+                    rank += l * a.abreast;
+                    if (lane == l) reinterpret_cast<i4_t *>(&now.next)[0] = x, reinterpret_cast<i4_t *>(&now.next)[1] = y;
+                    break;
+                }
+            }
+            if (rank >= n_items && lane == 0) now.next.n = -1;
+        }
+        join();
+        if (lane == 0) now.p[wave] = p, now.q[wave] = q, now.top[wave] = top;
+        __syncthreads();
+        const Item done = it;
+        it = now.next;
+        if (wave == 0) {
+            PartSums * const sums = a.sums + (int64_t) done.r * a.parts;
+            p = q = Running{-INFINITY, 0.0};
+            top = 0x7fffffff;
+            // first of the wavefronts, then, for the last of the row's workgroups to end, of the parts
+#pragma unroll 1
+            for (int round = 0;; round = 1) {
+                for (int i = lane; i < (round ? a.parts : kT / 64); i += 64) {
+                    const PartSums z = round ? shared(sums + i) : PartSums{now.p[i].s, now.q[i].s, now.p[i].m, now.q[i].m, now.top[i], 0};
+                    if (greedy) argmax_take(p.m, top, z.m_p, z.top);
+                    else {
+                        p.take(roots, scale, z.m_p, z.p);
+                        if (drawn) q.take(roots, scale, z.m_q, z.q);
+                    }
+                }
+                join();
+                if (round) break;
+                int last = 0;
+                if (lane == 0) {
+                    share(sums + part, PartSums{p.s, q.s, p.m, q.m, top, 0});
+                    stores_done();
+                    last = __hip_atomic_fetch_add(a.arrived + done.r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
+                }
+                if (!__builtin_amdgcn_readfirstlane(last)) {
+                    top = -2;
+                    break;
+                }
+                p = q = Running{-INFINITY, 0.0};
+                top = 0x7fffffff;
+            }
+            if (top != -2) {
+                double C = 0.0;
+                int next = kNone;
+                if (p.m > -INFINITY && done.child < w.n)
+                    next = decide(a, w, done.j, done.j, greedy ? top : -1, 1.0, soft(roots, scale, p.m, p.s), soft(roots, scale, q.m, q.s), kids, done.j + 1, C);
+                if (lane == 0) {
+                    agent_store(&a.next[done.r], next);
+                    a.state[done.r] = RowState{p.s, q.s, C, p.m, q.m, top, 0};
+                }
+            }
+        }
+        if (it.n < 0) return;
+    }
+}
+
+// The walk of one sequence. Where a drawn child of its last row fell each workgroup sums a part of r, for the draw or for the next child, and
+// the last to end goes on, in the last launch alone to the end; else the parts' sums are k_verify_rows's, and workgroup 0 draws.
 __global__ __launch_bounds__(kT) void k_verify_walk(const VerifyArgs a) {
-    constexpr int E = kDraw * kT;
-    __shared__ double roots[16], red[2][kT / 64];
-    __shared__ int next[kMaxRows], path[kMaxRows];
-    __shared__ uint32_t gone[E / 32];
-    __shared__ int flag, n_path, said;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, s = blockIdx.x / a.draws;
-    if (a.seq[s].done) return;
+    __shared__ PathLds m;
+    const int tid = threadIdx.x, wave = tid >> 6, s = blockIdx.x / a.each, own = blockIdx.x % a.each;
     const Rows w = rows_of(a.starts, s, a.n_rows, a.max_rows);
     const float t = a.temperature ? a.temperature[s] : 1.0f;
+    if (a.seq[s].done) return;
     const bool greedy = !(t > 0.0f);
-    const double inv_t = greedy ? 1.0 : 1.0 / (double) t;
-    if (tid < 16) roots[tid] = a.roots[tid];
-    bool alone = false;
-    for (;;) {
-        // the path as far as it is known
-        for (int j = tid; j < w.n; j += kT) next[j] = a.state[w.r0 + j].next;
-        __syncthreads();
-        if (tid == 0) {
-            int n = 0;
-            for (int u = 0; w.n > 0 && n < a.max_path;) {
-                path[n++] = u;
-                if (next[u] <= u || next[u] >= w.n) break;
-                u = next[u];
+    const double scale = greedy ? 1.0 : scale_of(t);
+    if (tid < 16) m.roots[tid] = kRoots[tid];
+    for (bool alone = false;;) {
+        int u;
+        const int n = find_path(a, w, m, u), then = n ? __builtin_amdgcn_readfirstlane(m.next[u]) : (int) kOpen;
+        const RowState st = n ? shared(a.state + w.r0 + u) : RowState{};
+        const Source z = source(w, s, u, st, m.roots, scale);
+        if (n && !greedy && st.C > 0.0 && (then == kNone || then <= kFell)) {
+#pragma unroll 1
+            for (int b = alone ? 0 : own; b < (alone ? a.parts : own + 1); b++) {
+                const double v = runs(a, z, m, b, false);
+                if (tid == 0) share(a.drawn + (int64_t) s * a.parts + b, v);
             }
-            n_path = n;
-        }
-        __syncthreads();
-        const int n = n_path, u = n ? path[n - 1] : 0;
-        const RowState z = n ? a.state[w.r0 + u] : RowState{};
-        const bool fell = z.next <= kFell, draw = n && (z.next == kNone || fell) && z.m_p > -INFINITY && !greedy;
-        int token = -1;
-        if (!draw) {
-            if (!alone && blockIdx.x % a.draws) return;
-            if (n && z.next >= 0 && z.next < w.n) token = a.tokens[w.r0 + z.next];  // (a path cut short)
-            else if (n && greedy && z.m_p > -INFINITY) token = z.top;
-        } else {
-            const Soft p = soft(roots, inv_t, z.m_p, z.sum_p), q = soft(roots, inv_t, z.m_q, z.sum_q);
-            const float * x = a.logits + (w.r0 + u) * a.ld, * y = a.draft + (w.r0 + u) * a.draft_ld;
-            // the weights of the part's tokens i .. that this thread has; all: of r, the guesses that fell taken out, or of p
-            const auto weights = [&](int part, bool all, double (&v)[kDraw], double & sum_w, double & sum_p) {
-                const int i = part * E + kDraw * tid;
-                float l[kDraw];
-                values<kDraw>(x, i, a.V, a.vec, l);
-                uint32_t out = 0;
-                if (!a.draft) {
-                    for (int b = tid; b < E / 32; b += kT) gone[b] = 0;
-                    __syncthreads();
-                    for (int j = u + 1 + tid; j < w.n; j += kT)
-                        if (a.parents[w.r0 + j] == u) {
-                            const unsigned e = (unsigned) a.tokens[w.r0 + j] - (unsigned) (part * E);
-                            if (e < (unsigned) E) atomicOr(&gone[e / 32], 1u << (e % 32));
-                        }
-                    __syncthreads();
-                    out = gone[tid * kDraw / 32] >> (tid * kDraw % 32);
-                }
-                sum_w = sum_p = 0.0;
-                float d[kDraw];
-                if (z.C > 0.0) values<kDraw>(y, i, a.V, a.vec, d);
-#pragma unroll
-                for (int e = 0; e < kDraw; e++) {
-                    const double pe = p.p(l[e]);
-                    v[e] = all ? pe : out >> e & 1 ? 0.0 : z.C > 0.0 ? fmax(pe - z.C * q.p(d[e]), 0.0) : pe;
-                    sum_w += v[e];
-                    sum_p += pe;
-                }
-            };
-            Drawn * const drawn = a.drawn + (int64_t) s * a.draws;
-            double v[kDraw];
-            for (int part = alone ? 0 : blockIdx.x % a.draws; part < a.draws; part++) {
-                double sw, sp;
-                weights(part, false, v, sw, sp);
-                sw = wave_sum_d(sw);
-                sp = wave_sum_d(sp);
-                if (lane == 0) red[0][wave] = sw, red[1][wave] = sp;
+            if (alone) {
+                if (tid == 0) stores_done();
                 __syncthreads();
-                if (tid == 0) {
-                    sw = sp = 0.0;
-                    for (int i = 0; i < kT / 64; i++) sw += red[0][i], sp += red[1][i];
-                    share(drawn + part, Drawn{sw, sp});
-                }
-                __syncthreads();
-                if (!alone) break;
-            }
-            if (!alone && !last_of(&a.seq[s].arrived, a.draws, &flag)) return;
-            // the parts' sums up to each one's, 64 parts at a time
-            const Drawn mine64 = lane < a.draws ? shared(drawn + lane) : Drawn{};
-            const auto part_of = [&](int i0) { return i0 ? (i0 + lane < a.draws ? shared(drawn + i0 + lane) : Drawn{}) : mine64; };
-            const auto upto = [&](double v) {
-                for (int o = 1; o < 64; o <<= 1) {
-                    const double b = __shfl_up(v, o, 64);
-                    if (lane >= o) v += b;
-                }
-                return v;
-            };
-            const auto sum_of = [&](bool all) {
-                double sum = 0.0;
-                for (int i0 = 0; i0 < a.draws; i0 += 64) {
-                    const Drawn d = part_of(i0);
-                    sum += readlane_d(upto(all ? d.p : d.w), 63);
-                }
-                return sum;
-            };
-            double total = sum_of(false);
-            if (fell) {
+            } else if (!last_of(&a.seq[s].arrived, a.parts, &m.flag)) return;
+            if (then <= kFell) {
                 if (wave == 0) {
-                    RowState o = z;
-                    const int from = kFell - z.next, j0 = from + 1;
-                    decide_drawn(a, w, u, from, total, p, q, children(a, w, u, j0), j0, o);
-                    if (lane == 0) a.state[w.r0 + u].C = o.C, a.state[w.r0 + u].next = o.next;
+                    double C = st.C, c = 0.0;
+                    for (int i0 = 0; i0 < a.parts; i0 += 64) c += wave_sum_d(part_sum(a, z, i0, false));
+                    const int from = kFell - then, next = decide(a, w, u, from, -1, c, z.p, z.q, children(a, w, u, from + 1), from + 1, C);
+                    if (tid == 0) {
+                        agent_store(&a.state[w.r0 + u].C, C);
+                        agent_store(&a.next[w.r0 + u], next);
+                        stores_done();
+                    }
                 }
                 if (!a.last) {
                     if (tid == 0) a.seq[s].arrived = 0;
                     return;
                 }
-                alone = true;
                 __syncthreads();
+                alone = true;
                 continue;
             }
-            // the part, the thread, the token where the cumulative sum passes the coin's share
-            const bool all = !(total > 0.0);
-            if (all) total = sum_of(true);
-            const float coin = a.coins[w.r0];
-            const double want = (coin > 0.0f ? fmin((double) coin, 1.0 - 0x1p-24) : 0.0) * total;
-            int part = 0;
-            double base = 0.0, below = 0.0;
-            for (int i0 = 0; i0 < a.draws; i0 += 64) {
-                const Drawn x = part_of(i0);
-                const double d = all ? x.p : x.w, sum = upto(d);
-                const uint64_t some = __ballot(d > 0.0), hit = __ballot(d > 0.0 && below + sum > want);
-                if (some) {  // (the last one with a weight, if rounding leaves no other)
-                    const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
-                    part = i0 + l;
-                    base = l ? below + readlane_d(sum, l - 1) : below;
-                }
-                if (hit) break;
-                below += readlane_d(sum, 63);
-            }
-            double mine, sp;
-            weights(part, all, v, mine, sp);
-            if (all) mine = sp;
-            const double sums = upto(mine);
-            if (lane == 63) red[0][wave] = sums;
-            if (tid == 0) flag = kT, said = -1;
-            __syncthreads();
-            for (int i = 0; i < wave; i++) base += red[0][i];
-            if (mine > 0.0) {
-                if (base + sums > want) atomicMin(&flag, tid);
-                atomicMax(&said, tid);
-            }
-            __syncthreads();
-            const int who = flag < kT ? flag : said;  // (rounding may leave none: the last one)
-            __syncthreads();
-            if (tid == who) {
-                double c = base + (sums - mine);
-                int e0 = 0;
-                for (int e = 0; e < kDraw; e++)
-                    if (v[e] > 0.0) {
-                        e0 = e;
-                        c += v[e];
-                        if (c > want) break;
-                    }
-                said = part * E + kDraw * tid + e0;
-            }
-            __syncthreads();
-            token = said;
-        }
-        int32_t * const rows = a.rows + (int64_t) s * a.max_path, * const out = a.out + (int64_t) s * a.max_path;
-        for (int i = tid; i < a.max_path; i += kT) {
-            rows[i] = i < n ? path[i] : -1;
-            out[i] = i + 1 < n ? a.tokens[w.r0 + path[i + 1]] : i < n ? token : -1;
-        }
-        if (tid == 0) a.count[s] = n, a.seq[s].done = 1;
+        } else if (own && !alone) return;
+        int token = -1;
+        if (n && then >= 0 && then < w.n) token = a.tokens[w.r0 + then];  // (a path cut short)
+        else if (n && then == kNone && st.m_p > -INFINITY) token = greedy ? st.top : draw(a, z, m);
+        __syncthreads();
+        put_path(a, w, s, n, token, m);
         return;
     }
 }
 
-// How a call is cut: values of a workgroup, and of a draw's.
+// How a call is cut, and its workspace.
 struct VerifyShape {
-    int nv, parts, draws;
-    size_t items, state, sums, seq, drawn, total;  // offsets
+    int steps, parts;
+    size_t items, state, next, arrived, sums, seq, drawn, total;  // offsets
 };
 VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     VerifyShape z{};
-    z.nv = n_rows * ((V + 8191) / 8192) >= 1024 ? 8 : 2;
-    z.parts = (int) ((V + z.nv * 4 * kT - 1) / (z.nv * 4 * kT));
-    z.draws = (int) ((V + kDraw * kT - 1) / (kDraw * kT));
+    z.steps = 2;
+    while (z.steps < kSteps && n_rows * ((V + z.steps * kStep - 1) / (z.steps * kStep)) > kRowGroups) z.steps *= 2;
+    z.parts = (int) ((V + z.steps * kStep - 1) / (z.steps * kStep));
     z.items = 256;
     z.state = z.items + align256((size_t) n_rows * sizeof(Item));
-    z.sums = z.state + align256((size_t) n_rows * sizeof(RowState));
+    z.next = z.state + align256((size_t) n_rows * sizeof(RowState));
+    z.arrived = z.next + align256((size_t) n_rows * sizeof(int));
+    z.sums = z.arrived + align256((size_t) n_rows * sizeof(int));
     z.seq = z.sums + align256((size_t) n_rows * z.parts * sizeof(PartSums));
     z.drawn = z.seq + align256((size_t) n_seq * sizeof(SeqState));
-    z.total = z.drawn + align256((size_t) n_seq * z.draws * sizeof(Drawn));
+    z.total = z.drawn + align256((size_t) n_seq * z.parts * sizeof(double));
     return z;
 }
 
@@ -792,25 +958,25 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         a.starts = starts, a.parents = parents, a.tokens = tokens, a.logits = logits, a.ld = ld, a.draft = draft_logits, a.draft_ld = draft_ld;
         a.temperature = temperature, a.coins = coins, a.n_seq = n_seq, a.n_rows = (int) n_rows, a.V = (int) n_vocab;
         a.max_rows = (int) std::min<int64_t>(max_rows, std::max<int64_t>(n_rows, 1)), a.max_path = max_path;
-        a.parts = z.parts, a.draws = z.draws;
+        a.parts = z.parts, a.steps = z.steps;
         a.vec = aligned(logits, 16) && ld % 4 == 0 && (!draft_logits || (aligned(draft_logits, 16) && draft_ld % 4 == 0));
         a.count = count, a.rows = rows, a.out = tokens_out;
-        a.n_items = (int *) at, a.items = (Item *) (at + z.items), a.state = (RowState *) (at + z.state);
-        a.sums = (PartSums *) (at + z.sums), a.seq = (SeqState *) (at + z.seq), a.drawn = (Drawn *) (at + z.drawn);
-        for (int i = 0; i < 16; i++) a.roots[i] = std::exp2(i / 16.0);
+        a.n_items = (int *) at, a.items = (Item *) (at + z.items), a.state = (RowState *) (at + z.state), a.next = (int *) (at + z.next);
+        a.arrived = (int *) (at + z.arrived), a.sums = (PartSums *) (at + z.sums), a.seq = (SeqState *) (at + z.seq), a.drawn = (double *) (at + z.drawn);
         hipStream_t st = as_stream(stream);
         k_verify_begin<<<paged_grid(std::max<int64_t>((n_rows + 3) / 4, 1), kT), kT, 0, st>>>(a);
         check_launch("draft verify");
-        if (n_rows) {
-            const unsigned grid = paged_grid(n_rows * z.parts, kT);
-            if (z.nv == 8) k_verify_rows<8><<<grid, kT, 0, st>>>(a);
-            else k_verify_rows<2><<<grid, kT, 0, st>>>(a);
-            check_launch("draft verify rows");
-        }
+        if (n_rows == 0) return;
+        a.each = draft_logits ? z.parts : 1;
+        a.abreast = (int) std::min<int64_t>(n_rows, std::max(1, kRowGroups / z.parts));
+        const unsigned grid = paged_grid((int64_t) a.abreast * z.parts, kT);
+        k_verify_rows<<<grid, kT, 0, st>>>(a);
+        check_launch("draft verify rows");
         // A path that cannot be all of a sequence's rows tells that rows have several children, of which some will fall.
-        for (int left = draft_logits && max_path < a.max_rows && z.draws > 4 ? 3 : 1; left; left--) {
-            a.last = left == 1;
-            k_verify_walk<<<paged_grid((int64_t) n_seq * z.draws, kT), kT, 0, st>>>(a);
+        const int walks = draft_logits && max_path < a.max_rows && z.parts > 4 ? 3 : 1;
+        for (int i = 0; i < walks; i++) {
+            a.last = i == walks - 1;
+            k_verify_walk<<<paged_grid((int64_t) n_seq * a.each, kT), kT, 0, st>>>(a);
             check_launch("draft verify walk");
         }
     });
