@@ -156,55 +156,57 @@ struct VerifyArgs {
     double * drawn;
 };
 
-// 2^(i / 16)
-__constant__ double kRoots[16] = {
-    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.189207115002721, 1.241857812073484,
-    1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
-    1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+// 2^(i / 32)
+__constant__ double kRoots[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
+    1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103,
+    1.9152065613971474, 1.9571441241754002};
 
-// exp by a sixteenth of a power of two from LDS (a bank of its own each) and five terms of exp's series on what is left: |z| <= ln 2 / 32, the
-// sixth is 2^-43. 12 operations of 64 bits and 5 others in `weigh4`, where the kernels spend their arithmetic; the library's takes
-// some 30. (Loops are left as loops here, and code is written once: most of it runs once in a workgroup, and fetching 40 KB of it took
-// longer than what it did.)
-__device__ __forceinline__ double power(double r) {  // 2^(r / 16), |r| <= 1 / 2
-    constexpr double k = 0.043321698784996581;           // ln 2 / 16
-    double y = fma(r, k * k * k * k * k / 120, k * k * k * k / 24);
-    y = fma(r, y, k * k * k / 6);
+// exp by a 32nd of a power of two from LDS and four terms of exp's series on what is left, the fifth taken into the others
+// (z^5 = 5/4 a^2 z^3 - 5/16 a^4 z but for a^5 / 16, |z| <= a = ln 2 / 64: 2^-43). 11 operations of 64 bits and 5 others in `weigh4`, where the
+// kernels spend their arithmetic; the library's takes some 30. (Loops are left as loops here, and code is written once: most of it
+// runs once in a workgroup, and fetching 40 KB of it took longer than what it did.)
+__device__ __forceinline__ double power(double r) {  // 2^(r / 32), |r| <= 1 / 2
+    constexpr double k = 0.021660849392498290;           // ln 2 / 32
+    constexpr double c5 = k * k * k * k * k / 120;
+    double y = fma(r, k * k * k * k / 24, k * k * k / 6 + c5 * 0.3125);
     y = fma(r, y, k * k / 2);
-    y = fma(r, y, k);
+    y = fma(r, y, k - c5 * 0.01953125);
     return fma(r, y, 1.0);
 }
-// 2^(n / 16)
+// 2^(n / 32)
 __device__ __forceinline__ double root(const double * roots, int n) {
-    const double y = roots[n & 15];
-    return __hiloint2double(__double2hiint(y) + ((n & ~15) << 16), __double2loint(y));
+    const double y = roots[n & 31];
+    return __hiloint2double(__double2hiint(y) + ((n & ~31) << 15), __double2loint(y));
 }
 struct Soft {
     const double * roots;  // LDS
-    double scale, m, inv;  // 16 / (t ln 2); a logit that weighs 1, the row's weights are below 2^512; 1 / their sum
+    double scale, m, inv;  // 32 / (t ln 2); a logit that weighs 1, the row's weights are below 2^512; 1 / their sum
     // exp((l - m) / t), 0 from 2^-1000 on
     __device__ __forceinline__ double weight(float l) const {
         if (l > kHuge) l = kHuge;
         const double x = ((double) l - m) * scale, t = x + 0x1.8p52, y = power(x - (t - 0x1.8p52)) * root(roots, (int) (uint32_t) __double_as_longlong(t));
-        return x > -16000.0 ? y : 0.0;  // (nor for -inf and NaN)
+        return x > -32000.0 ? y : 0.0;  // (nor for -inf and NaN)
     }
     __device__ __forceinline__ double p(float l) const { return weight(l) * inv; }
 };
-__device__ __forceinline__ double scale_of(float t) { return 23.083120654223414 / (double) t; }
+__device__ __forceinline__ double scale_of(float t) { return 46.166241308446828 / (double) t; }
 __device__ __forceinline__ Soft soft(const double * roots, double scale, float m, double sum) { return {roots, scale, (double) m, sum > 0.0 ? 1.0 / sum : 0.0}; }
 
 // Logits around m where the short form serves: those above `low` (2^-1000; what is below counts as that, no more than 2^-1000 each, NaN too),
-// and not above `high`, 2^500. odd: there is no such range in f32, or no such m.
+// and not above `high`, 2^500; -inf if there is no such range in f32, or no such m.
 struct Range {
     float low, high;
-    int odd;
 };
 __device__ __forceinline__ Range range_of(float m, double scale) {
-    const double d = 16000.0 / scale;
-    Range z{(float) ((double) m - d), (float) ((double) m + 0.5 * d), 0};
+    const double d = 32000.0 / scale;
+    const Range z{(float) ((double) m - d), (float) ((double) m + 0.5 * d)};
     const double x = ((double) z.low - (double) m) * scale;
-    z.odd = !(fabsf(m) < 1e38f) || !(x > -16300.0 && x < -15700.0);  // (root's powers end at 2^-1022)
-    return z;
+    const bool odd = !(fabsf(m) < 1e38f) || !(x > -32600.0 && x < -31400.0);  // (root's powers end at 2^-1022)
+    return {z.low, odd ? -INFINITY : z.high};
 }
 // The weights of four logits in that range (two, then two: more at a time than the registers hold).
 __device__ __forceinline__ void weigh4(const double * roots, double scale, double m, float low, const float (&l)[4], double (&v)[4]) {
@@ -229,30 +231,30 @@ struct Running {
         s = s * z.weight(m) + s2 * z.weight(m2);
         m = fmaxf(m, m2);
     }
+    // in: m's, at first {0, -inf}
     __device__ __forceinline__ void take4(const double * roots, double scale, Range & in, const float (&l)[4]) {
         const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
-        if (__any(m == -INFINITY && top > -INFINITY))
+        if (__any(top > in.high)) {
             if (m == -INFINITY && top > -INFINITY) {
                 m = fminf(top, kHuge), s = 0.0;
-                const Range z = range_of(m, scale);
-                in.low = z.low, in.high = z.high, in.odd = z.odd;
+                in = range_of(m, scale);
             }
-        if (__any(top > in.high || in.odd)) {
-            const float to = fminf(fmaxf(m, top), kHuge);
-            if (to > -INFINITY) {
-                const Soft z{roots, scale, (double) to, 0.0};
-                s *= z.weight(m);
-                m = to;
-                const Range w = range_of(m, scale);
-                in.low = w.low, in.high = w.high, in.odd = w.odd;
-                float x = l[0], y = l[1], u = l[2], v = l[3];
+            if (__any(top > in.high)) {
+                const float to = fminf(fmaxf(m, top), kHuge);
+                if (to > -INFINITY) {
+                    const Soft z{roots, scale, (double) to, 0.0};
+                    s *= z.weight(m);
+                    m = to;
+                    in = range_of(m, scale);
+                    float x = l[0], y = l[1], u = l[2], v = l[3];
 #pragma unroll 1
-                for (int e = 0; e < 4; e++) {
-                    s += z.weight(x);
-                    x = y, y = u, u = v;
+                    for (int e = 0; e < 4; e++) {
+                        s += z.weight(x);
+                        x = y, y = u, u = v;
+                    }
                 }
+                return;
             }
-            return;
         }
         double v[4];
         weigh4(roots, scale, m > -INFINITY ? (double) m : 0.0, in.low, l, v);
@@ -419,7 +421,7 @@ __device__ __forceinline__ int decide(const VerifyArgs & a, const Rows & w, int 
 
 // What a workgroup keeps in LDS of the path and of a draw.
 struct PathLds {
-    double roots[16], seg[4 * kSteps];  // sums of a part's runs of 256 tokens
+    double roots[32], seg[4 * kSteps];  // sums of a part's runs of 256 tokens
     int next[kMaxRows], path[kMaxRows];
     uint32_t gone[kSteps * kStep / 32];
     int flag, said;
@@ -463,7 +465,7 @@ struct Source {
 };
 __device__ __forceinline__ Source source(const Rows & w, int s, int u, const RowState & st, const double * roots, double scale) {
     const Range p = range_of(st.m_p, scale), q = st.C > 0.0 ? range_of(st.m_q, scale) : p;
-    return {w, s, u, st.C, soft(roots, scale, st.m_p, st.sum_p), soft(roots, scale, st.m_q, st.sum_q), p.low, q.low, p.odd || q.odd};
+    return {w, s, u, st.C, soft(roots, scale, st.m_p, st.sum_p), soft(roots, scale, st.m_q, st.sum_q), p.low, q.low, !(p.high > -INFINITY && q.high > -INFINITY)};
 }
 // The weights of the tokens whose logits are l (the drafter's d), from token i of a part on, of r or (all) of p.
 __device__ __forceinline__ void weights4(const VerifyArgs & a, const Source & z, const PathLds & m, int i, bool all, const float (&l)[4], const float (&d)[4], double (&v)[4]) {
@@ -617,116 +619,104 @@ __device__ __forceinline__ void put_path(const VerifyArgs & a, const Rows & w, i
     if (threadIdx.x == 0) a.count[s] = n, a.seq[s].done = 1;
 }
 
-// A workgroup has one part of every abreast-th row: those in work at a time are the next of the order that are not cut off. The workgroup meets
-// once for a part, where its wavefronts' sums come together: wavefront 1 has then looked up the next row, wavefront 0 goes on to
-// share the part's sums and to decide the row while the others are at the next.
-__global__ __launch_bounds__(kT, 4) void k_verify_rows(const VerifyArgs a) {
+// A workgroup has one part of every abreast-th row: those in work at a time are the next of the order that are not cut off. Four wavefronts
+// read; the fifth meets them once for a part: it has then looked up the next row, and shares the part's sums and, its row's last,
+// decides while they read that.
+__global__ __launch_bounds__(kT + 64, 5) void k_verify_rows(const VerifyArgs a) {
     struct Met {
         Running p[kT / 64], q[kT / 64];
         int top[kT / 64];
         Item next;
     };
-    __shared__ double roots[16];
+    __shared__ double roots[32];
     __shared__ Met met[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = blockIdx.x % a.parts;
-    if (tid < 16) roots[tid] = kRoots[tid];
+    if (tid < 32) roots[tid] = kRoots[tid];
     int rank = blockIdx.x / a.parts;
     Item it = a.items[rank];
     const int n_items = min(*a.n_items, a.n_rows);
     if (rank >= n_items) return;
     __syncthreads();
+    const auto join = [&](bool greedy, bool drawn, double scale, Running & p, Running & q, int & top) {
+        if (greedy) {
+#pragma unroll 1
+            for (int o = 32; o > 0; o >>= 1) argmax_take(p.m, top, __shfl_xor(p.m, o, 64), __shfl_xor(top, o, 64));
+        } else {
+            p.wave(roots, scale);
+            if (drawn) q.wave(roots, scale);
+        }
+    };
+    const auto good = [&](const Item & it) {  // (starts that do not ascend)
+        return (unsigned) it.s < (unsigned) a.n_seq && it.r0 >= 0 && it.j >= 0 && it.r0 + it.j == it.r && it.j < it.n && it.r0 <= a.n_rows - it.n && it.n <= kMaxRows;
+    };
+    if (wave < kT / 64) {
+        for (int turn = 0; good(it); turn ^= 1) {
+            Met & now = met[turn];
+            const bool greedy = !(it.t > 0.0f), drawn = a.draft && !greedy && it.child < it.n;
+            const double scale = greedy ? 1.0 : scale_of(it.t);
+            const float * const x = a.logits + it.r * a.ld, * const y = drawn ? a.draft + it.r * a.draft_ld : x;
+            Running p{-INFINITY, 0.0}, q{-INFINITY, 0.0};
+            Range p_in{0.0f, -INFINITY}, q_in{0.0f, -INFINITY};
+            int top = 0x7fffffff, i0 = part * a.steps * kStep + 4 * tid;
+            asm("" : "+v"(i0));  // (or every comparison with it is kept over the loop)
+            const auto load = [&](int k, float (&l)[4], float (&d)[4]) {
+                const bool whole = a.vec && (part * a.steps + k + 1) * kStep <= a.V;
+                values4(x, i0 + k * kStep, a.V, whole, l);
+                if (drawn) values4(y, i0 + k * kStep, a.V, whole, d);
+            };
+            const auto take = [&](int k, const float (&l)[4], const float (&d)[4]) {
+                if (greedy) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) argmax_take(p.m, top, l[e] > kHuge ? kHuge : l[e], i0 + k * kStep + e);
+                } else {
+                    p.take4(roots, scale, p_in, l);
+                    if (drawn) q.take4(roots, scale, q_in, d);
+                }
+            };
+            float l[2][4], d[2][4];
+            load(0, l[0], d[0]);
+            load(1, l[1], d[1]);
+#pragma unroll 1
+            for (int k = 0; k < a.steps; k += 2) {  // (an even number)
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    take(k + b, l[b], d[b]);
+                    if (k + b + 2 < a.steps) load(k + b + 2, l[b], d[b]);
+                }
+            }
+            join(greedy, drawn, scale, p, q, top);
+            if (lane == 0) now.p[wave] = p, now.q[wave] = q, now.top[wave] = top;
+            __syncthreads();
+            it = now.next;
+        }
+        return;
+    }
+    Item done{};
     for (int turn = 0;; turn ^= 1) {
-        // (starts that do not ascend)
-        if ((unsigned) it.s >= (unsigned) a.n_seq || it.r0 < 0 || it.j < 0 || it.n < 0 || it.r0 + it.j != it.r || it.j >= it.n || it.r0 > a.n_rows - it.n || it.n > kMaxRows) return;
-        Met & now = met[turn];
-        const Rows w{it.r0, it.n};
-        const bool greedy = !(it.t > 0.0f), drawn = a.draft && !greedy && it.child < w.n;
-        const double scale = greedy ? 1.0 : scale_of(it.t);
-        const float * const x = a.logits + it.r * a.ld, * const y = drawn ? a.draft + it.r * a.draft_ld : x;
-        Running p{-INFINITY, 0.0}, q{-INFINITY, 0.0};
-        Range p_in{0.0f, INFINITY, 0}, q_in{0.0f, INFINITY, 0};
-        int top = 0x7fffffff, i0 = part * a.steps * kStep + 4 * tid;
-        asm("" : "+v"(i0));  // (or every comparison with it is kept over the loop)
-        const auto load = [&](int k, float (&l)[4], float (&d)[4]) {
-            const bool whole = a.vec && (part * a.steps + k + 1) * kStep <= a.V;
-            values4(x, i0 + k * kStep, a.V, whole, l);
-            if (drawn) values4(y, i0 + k * kStep, a.V, whole, d);
-        };
-        float l[4], d[4], l1[4], d1[4];
-        load(0, l, d);
-        load(1, l1, d1);
-        Children kids{};
-        if (wave == 0 && it.child < w.n) kids = children(a, w, it.j, it.j + 1);
-#pragma unroll 1
-        for (int k = 0; k < a.steps; k++) {
-            float l2[4], d2[4];
-            if (k + 2 < a.steps) load(k + 2, l2, d2);
-            if (greedy) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) argmax_take(p.m, top, l[e] > kHuge ? kHuge : l[e], i0 + k * kStep + e);
-            } else {
-                p.take4(roots, scale, p_in, l);
-                if (drawn) q.take4(roots, scale, q_in, d);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) l[e] = l1[e], l1[e] = l2[e], d[e] = d1[e], d1[e] = d2[e];
-        }
-        const auto join = [&] {
-            if (greedy) {
-#pragma unroll 1
-                for (int o = 32; o > 0; o >>= 1) argmax_take(p.m, top, __shfl_xor(p.m, o, 64), __shfl_xor(top, o, 64));
-            } else {
-                p.wave(roots, scale);
-                if (drawn) q.wave(roots, scale);
-            }
-        };
-        if (wave == 1) {  // the next row that no decision so far cuts off, 64 at a time
-            for (rank += a.abreast; rank < n_items; rank += 64 * a.abreast) {
-                const int mine = rank + lane * a.abreast;
-                // (as two vectors: an Item goes by way of an address, which is made from the launch packet, in the host's memory:
-                // 2 us, 15 where a thousand workgroups do so)
-                bool on = mine >= rank && mine < n_items;
-                i4_t x = {}, y = {};  // r, s, j, parent; r0, n, t, child
-                if (on) {
-                    x = reinterpret_cast<const i4_t *>(a.items + mine)[0], y = reinterpret_cast<const i4_t *>(a.items + mine)[1];
-                    on = x.z == 0 || x.w >= 0;
-                    for (int c = x.z, u = x.w; on && u >= 0 && u < c && y.x >= 0 && y.x + c < a.n_rows;) {
-                        const int next = agent_load(&a.next[y.x + u]), up = a.parents[y.x + u];
-                        on = next == kOpen || next == c || (next <= kFell && c > kFell - next);
-                        c = u, u = up;
-                    }
-                }
-                const uint64_t at = __ballot(on);
-                if (at) {
-                    const int l = __builtin_ctzll(at);
-                    rank += l * a.abreast;
-                    if (lane == l) reinterpret_cast<i4_t *>(&now.next)[0] = x, reinterpret_cast<i4_t *>(&now.next)[1] = y;
-                    break;
-                }
-            }
-            if (rank >= n_items && lane == 0) now.next.n = -1;
-        }
-        join();
-        if (lane == 0) now.p[wave] = p, now.q[wave] = q, now.top[wave] = top;
-        __syncthreads();
-        const Item done = it;
-        it = now.next;
-        if (wave == 0) {
+        // the row before: its sums first of the wavefronts, then, for the last of the row's workgroups to end, of the parts
+        const auto end = [&] {
+            const Met & was = met[turn ^ 1];
+            const Rows w{done.r0, done.n};
+            const bool greedy = !(done.t > 0.0f), drawn = a.draft && !greedy && done.child < done.n;
+            const double scale = greedy ? 1.0 : scale_of(done.t);
             PartSums * const sums = a.sums + (int64_t) done.r * a.parts;
-            p = q = Running{-INFINITY, 0.0};
-            top = 0x7fffffff;
-            // first of the wavefronts, then, for the last of the row's workgroups to end, of the parts
+            Children kids{};
+            if (done.child < done.n) kids = children(a, w, done.j, done.j + 1);
+            Running p, q;
+            int top;
 #pragma unroll 1
-            for (int round = 0;; round = 1) {
+            for (int round = 0; round < 2; round++) {
+                p = q = Running{-INFINITY, 0.0};
+                top = 0x7fffffff;
                 for (int i = lane; i < (round ? a.parts : kT / 64); i += 64) {
-                    const PartSums z = round ? shared(sums + i) : PartSums{now.p[i].s, now.q[i].s, now.p[i].m, now.q[i].m, now.top[i], 0};
+                    const PartSums z = round ? shared(sums + i) : PartSums{was.p[i].s, was.q[i].s, was.p[i].m, was.q[i].m, was.top[i], 0};
                     if (greedy) argmax_take(p.m, top, z.m_p, z.top);
                     else {
                         p.take(roots, scale, z.m_p, z.p);
                         if (drawn) q.take(roots, scale, z.m_q, z.q);
                     }
                 }
-                join();
+                join(greedy, drawn, scale, p, q, top);
                 if (round) break;
                 int last = 0;
                 if (lane == 0) {
@@ -734,25 +724,47 @@ __global__ __launch_bounds__(kT, 4) void k_verify_rows(const VerifyArgs a) {
                     stores_done();
                     last = __hip_atomic_fetch_add(a.arrived + done.r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
                 }
-                if (!__builtin_amdgcn_readfirstlane(last)) {
-                    top = -2;
-                    break;
-                }
-                p = q = Running{-INFINITY, 0.0};
-                top = 0x7fffffff;
+                if (!__builtin_amdgcn_readfirstlane(last)) return;
             }
-            if (top != -2) {
-                double C = 0.0;
-                int next = kNone;
-                if (p.m > -INFINITY && done.child < w.n)
-                    next = decide(a, w, done.j, done.j, greedy ? top : -1, 1.0, soft(roots, scale, p.m, p.s), soft(roots, scale, q.m, q.s), kids, done.j + 1, C);
-                if (lane == 0) {
-                    agent_store(&a.next[done.r], next);
-                    a.state[done.r] = RowState{p.s, q.s, C, p.m, q.m, top, 0};
+            double C = 0.0;
+            int next = kNone;
+            if (p.m > -INFINITY && done.child < done.n)
+                next = decide(a, w, done.j, done.j, greedy ? top : -1, 1.0, soft(roots, scale, p.m, p.s), soft(roots, scale, q.m, q.s), kids, done.j + 1, C);
+            if (lane == 0) {
+                agent_store(&a.next[done.r], next);
+                a.state[done.r] = RowState{p.s, q.s, C, p.m, q.m, top, 0};
+            }
+        };
+        if (done.n > 0) end();
+        if (!good(it)) return;
+        // the next row that no decision so far cuts off, 64 at a time
+        // (as two vectors: an Item goes by way of an address, which is made from the launch packet, in the host's memory: 2 us, 15 where a
+        // thousand workgroups do so)
+        i4_t x = {}, y = {};  // r, s, j, parent; r0, n, t, child
+        for (rank += a.abreast; rank < n_items; rank += 64 * a.abreast) {
+            const int mine = rank + lane * a.abreast;
+            bool on = mine >= rank && mine < n_items;
+            if (on) {
+                x = reinterpret_cast<const i4_t *>(a.items + mine)[0], y = reinterpret_cast<const i4_t *>(a.items + mine)[1];
+                on = x.z == 0 || x.w >= 0;
+                for (int c = x.z, u = x.w; on && u >= 0 && u < c && y.x >= 0 && y.x + c < a.n_rows;) {
+                    const int next = agent_load(&a.next[y.x + u]), up = a.parents[y.x + u];
+                    on = next == kOpen || next == c || (next <= kFell && c > kFell - next);
+                    c = u, u = up;
                 }
+            }
+            const uint64_t at = __ballot(on);
+            if (at) {
+                const int l = __builtin_ctzll(at);
+                rank += l * a.abreast;
+                if (lane == l) reinterpret_cast<i4_t *>(&met[turn].next)[0] = x, reinterpret_cast<i4_t *>(&met[turn].next)[1] = y;
+                break;
             }
         }
-        if (it.n < 0) return;
+        if (rank >= n_items && lane == 0) met[turn].next.n = -1, met[turn].next.j = 0;
+        __syncthreads();
+        done = it;
+        it = met[turn].next;
     }
 }
 
@@ -766,7 +778,7 @@ __global__ __launch_bounds__(kT) void k_verify_walk(const VerifyArgs a) {
     if (a.seq[s].done) return;
     const bool greedy = !(t > 0.0f);
     const double scale = greedy ? 1.0 : scale_of(t);
-    if (tid < 16) m.roots[tid] = kRoots[tid];
+    if (tid < 32) m.roots[tid] = kRoots[tid];
     for (bool alone = false;;) {
         int u;
         const int n = find_path(a, w, m, u), then = n ? __builtin_amdgcn_readfirstlane(m.next[u]) : (int) kOpen;
@@ -969,8 +981,8 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         if (n_rows == 0) return;
         a.each = draft_logits ? z.parts : 1;
         a.abreast = (int) std::min<int64_t>(n_rows, std::max(1, kRowGroups / z.parts));
-        const unsigned grid = paged_grid((int64_t) a.abreast * z.parts, kT);
-        k_verify_rows<<<grid, kT, 0, st>>>(a);
+        const unsigned grid = paged_grid((int64_t) a.abreast * z.parts, kT + 64);
+        k_verify_rows<<<grid, kT + 64, 0, st>>>(a);
         check_launch("draft verify rows");
         // A path that cannot be all of a sequence's rows tells that rows have several children, of which some will fall.
         const int walks = draft_logits && max_path < a.max_rows && z.parts > 4 ? 3 : 1;
