@@ -100,8 +100,9 @@ __global__ __launch_bounds__(256) void k_draft_tree(const TreeArgs a) {
 // in parts, a workgroup to a part: the largest and the sum of exponentials, of the target's and, where a row has children, the
 // drafter's. Whichever of a row's workgroups ends last has the row's softmax and decides which child stands, which depends on
 // nothing but the row. Rows that an earlier decision has cut off from the path are passed over if it is known by then: in this
-// order, where rows are many, it mostly is (nobody waits for it, and no result depends on it). k_verify_walk follows the
-// decisions from the root on and draws the last row's token. Where a drawn child fell it is drawn from what is left:
+// order, where rows are many, it mostly is (nobody waits for it, and no result depends on it). The decision that completes a path
+// from the root puts it out and leaves the last row to k_verify_draw, which draws its token. Where drawn children fell it is drawn
+// from what they left:
 //   r after k fallen drafts is w_k / c_k, w_k = max(p - C_k q, 0), c_k its sum, C_0 = 0 and C_k+1 = C_k + c_k, since
 //   max(max(a, 0) - b, 0) = max(a - b, 0) for b >= 0: one sum over the vocabulary for each that falls, made for the rows on the
 //   path alone.
@@ -117,7 +118,7 @@ constexpr int kRowGroups = 1024;         // workgroups at a time in k_verify_row
 constexpr float kHuge = 3.402823466e38f;
 
 // What became of a row: the child that stands (>= 0), or
-enum : int { kNone = -1, kOpen = -2, kFell = -16 };  // not known yet; kFell - j: child j fell, others are left, r's sum is not known
+enum : int { kNone = -1, kOpen = -2, kLeft = -3, kFell = -16 };  // not known yet; all drawn ones fell; kFell - j: child j fell, others are left
 
 struct __align__(16) RowState {
     double sum_p, sum_q, C;  // sums of exp((l - m) / t)
@@ -129,8 +130,10 @@ struct __align__(16) PartSums {
     float m_p, m_q;
     int top, pad;
 };
-struct SeqState {
-    int arrived, done;
+struct __align__(16) SeqState {  // a sequence whose path is known
+    int u, n, then, r0;            // the path's last row, its rows (0: not known, or ended), what became of it; the sequence's rows
+    int rows, arrived, listed;
+    float t;
 };
 struct __align__(16) Item {  // a row in its order
     int r, s, j, parent;  // parent < 0: none
@@ -144,10 +147,10 @@ struct VerifyArgs {
     const float * logits, * draft, * temperature, * coins;
     int64_t ld, draft_ld;
     int n_seq, n_rows, V, max_rows, max_path;
-    int parts, steps, abreast, each;  // parts of a row and a part's steps; rows abreast in k_verify_rows; workgroups to a sequence in k_verify_walk
-    bool vec, last;             // rows of whole 16-byte pieces; the last walk
+    int parts, steps, abreast, blocks, block_steps;  // parts of a row and a part's steps; rows abreast in k_verify_rows; parts of what is left
+    bool vec, last;                     // rows of whole 16-byte pieces; the last k_verify_draw
     int32_t * count, * rows, * out;
-    int * n_items;
+    int * n_items, * n_list, * list;  // the sequences that draw from what is left
     Item * items;
     RowState * state;
     int * next, * arrived;  // of the rows
@@ -325,13 +328,10 @@ __device__ __forceinline__ int child_after(const int32_t * parents, const Rows &
 // A wavefront to a row: its place in the order, and its state.
 __global__ __launch_bounds__(kT) void k_verify_begin(const VerifyArgs a) {
     const int lane = threadIdx.x & 63, r = blockIdx.x * (kT / 64) + (threadIdx.x >> 6);
-    for (int s = blockIdx.x * kT + threadIdx.x; s < a.n_seq; s += gridDim.x * kT) {
-        a.seq[s] = SeqState{};
-        const Rows w = rows_of(a.starts, s, a.n_rows, a.max_rows);
-        if (w.n) continue;
-        a.count[s] = 0, a.seq[s].done = 1;
-        for (int i = 0; i < a.max_path; i++) a.rows[(int64_t) s * a.max_path + i] = a.out[(int64_t) s * a.max_path + i] = -1;
-    }
+    const int id = blockIdx.x * kT + threadIdx.x, all_ids = gridDim.x * kT;
+    if (id == 0) *a.n_list = 0;
+    for (int s = id; s < a.n_seq; s += all_ids) a.seq[s] = SeqState{}, a.count[s] = 0;
+    for (int64_t i = id; i < (int64_t) a.n_seq * a.max_path; i += all_ids) a.rows[i] = a.out[i] = -1;
     if (r >= a.n_rows) return;
     if (lane == 0) a.next[r] = kOpen, a.arrived[r] = 0;
     const auto load = [&](int s0) { return s0 + lane < a.n_seq ? rows_of(a.starts, s0 + lane, a.n_rows, a.max_rows) : Rows{}; };
@@ -410,7 +410,7 @@ __device__ __forceinline__ int decide(const VerifyArgs & a, const Rows & w, int 
             if ((double) readlane_f(k.coin, l) * c * ql < v) return j0 + l;
             if (a.draft) {
                 C += c;
-                return at & (at - 1) || child_after(a.parents, w, u, j0 + 63) < w.n ? kFell - (j0 + l) : (int) kNone;
+                return at & (at - 1) || child_after(a.parents, w, u, j0 + 63) < w.n ? kFell - (j0 + l) : (int) kLeft;
             }
             c -= v;
         }
@@ -419,29 +419,44 @@ __device__ __forceinline__ int decide(const VerifyArgs & a, const Rows & w, int 
     }
 }
 
-// What a workgroup keeps in LDS of the path and of a draw.
-struct PathLds {
+// What a workgroup keeps in LDS for a draw.
+struct DrawLds {
     double roots[32], seg[4 * kSteps];  // sums of a part's runs of 256 tokens
-    int next[kMaxRows], path[kMaxRows];
     uint32_t gone[kSteps * kStep / 32];
     int flag, said;
 };
 
-// The path from the root as far as it is known: the number of its rows and the last one.
-__device__ __forceinline__ int find_path(const VerifyArgs & a, const Rows & w, PathLds & m, int & last) {
-    for (int j = threadIdx.x; j < w.n; j += kT) m.next[j] = agent_load(&a.next[w.r0 + j]);
-    __syncthreads();
-    int n = 0;
-    last = 0;
-    for (int u = 0; w.n > 0 && n < a.max_path;) {
-        if (threadIdx.x == 0) m.path[n] = u;
-        n++;
-        last = u;
-        const int v = __builtin_amdgcn_readfirstlane(m.next[u]);
-        if (v <= u || v >= w.n) break;
-        u = v;
+// The path on from row u, its row n (a wavefront): its rows, the last one and what became of that; on: `row` is one of them. PUT: into the results.
+struct Path {
+    int n, u, then;
+    bool on;
+};
+template <bool PUT>
+__device__ __forceinline__ Path follow(const VerifyArgs & a, const Rows & w, int s, int n, int u, int row) {
+    const int lane = threadIdx.x & 63;
+    Path z{n, u, kOpen, false};
+    int at = -1, next = kOpen, mine = 0, first = n;
+    const auto put = [&] {  // rows first .. n - 1, and that each follows the one before
+        const int i = first + lane;
+        if (!PUT || i >= z.n) return;
+        a.rows[(int64_t) s * a.max_path + i] = mine;
+        if (i) a.out[(int64_t) s * a.max_path + i - 1] = a.tokens[w.r0 + mine];
+    };
+    for (;;) {
+        if (lane == z.n - first) mine = z.u;
+        z.on = z.on || z.u == row;
+        z.n++;
+        if (PUT && z.n - first == 64) put(), first = z.n;
+        if (z.u >> 6 != at) {
+            at = z.u >> 6;
+            next = agent_load(&a.next[w.r0 + min(64 * at + lane, w.n - 1)]);
+        }
+        z.then = __builtin_amdgcn_readlane(next, z.u & 63);
+        if (z.then <= z.u || z.then >= w.n || z.n >= a.max_path) break;
+        z.u = z.then;
     }
-    return n;
+    put();
+    return z;
 }
 
 // A lane's value and those of the lanes before.
@@ -462,13 +477,15 @@ struct Source {
     Soft p, q;
     float p_low, q_low;  // Range's
     bool odd;
+    int parts, steps;
 };
-__device__ __forceinline__ Source source(const Rows & w, int s, int u, const RowState & st, const double * roots, double scale) {
+__device__ __forceinline__ Source source(const VerifyArgs & a, const Rows & w, int s, int u, const RowState & st, const double * roots, double scale) {
     const Range p = range_of(st.m_p, scale), q = st.C > 0.0 ? range_of(st.m_q, scale) : p;
-    return {w, s, u, st.C, soft(roots, scale, st.m_p, st.sum_p), soft(roots, scale, st.m_q, st.sum_q), p.low, q.low, !(p.high > -INFINITY && q.high > -INFINITY)};
+    return {w, s, u, st.C, soft(roots, scale, st.m_p, st.sum_p), soft(roots, scale, st.m_q, st.sum_q), p.low, q.low, !(p.high > -INFINITY && q.high > -INFINITY),
+            st.C > 0.0 ? a.blocks : a.parts, st.C > 0.0 ? a.block_steps : a.steps};
 }
 // The weights of the tokens whose logits are l (the drafter's d), from token i of a part on, of r or (all) of p.
-__device__ __forceinline__ void weights4(const VerifyArgs & a, const Source & z, const PathLds & m, int i, bool all, const float (&l)[4], const float (&d)[4], double (&v)[4]) {
+__device__ __forceinline__ void weights4(const VerifyArgs & a, const Source & z, const DrawLds & m, int i, bool all, const float (&l)[4], const float (&d)[4], double (&v)[4]) {
     const bool fell = z.C > 0.0 && !all;
     double q[4];
     if (z.odd) {
@@ -490,13 +507,13 @@ __device__ __forceinline__ void weights4(const VerifyArgs & a, const Source & z,
     }
 }
 __device__ __forceinline__ void logits4(const VerifyArgs & a, const Source & z, int part, int i, bool all, float (&l)[4], float (&d)[4]) {
-    const int at = part * a.steps * kStep + i;
+    const int at = part * z.steps * kStep + i;
     const bool whole = a.vec && at + 3 < a.V;
     values4(a.logits + (z.w.r0 + z.u) * a.ld, at, a.V, whole, l);
     if (z.C > 0.0 && !all) values4(a.draft + (z.w.r0 + z.u) * a.draft_ld, at, a.V, whole, d);
 }
 // The sums of a part's runs of 256 tokens, and of the part (all threads).
-__device__ __forceinline__ double runs(const VerifyArgs & a, const Source & z, PathLds & m, int part, bool all) {
+__device__ __forceinline__ double runs(const VerifyArgs & a, const Source & z, DrawLds & m, int part, bool all) {
     const int tid = threadIdx.x;
     __syncthreads();
     if (!a.draft && !all) {
@@ -504,16 +521,16 @@ __device__ __forceinline__ double runs(const VerifyArgs & a, const Source & z, P
         __syncthreads();
         for (int j = z.u + 1 + tid; j < z.w.n; j += kT)
             if (a.parents[z.w.r0 + j] == z.u) {
-                const unsigned e = (unsigned) a.tokens[z.w.r0 + j] - (unsigned) (part * a.steps * kStep);
-                if (e < (unsigned) (a.steps * kStep)) atomicOr(&m.gone[e / 32], 1u << (e % 32));
+                const unsigned e = (unsigned) a.tokens[z.w.r0 + j] - (unsigned) (part * z.steps * kStep);
+                if (e < (unsigned) (z.steps * kStep)) atomicOr(&m.gone[e / 32], 1u << (e % 32));
             }
         __syncthreads();
     }
     float l[4], d[4], l1[4], d1[4];
     logits4(a, z, part, 4 * tid, all, l, d);
 #pragma unroll 1
-    for (int k = 0; k < a.steps; k++) {
-        if (k + 1 < a.steps) logits4(a, z, part, (k + 1) * kStep + 4 * tid, all, l1, d1);
+    for (int k = 0; k < z.steps; k++) {
+        if (k + 1 < z.steps) logits4(a, z, part, (k + 1) * kStep + 4 * tid, all, l1, d1);
         double v[4];
         weights4(a, z, m, k * kStep + 4 * tid, all, l, d, v);
 #pragma unroll
@@ -522,17 +539,19 @@ __device__ __forceinline__ double runs(const VerifyArgs & a, const Source & z, P
         if ((tid & 63) == 0) m.seg[4 * k + (tid >> 6)] = sum;
     }
     __syncthreads();
-    return wave_sum_d((tid & 63) < 4 * a.steps ? m.seg[tid & 63] : 0.0);
+    return wave_sum_d((tid & 63) < 4 * z.steps ? m.seg[tid & 63] : 0.0);
 }
 static_assert(kSteps * kStep / 32 == kT && 4 * kSteps <= 64, "a word of gone to a thread, a run to a lane");
 
-// The sum of a lane's part, of those from i0 on: what fell of drawn ones was summed for this draw, others are k_verify_rows's, less what fell.
-__device__ __forceinline__ double part_sum(const VerifyArgs & a, const Source & z, int i0, bool all) {
+// The sum of a lane's part, of those from i0 on: what fell of drawn ones was summed for this draw, others are k_verify_rows's (the first 64
+// of them `early`), less what fell.
+__device__ __forceinline__ double part_sum(const VerifyArgs & a, const Source & z, int i0, bool all, const PartSums & early) {
     const int lane = threadIdx.x & 63, part = i0 + lane;
-    if (z.C > 0.0 && !all) return part < a.parts ? shared(a.drawn + (int64_t) z.s * a.parts + part) : 0.0;
+    if (z.C > 0.0 && !all) return part < z.parts ? shared(a.drawn + (int64_t) z.s * z.parts + part) : 0.0;
     double v = 0.0;
-    if (part < a.parts) {
-        const PartSums x = shared(a.sums + (int64_t) (z.w.r0 + z.u) * a.parts + part);
+    if (part < z.parts) {
+        PartSums x = early;
+        if (i0) x = a.sums[(int64_t) (z.w.r0 + z.u) * z.parts + part];
         v = x.p * z.p.p(x.m_p);
     }
     if (all || a.draft) return v;
@@ -541,82 +560,70 @@ __device__ __forceinline__ double part_sum(const VerifyArgs & a, const Source & 
         const double pt = z.p.p(k.x);
         for (uint64_t at = k.at; at; at &= at - 1) {
             const int l = __builtin_ctzll(at), token = __builtin_amdgcn_readlane(k.token, l);
-            if (token >= 0 && token / (a.steps * kStep) == part && !again(a, z.w, z.u, k, j0, l, token)) v -= readlane_d(pt, l);
+            if (token >= 0 && token / (z.steps * kStep) == part && !again(a, z.w, z.u, k, j0, l, token)) v -= readlane_d(pt, l);
         }
     }
     return fmax(v, 0.0);
 }
 constexpr double kNothing = 0x1p-900;  // no token's weight
-// Of 64 lanes' values, the one where the sum passes `want`, the last above nothing if rounding leaves none, -1 if all are 0; below grows by those before
+// Of 64 lanes' values d, their sums up to each one `sum`: the one where it passes `want`, the last above nothing if rounding leaves none, -1 if all are 0; below grows by those before
 // it, or by all.
-__device__ __forceinline__ int pass(double d, double want, double & below, bool & hit) {
-    const double sum = upto(d);
+__device__ __forceinline__ int pass(double d, double sum, double want, double & below, bool & hit) {
     const uint64_t some = __ballot(d > kNothing), at = __ballot(d > kNothing && below + sum > want);
     hit = at != 0;
     const int l = hit ? __builtin_ctzll(at) : some ? 63 - __builtin_clzll(some) : -1;
     below += hit ? (l ? readlane_d(sum, l - 1) : 0.0) : readlane_d(sum, 63);
     return l;
 }
-// The token where the cumulative sum passes the coin's share of it: the part, the run, the lane, the token. From p if r has nothing.
-__device__ __forceinline__ int draw(const VerifyArgs & a, const Source & z, PathLds & m) {
+// The token where the cumulative sum passes the coin's share of it: the part, the run, the lane, the token; -1 if there is no sum. all: of p, whatever fell.
+__device__ __forceinline__ int draw(const VerifyArgs & a, const Source & z, DrawLds & m, bool all, const PartSums & early) {
     const int lane = threadIdx.x & 63;
     const float coin = a.coins[z.w.r0];
-    const double portion = coin > 0.0f ? fmin((double) coin, 1.0 - 0x1p-24) : 0.0;
+    double d = 0.0, sum = 0.0, want = INFINITY, base = 0.0, rest = 0.0;
+    int part = -1;
+    bool hit = false;
 #pragma unroll 1
-    for (int all = 0; all < 2; all++) {
-        double first = 0.0, want = INFINITY, base = 0.0, rest = 0.0;
-        int part = -1;
-        bool hit = false;
-#pragma unroll 1
-        for (int find = 0; find < 2; find++) {  // the total, then the part
-            double below = 0.0;
-            for (int i0 = 0; i0 < a.parts && !hit; i0 += 64) {
-                const double d = find && i0 == 0 ? first : part_sum(a, z, i0, all), before = below;
-                if (i0 == 0) first = d;
-                const int l = pass(d, want, below, hit);
-                if (find && l >= 0) part = i0 + l, base = hit ? below : before, rest = hit ? want : INFINITY;
-            }
-            want = portion * below;
+    for (int find = 0; find < 2; find++) {  // the total, then the part
+        double below = 0.0;
+        for (int i0 = 0; i0 < z.parts && !hit; i0 += 64) {
+            const double before = below;
+            if (!find || z.parts > 64) d = part_sum(a, z, i0, all, early), sum = upto(d);
+            const int l = pass(d, sum, want, below, hit);
+            if (find && l >= 0) part = i0 + l, base = hit ? below : before, rest = hit ? want : INFINITY;
         }
-        if (part < 0) continue;
-        want = rest;  // (no part passes it, by rounding: the last token of the last)
-        runs(a, z, m, part, all);
-        if (threadIdx.x < 64) {
-            const int run = pass(lane < 4 * a.steps ? m.seg[lane] : 0.0, want, base, hit);
-            int token = -1;
-            if (run >= 0) {
+        want = (coin > 0.0f ? fmin((double) coin, 1.0 - 0x1p-24) : 0.0) * below;
+    }
+    if (part < 0) return -1;
+    want = rest;  // (no part passes it, by rounding: the last token of the last)
+    runs(a, z, m, part, all);
+    if (threadIdx.x < 64) {
+        d = lane < 4 * z.steps ? m.seg[lane] : 0.0;
+        const int run = pass(d, upto(d), want, base, hit);
+        int token = -1;
+        if (run >= 0) {
+            if (!hit) want = INFINITY;
+            float x[4], y[4];
+            double v[4];
+            logits4(a, z, part, run * 256 + 4 * lane, all, x, y);
+            weights4(a, z, m, run * 256 + 4 * lane, all, x, y, v);
+            d = (v[0] + v[1]) + (v[2] + v[3]);
+            const int who = pass(d, upto(d), want, base, hit);
+            if (who >= 0) {
                 if (!hit) want = INFINITY;
-                float l[4], d[4];
-                double v[4];
-                logits4(a, z, part, run * 256 + 4 * lane, all, l, d);
-                weights4(a, z, m, run * 256 + 4 * lane, all, l, d, v);
-                const int who = pass((v[0] + v[1]) + (v[2] + v[3]), want, base, hit);
-                if (who >= 0) {
-                    if (!hit) want = INFINITY;
-                    int e = -1;
+                int e = -1;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const double x = readlane_d(v[i], who);
-                        if (x > kNothing && (e < 0 || !(base > want))) e = i;
-                        base += x;
-                    }
-                    token = part * a.steps * kStep + run * 256 + 4 * who + e;
+                for (int i = 0; i < 4; i++) {
+                    const double x = readlane_d(v[i], who);
+                    if (x > kNothing && (e < 0 || !(base > want))) e = i;
+                    base += x;
                 }
+                token = part * z.steps * kStep + run * 256 + 4 * who + e;
             }
-            if (lane == 0) m.said = token;
         }
-        __syncthreads();
-        if (m.said >= 0) return m.said;
+        if (lane == 0) m.said = token;
     }
-    return -1;
-}
-__device__ __forceinline__ void put_path(const VerifyArgs & a, const Rows & w, int s, int n, int token, const PathLds & m) {
-    int32_t * const rows = a.rows + (int64_t) s * a.max_path, * const out = a.out + (int64_t) s * a.max_path;
-    for (int i = threadIdx.x; i < a.max_path; i += kT) {
-        rows[i] = i < n ? m.path[i] : -1;
-        out[i] = i + 1 < n ? a.tokens[w.r0 + m.path[i + 1]] : i < n ? token : -1;
-    }
-    if (threadIdx.x == 0) a.count[s] = n, a.seq[s].done = 1;
+    __syncthreads();
+    return m.said;
 }
 
 // A workgroup has one part of every abreast-th row: those in work at a time are the next of the order that are not cut off. Four wavefronts
@@ -731,9 +738,21 @@ __global__ __launch_bounds__(kT + 64, 5) void k_verify_rows(const VerifyArgs a) 
             if (p.m > -INFINITY && done.child < done.n)
                 next = decide(a, w, done.j, done.j, greedy ? top : -1, 1.0, soft(roots, scale, p.m, p.s), soft(roots, scale, q.m, q.s), kids, done.j + 1, C);
             if (lane == 0) {
-                agent_store(&a.next[done.r], next);
                 a.state[done.r] = RowState{p.s, q.s, C, p.m, q.m, top, 0};
+                agent_store(&a.next[done.r], next);
+                stores_done();
             }
+            // Whoever decides a path's last row to be decided sees the others' decisions, its own being known before they are looked at.
+            const Path path = follow<false>(a, w, done.s, 0, 0, done.j);
+            if (!path.on || path.then == kOpen || (path.then >= 0 && path.n < a.max_path)) return;
+            follow<true>(a, w, done.s, 0, 0, done.j);
+            if (lane) return;
+            SeqState & seq = a.seq[done.s];  // (two at once write the same)
+            a.count[done.s] = path.n;
+            if (path.then >= 0) a.out[(int64_t) done.s * a.max_path + path.n - 1] = a.tokens[w.r0 + path.then];  // (cut short)
+            else seq.u = path.u, seq.n = path.n, seq.then = path.then, seq.r0 = w.r0, seq.rows = w.n, seq.t = done.t;
+            if (path.then < kOpen && __hip_atomic_exchange(&seq.listed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0)
+                a.list[__hip_atomic_fetch_add(a.n_list, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)] = done.s;
         };
         if (done.n > 0) end();
         if (!good(it)) return;
@@ -768,65 +787,90 @@ __global__ __launch_bounds__(kT + 64, 5) void k_verify_rows(const VerifyArgs a) 
     }
 }
 
-// The walk of one sequence. Where a drawn child of its last row fell each workgroup sums a part of r, for the draw or for the next child, and
-// the last to end goes on, in the last launch alone to the end; else the parts' sums are k_verify_rows's, and workgroup 0 draws.
-__global__ __launch_bounds__(kT) void k_verify_walk(const VerifyArgs a) {
-    __shared__ PathLds m;
-    const int tid = threadIdx.x, wave = tid >> 6, s = blockIdx.x / a.each, own = blockIdx.x % a.each;
-    const Rows w = rows_of(a.starts, s, a.n_rows, a.max_rows);
-    const float t = a.temperature ? a.temperature[s] : 1.0f;
-    if (a.seq[s].done) return;
-    const bool greedy = !(t > 0.0f);
-    const double scale = greedy ? 1.0 : scale_of(t);
+// The last rows' tokens: of p by workgroup s, from k_verify_rows's sums; of what drawn children left a workgroup a part, which it sums, for the
+// draw or for the next child: the last of the sequence's to end goes on, in the last launch alone to the path's end.
+__global__ __launch_bounds__(kT) void k_verify_draw(const VerifyArgs a) {
+    __shared__ DrawLds m;
+    __shared__ Path path;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (tid < 32) m.roots[tid] = kRoots[tid];
-    for (bool alone = false;;) {
-        int u;
-        const int n = find_path(a, w, m, u), then = n ? __builtin_amdgcn_readfirstlane(m.next[u]) : (int) kOpen;
-        const RowState st = n ? shared(a.state + w.r0 + u) : RowState{};
-        const Source z = source(w, s, u, st, m.roots, scale);
-        if (n && !greedy && st.C > 0.0 && (then == kNone || then <= kFell)) {
+    const bool of_p = (int) blockIdx.x < a.n_seq;
+    const int units = of_p ? a.n_seq : min(*a.n_list, a.n_seq) * a.blocks;
+    for (int unit = of_p ? blockIdx.x : blockIdx.x - a.n_seq; unit < units; unit += of_p ? a.n_seq : gridDim.x - a.n_seq) {
+        const int s = of_p ? unit : a.list[unit / a.blocks], own = unit % a.blocks;
+        if ((unsigned) s >= (unsigned) a.n_seq) return;
+        const SeqState & q = a.seq[s];
+        const Rows w{q.r0, q.rows};
+        const float t = q.t;
+        int u = q.u, n = q.n, then = q.then;
+        const bool greedy = !(t > 0.0f);
+        const double scale = greedy ? 1.0 : scale_of(t);
+        if (n <= 0 || n > a.max_path || (then == kNone) != of_p) continue;
+        if (u < 0 || u >= w.n || w.r0 < 0 || w.r0 > a.n_rows - w.n) return;
+        for (bool alone = false;;) {
+            PartSums early{0.0, 0.0, -INFINITY, -INFINITY, 0, 0};
+            if (then == kNone && lane < a.parts) early = a.sums[(int64_t) (w.r0 + u) * a.parts + lane];
+            const RowState st = shared(a.state + w.r0 + u);
+            const Source z = source(a, w, s, u, st, m.roots, scale);
+            if (then == kLeft || then <= kFell) {
 #pragma unroll 1
-            for (int b = alone ? 0 : own; b < (alone ? a.parts : own + 1); b++) {
-                const double v = runs(a, z, m, b, false);
-                if (tid == 0) share(a.drawn + (int64_t) s * a.parts + b, v);
+                for (int b = alone ? 0 : own; b < (alone ? a.blocks : own + 1); b++) {
+                    const double v = runs(a, z, m, b, false);
+                    if (tid == 0) share(a.drawn + (int64_t) s * a.blocks + b, v);
+                }
+                if (alone) {
+                    if (tid == 0) stores_done();
+                    __syncthreads();
+                } else if (!last_of(&a.seq[s].arrived, a.blocks, &m.flag)) break;
             }
-            if (alone) {
-                if (tid == 0) stores_done();
-                __syncthreads();
-            } else if (!last_of(&a.seq[s].arrived, a.parts, &m.flag)) return;
             if (then <= kFell) {
                 if (wave == 0) {
                     double C = st.C, c = 0.0;
-                    for (int i0 = 0; i0 < a.parts; i0 += 64) c += wave_sum_d(part_sum(a, z, i0, false));
-                    const int from = kFell - then, next = decide(a, w, u, from, -1, c, z.p, z.q, children(a, w, u, from + 1), from + 1, C);
+                    for (int i0 = 0; i0 < a.blocks; i0 += 64) c += wave_sum_d(part_sum(a, z, i0, false, early));
+                    const int from = kFell - then;
+                    Path on{n, u, decide(a, w, u, from, -1, c, z.p, z.q, children(a, w, u, from + 1), from + 1, C), true};
                     if (tid == 0) {
                         agent_store(&a.state[w.r0 + u].C, C);
-                        agent_store(&a.next[w.r0 + u], next);
+                        agent_store(&a.next[w.r0 + u], on.then);
                         stores_done();
                     }
-                }
-                if (!a.last) {
-                    if (tid == 0) a.seq[s].arrived = 0;
-                    return;
+                    if (on.then >= 0 && n < a.max_path) on = follow<true>(a, w, s, n, on.then, 0);
+                    if (tid == 0) {
+                        path = on;
+                        a.count[s] = on.n;
+                        a.seq[s].u = on.u, a.seq[s].n = on.then >= 0 ? 0 : on.n, a.seq[s].then = on.then, a.seq[s].arrived = 0;
+                        if (on.then >= 0 && on.then < w.n) a.out[(int64_t) s * a.max_path + on.n - 1] = a.tokens[w.r0 + on.then];  // (cut short)
+                    }
                 }
                 __syncthreads();
+                u = path.u, n = path.n, then = path.then;
+                if (then >= 0 || (then != kNone && !a.last)) break;
                 alone = true;
+                __syncthreads();
                 continue;
             }
-        } else if (own && !alone) return;
-        int token = -1;
-        if (n && then >= 0 && then < w.n) token = a.tokens[w.r0 + then];  // (a path cut short)
-        else if (n && then == kNone && st.m_p > -INFINITY) token = greedy ? st.top : draw(a, z, m);
+            int token = -1;
+            if (st.m_p > -INFINITY) {
+                token = greedy ? st.top : draw(a, z, m, false, early);
+                if (token < 0) {  // (nothing is left, by rounding)
+                    RowState all = st;
+                    all.C = 0.0;
+                    if (lane < a.parts) early = a.sums[(int64_t) (w.r0 + u) * a.parts + lane];
+                    token = draw(a, source(a, w, s, u, all, m.roots, scale), m, true, early);
+                }
+            }
+            if (tid == 0) a.out[(int64_t) s * a.max_path + n - 1] = token, a.seq[s].n = 0;
+            break;
+        }
         __syncthreads();
-        put_path(a, w, s, n, token, m);
-        return;
     }
 }
 
 // How a call is cut, and its workspace.
 struct VerifyShape {
     int steps, parts;
-    size_t items, state, next, arrived, sums, seq, drawn, total;  // offsets
+    int blocks, block_steps;
+    size_t items, state, next, arrived, sums, seq, list, drawn, total;  // offsets
 };
 VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     VerifyShape z{};
@@ -839,8 +883,12 @@ VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     z.arrived = z.next + align256((size_t) n_rows * sizeof(int));
     z.sums = z.arrived + align256((size_t) n_rows * sizeof(int));
     z.seq = z.sums + align256((size_t) n_rows * z.parts * sizeof(PartSums));
-    z.drawn = z.seq + align256((size_t) n_seq * sizeof(SeqState));
-    z.total = z.drawn + align256((size_t) n_seq * z.parts * sizeof(double));
+    z.block_steps = 2;  // (half of the sequences may have something left)
+    while (z.block_steps < kSteps && n_seq * ((V + z.block_steps * kStep - 1) / (z.block_steps * kStep)) > 2 * kRowGroups) z.block_steps *= 2;
+    z.blocks = (int) ((V + z.block_steps * kStep - 1) / (z.block_steps * kStep));
+    z.list = z.seq + align256((size_t) n_seq * sizeof(SeqState));
+    z.drawn = z.list + align256((size_t) n_seq * sizeof(int));
+    z.total = z.drawn + align256((size_t) n_seq * z.blocks * sizeof(double));
     return z;
 }
 
@@ -973,23 +1021,24 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         a.parts = z.parts, a.steps = z.steps;
         a.vec = aligned(logits, 16) && ld % 4 == 0 && (!draft_logits || (aligned(draft_logits, 16) && draft_ld % 4 == 0));
         a.count = count, a.rows = rows, a.out = tokens_out;
-        a.n_items = (int *) at, a.items = (Item *) (at + z.items), a.state = (RowState *) (at + z.state), a.next = (int *) (at + z.next);
-        a.arrived = (int *) (at + z.arrived), a.sums = (PartSums *) (at + z.sums), a.seq = (SeqState *) (at + z.seq), a.drawn = (double *) (at + z.drawn);
+        a.n_items = (int *) at, a.n_list = a.n_items + 1, a.items = (Item *) (at + z.items), a.state = (RowState *) (at + z.state);
+        a.next = (int *) (at + z.next), a.arrived = (int *) (at + z.arrived), a.sums = (PartSums *) (at + z.sums), a.seq = (SeqState *) (at + z.seq);
+        a.list = (int *) (at + z.list), a.drawn = (double *) (at + z.drawn);
         hipStream_t st = as_stream(stream);
         k_verify_begin<<<paged_grid(std::max<int64_t>((n_rows + 3) / 4, 1), kT), kT, 0, st>>>(a);
         check_launch("draft verify");
         if (n_rows == 0) return;
-        a.each = draft_logits ? z.parts : 1;
+        a.blocks = z.blocks, a.block_steps = z.block_steps;
         a.abreast = (int) std::min<int64_t>(n_rows, std::max(1, kRowGroups / z.parts));
-        const unsigned grid = paged_grid((int64_t) a.abreast * z.parts, kT + 64);
-        k_verify_rows<<<grid, kT + 64, 0, st>>>(a);
+        k_verify_rows<<<paged_grid((int64_t) a.abreast * z.parts, kT + 64), kT + 64, 0, st>>>(a);
         check_launch("draft verify rows");
         // A path that cannot be all of a sequence's rows tells that rows have several children, of which some will fall.
-        const int walks = draft_logits && max_path < a.max_rows && z.parts > 4 ? 3 : 1;
-        for (int i = 0; i < walks; i++) {
-            a.last = i == walks - 1;
-            k_verify_walk<<<paged_grid((int64_t) n_seq * a.each, kT), kT, 0, st>>>(a);
-            check_launch("draft verify walk");
+        const int draws = draft_logits && max_path < a.max_rows && z.blocks > 8 ? 3 : 1;
+        for (int i = 0; i < draws; i++) {
+            a.last = i == draws - 1;
+            const int64_t groups = n_seq + (draft_logits ? std::min<int64_t>((int64_t) n_seq * z.blocks, 2 * kRowGroups) : 0);
+            k_verify_draw<<<paged_grid(groups, kT), kT, 0, st>>>(a);
+            check_launch("draft verify draw");
         }
     });
 }
