@@ -113,7 +113,8 @@ __global__ __launch_bounds__(256) void k_draft_tree(const TreeArgs a) {
 typedef int i4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kT = 256, kStep = 4 * kT;  // threads, logits of a workgroup at a time
-constexpr int kSteps = 8;                // .. of a part at most
+constexpr int kSteps = 16;               // .. of a part at most
+constexpr int kDrawT = 512;              // threads of k_verify_draw
 constexpr int kRowGroups = 1024;         // workgroups at a time in k_verify_rows
 constexpr float kHuge = 3.402823466e38f;
 
@@ -261,7 +262,8 @@ struct Running {
         }
         double v[4];
         weigh4(roots, scale, m > -INFINITY ? (double) m : 0.0, in.low, l, v);
-        s += (v[0] + v[1]) + (v[2] + v[3]);
+        const double more = (v[0] + v[1]) + (v[2] + v[3]);
+        s += top > -INFINITY ? more : 0.0;  // (there may be no m yet, or no short form)
     }
     __device__ __forceinline__ void wave(const double * roots, double scale) {
         const float top = wave_max(m);
@@ -517,9 +519,9 @@ __device__ __forceinline__ double runs(const VerifyArgs & a, const Source & z, D
     const int tid = threadIdx.x;
     __syncthreads();
     if (!a.draft && !all) {
-        m.gone[tid] = 0;
+        for (int i = tid; i < kSteps * kStep / 32; i += kDrawT) m.gone[i] = 0;
         __syncthreads();
-        for (int j = z.u + 1 + tid; j < z.w.n; j += kT)
+        for (int j = z.u + 1 + tid; j < z.w.n; j += kDrawT)
             if (a.parents[z.w.r0 + j] == z.u) {
                 const unsigned e = (unsigned) a.tokens[z.w.r0 + j] - (unsigned) (part * z.steps * kStep);
                 if (e < (unsigned) (z.steps * kStep)) atomicOr(&m.gone[e / 32], 1u << (e % 32));
@@ -529,19 +531,19 @@ __device__ __forceinline__ double runs(const VerifyArgs & a, const Source & z, D
     float l[4], d[4], l1[4], d1[4];
     logits4(a, z, part, 4 * tid, all, l, d);
 #pragma unroll 1
-    for (int k = 0; k < z.steps; k++) {
-        if (k + 1 < z.steps) logits4(a, z, part, (k + 1) * kStep + 4 * tid, all, l1, d1);
+    for (int i = 4 * tid; i < z.steps * kStep; i += 4 * kDrawT) {
+        if (i + 4 * kDrawT < z.steps * kStep) logits4(a, z, part, i + 4 * kDrawT, all, l1, d1);
         double v[4];
-        weights4(a, z, m, k * kStep + 4 * tid, all, l, d, v);
+        weights4(a, z, m, i, all, l, d, v);
 #pragma unroll
         for (int e = 0; e < 4; e++) l[e] = l1[e], d[e] = d1[e];
         const double sum = wave_sum_d((v[0] + v[1]) + (v[2] + v[3]));
-        if ((tid & 63) == 0) m.seg[4 * k + (tid >> 6)] = sum;
+        if ((tid & 63) == 0) m.seg[i / 256] = sum;
     }
     __syncthreads();
     return wave_sum_d((tid & 63) < 4 * z.steps ? m.seg[tid & 63] : 0.0);
 }
-static_assert(kSteps * kStep / 32 == kT && 4 * kSteps <= 64, "a word of gone to a thread, a run to a lane");
+static_assert(4 * kSteps <= 64 && kStep % (4 * 64) == 0, "a run to a lane, whole runs");
 
 // The sum of a lane's part, of those from i0 on: what fell of drawn ones was summed for this draw, others are k_verify_rows's (the first 64
 // of them `early`), less what fell.
@@ -560,7 +562,8 @@ __device__ __forceinline__ double part_sum(const VerifyArgs & a, const Source & 
         const double pt = z.p.p(k.x);
         for (uint64_t at = k.at; at; at &= at - 1) {
             const int l = __builtin_ctzll(at), token = __builtin_amdgcn_readlane(k.token, l);
-            if (token >= 0 && token / (z.steps * kStep) == part && !again(a, z.w, z.u, k, j0, l, token)) v -= readlane_d(pt, l);
+            const bool first = !again(a, z.w, z.u, k, j0, l, token);  // (all lanes)
+            if (first && token >= 0 && token / (z.steps * kStep) == part) v -= readlane_d(pt, l);
         }
     }
     return fmax(v, 0.0);
@@ -789,7 +792,7 @@ __global__ __launch_bounds__(kT + 64, 5) void k_verify_rows(const VerifyArgs a) 
 
 // The last rows' tokens: of p by workgroup s, from k_verify_rows's sums; of what drawn children left a workgroup a part, which it sums, for the
 // draw or for the next child: the last of the sequence's to end goes on, in the last launch alone to the path's end.
-__global__ __launch_bounds__(kT) void k_verify_draw(const VerifyArgs a) {
+__global__ __launch_bounds__(kDrawT) void k_verify_draw(const VerifyArgs a) {
     __shared__ DrawLds m;
     __shared__ Path path;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -874,9 +877,16 @@ struct VerifyShape {
 };
 VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     VerifyShape z{};
-    z.steps = 2;
-    while (z.steps < kSteps && n_rows * ((V + z.steps * kStep - 1) / (z.steps * kStep)) > kRowGroups) z.steps *= 2;
-    z.parts = (int) ((V + z.steps * kStep - 1) / (z.steps * kStep));
+    const auto parts = [&](int steps) { return (V + steps * kStep - 1) / (steps * kStep); };
+    // A part costs its steps and some four more; workgroups take theirs in as many turns. Parts of up to 16 steps where that is
+    // two turns for all rows, of up to 8 where there are more, so that decisions come early enough to spare rows. (205 rows of 64
+    // chains of 128256 tokens: 77 us with up to 16 steps, 87 with 8; 800 rows of 16 trees: 68 and 56.)
+    int64_t best = INT64_MAX;
+    for (int k = 2; k <= (n_rows * parts(kSteps) <= 2 * kRowGroups ? kSteps : kSteps / 2); k += 2) {
+        const int64_t cost = (n_rows * parts(k) + kRowGroups - 1) / kRowGroups * (k + 4);
+        if (cost < best) best = cost, z.steps = k;
+    }
+    z.parts = (int) parts(z.steps);
     z.items = 256;
     z.state = z.items + align256((size_t) n_rows * sizeof(Item));
     z.next = z.state + align256((size_t) n_rows * sizeof(RowState));
@@ -884,8 +894,8 @@ VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     z.sums = z.arrived + align256((size_t) n_rows * sizeof(int));
     z.seq = z.sums + align256((size_t) n_rows * z.parts * sizeof(PartSums));
     z.block_steps = 2;  // (half of the sequences may have something left)
-    while (z.block_steps < kSteps && n_seq * ((V + z.block_steps * kStep - 1) / (z.block_steps * kStep)) > 2 * kRowGroups) z.block_steps *= 2;
-    z.blocks = (int) ((V + z.block_steps * kStep - 1) / (z.block_steps * kStep));
+    while (z.block_steps < kSteps && n_seq * parts(z.block_steps) > 2 * kRowGroups) z.block_steps *= 2;
+    z.blocks = (int) parts(z.block_steps);
     z.list = z.seq + align256((size_t) n_seq * sizeof(SeqState));
     z.drawn = z.list + align256((size_t) n_seq * sizeof(int));
     z.total = z.drawn + align256((size_t) n_seq * z.blocks * sizeof(double));
@@ -947,7 +957,9 @@ size_t verify_workspace(int n_seq, int64_t n_rows, int64_t V, int64_t max_rows) 
     paged_require(n_rows >= 0 && n_rows < (1 << 30), "draft_verify: n_rows out of range");
     paged_require(V > 0 && V < (1 << 30), "draft_verify: n_vocab out of range");
     paged_require(max_rows > 0 && std::min(max_rows, n_rows) <= kMaxRows, "draft_verify: max_rows must be 1 .. 1024");
-    return verify_shape(n_seq, n_rows, V).total;
+    const VerifyShape z = verify_shape(n_seq, n_rows, V);
+    paged_require((int64_t) n_seq * z.blocks < (1 << 30) && n_rows * z.parts < ((int64_t) 1 << 40), "draft_verify: too many sequences and tokens");
+    return z.total;
 }
 
 }  // namespace
@@ -1037,7 +1049,7 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         for (int i = 0; i < draws; i++) {
             a.last = i == draws - 1;
             const int64_t groups = n_seq + (draft_logits ? std::min<int64_t>((int64_t) n_seq * z.blocks, 2 * kRowGroups) : 0);
-            k_verify_draw<<<paged_grid(groups, kT), kT, 0, st>>>(a);
+            k_verify_draw<<<paged_grid(groups, kDrawT), kDrawT, 0, st>>>(a);
             check_launch("draft verify draw");
         }
     });

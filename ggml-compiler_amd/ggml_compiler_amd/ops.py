@@ -414,11 +414,14 @@ def paged_attn(cache: PagedCache, batch: PagedBatch, q: torch.Tensor, scale: flo
     `window` of them if window > 0. q f16 [n, H, D] (strides multiples of 8, unit inner stride) -> f32 [n, H, D] (into
     out if given; rows of no sequence stay as they are; a row that sees no token gives zeros). max_rows: no sequence
     has more rows than this (default n); 1 for a decode step. tree: the rows are draft trees, each sees its sequence's past (of a window
-    the part that its position leaves) and those rows that the tree's mask names."""
+    the part that its position leaves) and those rows that the tree's mask names (max_rows then by default as many as it has
+    bits)."""
     d, (n, H) = _paged_device(cache, batch), _rows_heads(q)
     shape = (n, H, cache.D)
     qs = _paged_rows(q, torch.float16, "q", shape, d)
     out = _paged_out(out, shape, torch.float32, "out", q)
+    if max_rows is None and tree is not None:
+        max_rows = 32 * tree.mask.shape[1]
     max_rows = max(n, 1) if max_rows is None else min(max_rows, max(n, 1))
     if not 0 <= window < 1 << 31:
         raise ValueError(f"window {window} is not in 0 .. 2^31 - 1")
@@ -452,7 +455,7 @@ class DraftTree:
     mask: torch.Tensor
 
     def __post_init__(self) -> None:
-        n, d = self.parents.numel(), self.parents.get_device()
+        n, d = _cuda(self.parents, torch.int32, "parents").numel(), self.parents.get_device()
         _ints(self.parents, "parents", (n,), d)
         _ints(self.positions, "positions", (n,), d)
         words = self.mask.shape[-1]
