@@ -432,20 +432,25 @@ struct DrawLds {
 struct Path {
     int n, u, then;
     bool on;
+    int mine;  // a lane's of its last rows, those of one 64
 };
+// Rows first .. n - 1 of a path, a lane's each, and that each follows the one before.
+__device__ __forceinline__ void put_rows(const VerifyArgs & a, const Rows & w, int s, int first, int n, int row) {
+    const int i = first + (threadIdx.x & 63);
+    if (i >= n) return;
+    a.rows[(int64_t) s * a.max_path + i] = row;
+    if (i) a.out[(int64_t) s * a.max_path + i - 1] = a.tokens[w.r0 + row];
+}
 template <bool PUT>
 __device__ __forceinline__ Path follow(const VerifyArgs & a, const Rows & w, int s, int n, int u, int row) {
     const int lane = threadIdx.x & 63;
-    Path z{n, u, kOpen, false};
-    int at = -1, next = kOpen, mine = 0, first = n;
-    const auto put = [&] {  // rows first .. n - 1, and that each follows the one before
-        const int i = first + lane;
-        if (!PUT || i >= z.n) return;
-        a.rows[(int64_t) s * a.max_path + i] = mine;
-        if (i) a.out[(int64_t) s * a.max_path + i - 1] = a.tokens[w.r0 + mine];
+    Path z{n, u, kOpen, false, 0};
+    int at = -1, next = kOpen, first = n;
+    const auto put = [&] {
+        if (PUT) put_rows(a, w, s, first, z.n, z.mine);
     };
     for (;;) {
-        if (lane == z.n - first) mine = z.u;
+        if (lane == ((z.n - first) & 63)) z.mine = z.u;
         z.on = z.on || z.u == row;
         z.n++;
         if (PUT && z.n - first == 64) put(), first = z.n;
@@ -748,14 +753,16 @@ __global__ __launch_bounds__(kT + 64, 5) void k_verify_rows(const VerifyArgs a) 
             // Whoever decides a path's last row to be decided sees the others' decisions, its own being known before they are looked at.
             const Path path = follow<false>(a, w, done.s, 0, 0, done.j);
             if (!path.on || path.then == kOpen || (path.then >= 0 && path.n < a.max_path)) return;
-            follow<true>(a, w, done.s, 0, 0, done.j);
-            if (lane) return;
             SeqState & seq = a.seq[done.s];  // (two at once write the same)
+            int listed = 1;
+            if (path.then < kOpen && lane == 0) listed = __hip_atomic_exchange(&seq.listed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (path.n <= 64) put_rows(a, w, done.s, 0, path.n, path.mine);
+            else follow<true>(a, w, done.s, 0, 0, done.j);
+            if (lane) return;
             a.count[done.s] = path.n;
             if (path.then >= 0) a.out[(int64_t) done.s * a.max_path + path.n - 1] = a.tokens[w.r0 + path.then];  // (cut short)
             else seq.u = path.u, seq.n = path.n, seq.then = path.then, seq.r0 = w.r0, seq.rows = w.n, seq.t = done.t;
-            if (path.then < kOpen && __hip_atomic_exchange(&seq.listed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0)
-                a.list[__hip_atomic_fetch_add(a.n_list, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)] = done.s;
+            if (!listed) a.list[__hip_atomic_fetch_add(a.n_list, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)] = done.s;
         };
         if (done.n > 0) end();
         if (!good(it)) return;
@@ -831,7 +838,7 @@ __global__ __launch_bounds__(kDrawT) void k_verify_draw(const VerifyArgs a) {
                     double C = st.C, c = 0.0;
                     for (int i0 = 0; i0 < a.blocks; i0 += 64) c += wave_sum_d(part_sum(a, z, i0, false, early));
                     const int from = kFell - then;
-                    Path on{n, u, decide(a, w, u, from, -1, c, z.p, z.q, children(a, w, u, from + 1), from + 1, C), true};
+                    Path on{n, u, decide(a, w, u, from, -1, c, z.p, z.q, children(a, w, u, from + 1), from + 1, C), true, 0};
                     if (tid == 0) {
                         agent_store(&a.state[w.r0 + u].C, C);
                         agent_store(&a.next[w.r0 + u], on.then);

@@ -91,7 +91,9 @@ __device__ __forceinline__ int splits(int tiles, int chunk) { return max(1, (til
 // Items of split row tiles have a slot each for their sums. Those are fewer than 2 target: with u tiles in all items' and a chunk of more than
 // u / cut, a row tile has less than tiles cut / u splits more than one, all of them together less than cut <= target, and a split row tile has
 // at most twice as many splits as that.
-template <int ROWS>
+// FILL (trees): about the least chunk with which all items are resident at once: 61 rows over 65000 keys in 768 workgroups and not 704, 167 us
+// instead of 185; trees of 16 sequences 65 instead of 73. (Rows in lines keep the splits, and so the roundings, that they had.)
+template <int ROWS, bool FILL>
 struct Plan {
     const AttnArgs & a;
     SeqWork w;  // of sequence s0 + lane
@@ -111,7 +113,18 @@ struct Plan {
         u = wave_sum_d(u) * a.p.Hkv;
         n = wave_sum_d(n) * a.p.Hkv;
         const double cut = fmax(a.target - n, 0.5 * a.target);
-        chunk = __builtin_amdgcn_readfirstlane((int) fmax((double) a.min_chunk, fmin(u / cut + 1.0, 1e9)));
+        chunk = __builtin_amdgcn_readfirstlane((int) fmax((double) a.min_chunk, fmin(u / (FILL ? a.target : cut) + 1.0, 1e9)));
+        if (!FILL) return;
+        for (int turn = 0; turn < 8; turn++) {
+            int items = w.rts * splits(w.tiles, chunk);
+            for (int s0 = 64; s0 < a.p.n_seq; s0 += 64) {
+                const SeqWork x = seq_work<ROWS>(a, s0 + lane);
+                items += x.rts * splits(x.tiles, chunk);
+            }
+            const double more = (double) a.p.Hkv * __builtin_amdgcn_readlane(wave_scan(items), 63) / a.target;
+            if (more <= 1.0 || chunk > 1000000) break;  // (all items resident; or one split each, and still too many)
+            chunk = __builtin_amdgcn_readfirstlane((int) (chunk * fmin(0.5 + 0.5 * more, 1.5)) + 1);
+        }
     }
 
     // The sequence found, uniform.
@@ -232,7 +245,7 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
     h8_t * const sq = reinterpret_cast<h8_t *>(shared + (kRings > kSums ? kRings : kSums));  // [16 rows][block][lane]
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     __builtin_amdgcn_s_setprio(3);
-    Plan<ROWS> plan(a);
+    Plan<ROWS, TREE> plan(a);
     if (!plan.find(blockIdx.x)) {
         if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = Part{};
         return;
@@ -403,7 +416,9 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
                     const int w0 = (int) max(rel >> 5, (int64_t) -1), sh = (int) rel & 31;
 #pragma unroll
                     for (int i = 0; i < RA; i++) {
-                        const int r = row_of(16 * i + lr);
+                        int y = 16 * i + lr;
+                        asm("" : "+v"(y));  // (here: its row kept over the loop takes registers that there are not)
+                        const int r = row_of(y);
                         const uint32_t * m = a.tree.mask + (int64_t) r * a.tree.ld;
                         uint32_t bits = ~0u;
                         if (rel > -32) {

@@ -462,8 +462,7 @@ class DraftTree:
         _ints(self.mask, "mask", (n, words), d)
         if not 1 <= words <= 32:
             raise ValueError(f"masks of 1 to 32 words, got {words}")
-        for name, value in (("_n", n), ("_device", d), ("_c", (self.positions.data_ptr(), self.mask.data_ptr(), words))):
-            object.__setattr__(self, name, value)
+        self.__dict__.update(_n=n, _device=d, _c=(self.positions.data_ptr(), self.mask.data_ptr(), words))
 
 
 def draft_tree(batch: PagedBatch, parents: torch.Tensor, max_rows: int | None = None, window: int = 0,
@@ -481,7 +480,11 @@ def draft_tree(batch: PagedBatch, parents: torch.Tensor, max_rows: int | None = 
         if not 1 <= max_rows <= 1024:
             raise ValueError(f"max_rows {max_rows} is not in 1 .. 1024")
         _ints(parents, "parents", (n,), d)
-        out = DraftTree(parents, torch.empty_like(parents), parents.new_empty((n, (max_rows + 31) // 32)))
+        words = (max_rows + 31) // 32
+        positions, mask = torch.empty_like(parents), parents.new_empty((n, words))
+        at = positions.data_ptr(), mask.data_ptr()
+        out = object.__new__(DraftTree)  # (what __post_init__ would look at was just made)
+        out.__dict__.update(parents=parents, positions=positions, mask=mask, _n=n, _device=d, _c=(*at, words))
     elif out.parents is not parents or out._device != d:
         raise ValueError("out is a tree of other parents, or not on the current device")
     positions, mask, words = out._c
