@@ -160,17 +160,18 @@ struct VerifyArgs {
     double * drawn;
 };
 
-// 2^(i / 32)
-__constant__ double kRoots[32] = {
-    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
-    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
-    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
-    1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
-    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103,
-    1.9152065613971474, 1.9571441241754002};
+// 2^(i / 32) as bits, i 2^47 less: with n 2^47 more root n % 32 is 2^(n / 32).
+__constant__ uint64_t kRoots[32] = {
+    0x3ff0000000000000ull, 0x3fefd9b0d3158574ull, 0x3fefb5586cf9890full, 0x3fef9301d0125b51ull, 0x3fef72b83c7d517bull,
+    0x3fef54873168b9aaull, 0x3fef387a6e756238ull, 0x3fef1e9df51fdee1ull, 0x3fef06fe0a31b715ull, 0x3feef1a7373aa9cbull,
+    0x3feedea64c123422ull, 0x3feece086061892dull, 0x3feebfdad5362a27ull, 0x3feeb42b569d4f82ull, 0x3feeab07dd485429ull,
+    0x3feea47eb03a5585ull, 0x3feea09e667f3bcdull, 0x3fee9f75e8ec5f74ull, 0x3feea11473eb0187ull, 0x3feea589994cce13ull,
+    0x3feeace5422aa0dbull, 0x3feeb737b0cdc5e5ull, 0x3feec49182a3f090ull, 0x3feed503b23e255dull, 0x3feee89f995ad3adull,
+    0x3feeff76f2fb5e47ull, 0x3fef199bdd85529cull, 0x3fef3720dcef9069ull, 0x3fef5818dcfba487ull, 0x3fef7c97337b9b5full,
+    0x3fefa4afa2a490daull, 0x3fefd0765b6e4540ull};
 
 // exp by a 32nd of a power of two from LDS and four terms of exp's series on what is left, the fifth taken into the others
-// (z^5 = 5/4 a^2 z^3 - 5/16 a^4 z but for a^5 / 16, |z| <= a = ln 2 / 64: 2^-43). 11 operations of 64 bits and 5 others in `weigh4`, where the
+// (z^5 = 5/4 a^2 z^3 - 5/16 a^4 z but for a^5 / 16, |z| <= a = ln 2 / 64: 2^-43). 11 operations of 64 bits and 4 others in `weigh4`, where the
 // kernels spend their arithmetic; the library's takes some 30. (Loops are left as loops here, and code is written once: most of it
 // runs once in a workgroup, and fetching 40 KB of it took longer than what it did.)
 __device__ __forceinline__ double power(double r) {  // 2^(r / 32), |r| <= 1 / 2
@@ -184,7 +185,7 @@ __device__ __forceinline__ double power(double r) {  // 2^(r / 32), |r| <= 1 / 2
 // 2^(n / 32)
 __device__ __forceinline__ double root(const double * roots, int n) {
     const double y = roots[n & 31];
-    return __hiloint2double(__double2hiint(y) + ((n & ~31) << 15), __double2loint(y));
+    return __hiloint2double(__double2hiint(y) + (n << 15), __double2loint(y));
 }
 struct Soft {
     const double * roots;  // LDS
@@ -237,7 +238,9 @@ struct Running {
     }
     // in: m's, at first {0, -inf}
     __device__ __forceinline__ void take4(const double * roots, double scale, Range & in, const float (&l)[4]) {
-        const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+        // (the largest, NaNs passed over, as medians with infinity: fmaxf quiets its operands first, twice the operations)
+        const auto larger = [](float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); };
+        const float top = larger(larger(l[0], l[1]), larger(l[2], l[3]));
         if (__any(top > in.high)) {
             if (m == -INFINITY && top > -INFINITY) {
                 m = fminf(top, kHuge), s = 0.0;
@@ -646,7 +649,7 @@ __global__ __launch_bounds__(kT + 64, 5) void k_verify_rows(const VerifyArgs a) 
     __shared__ double roots[32];
     __shared__ Met met[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = blockIdx.x % a.parts;
-    if (tid < 32) roots[tid] = kRoots[tid];
+    if (tid < 32) roots[tid] = __longlong_as_double((long long) kRoots[tid]);
     int rank = blockIdx.x / a.parts;
     Item it = a.items[rank];
     const int n_items = min(*a.n_items, a.n_rows);
@@ -803,7 +806,7 @@ __global__ __launch_bounds__(kDrawT) void k_verify_draw(const VerifyArgs a) {
     __shared__ DrawLds m;
     __shared__ Path path;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid < 32) m.roots[tid] = kRoots[tid];
+    if (tid < 32) m.roots[tid] = __longlong_as_double((long long) kRoots[tid]);
     const bool of_p = (int) blockIdx.x < a.n_seq;
     const int units = of_p ? a.n_seq : min(*a.n_list, a.n_seq) * a.blocks;
     for (int unit = of_p ? blockIdx.x : blockIdx.x - a.n_seq; unit < units; unit += of_p ? a.n_seq : gridDim.x - a.n_seq) {
