@@ -1054,8 +1054,10 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         a.abreast = (int) std::min<int64_t>(n_rows, std::max(1, kRowGroups / z.parts));
         k_verify_rows<<<paged_grid((int64_t) a.abreast * z.parts, kT + 64), kT + 64, 0, st>>>(a);
         check_launch("draft verify rows");
-        // A path that cannot be all of a sequence's rows tells that rows have several children, of which some will fall.
-        const int draws = draft_logits && max_path < a.max_rows && z.blocks > 8 ? 3 : 1;
+        // A path that cannot be all of a sequence's rows tells that rows have several drawn children, of which some will fall: a sum of what is left for
+        // each, over the chip as often as most need, by one workgroup from there on. (128256 tokens, trees of 20 to 32 rows, one, 4 and 16
+        // sequences: 36, 55 and 132 us with three launches, 41, 60 and 109 with five.)
+        const int draws = draft_logits && max_path < a.max_rows && z.blocks > 8 ? (n_seq < 8 ? 3 : 5) : 1;
         for (int i = 0; i < draws; i++) {
             a.last = i == draws - 1;
             const int64_t groups = n_seq + (draft_logits ? std::min<int64_t>((int64_t) n_seq * z.blocks, 2 * kRowGroups) : 0);
