@@ -924,33 +924,55 @@ struct MoveArgs {
     int max_keep;
 };
 
-// A wavefront moves one sequence's tokens of one KV head in one cache: a lane has the same code bytes of every token. In order of the
-// targets, so that nothing is written before it is read: an entry's source is not below its own number, so no earlier target.
+// A wavefront moves one sequence's tokens of one KV head in one cache: a lane has the same code bytes of every token. Eight tokens are read, then
+// written, in order: an entry's source is not below its own number, so no earlier target, and nothing is written before it is read.
+// Latency (entries, page entries, bytes: 3.3 us), then the lines that it touches, some ten of 128 bytes for the 144 of a token and KV head of
+// 128: 32 sequences' paths of up to 7 rows in 32 layers of 8 KV heads 8.2 us; a token at a time 10.
 template <int D>
-__global__ __launch_bounds__(64) void k_paged_move(const MoveArgs a) {
-    constexpr int B = D / 64 > 0 ? D / 64 : 1;
-    const int lane = threadIdx.x, s = blockIdx.x / a.p.Hkv, hk = blockIdx.x % a.p.Hkv;
+__global__ __launch_bounds__(256) void k_paged_move(const MoveArgs a) {
+    constexpr int B = D / 128 > 0 ? D / 128 : 1, N = 8;
+    const int lane = threadIdx.x & 63, unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = unit / a.p.Hkv, hk = unit % a.p.Hkv;
+    if (s >= a.p.n_seq) return;
     Paged p = a.p;
     p.data = a.data[blockIdx.y];
     const int n = min(a.count[s], a.max_keep);
     const int64_t past = a.p.past[s];
-    for (int i = 0; i < n; i++) {
-        const int j = a.rows[s * a.ld + i];
-        if (j <= i) continue;
-        const int64_t src = paged_tile(p, s, past + j, hk, D), dst = paged_tile(p, s, past + i, hk, D);
-        if (src < 0 || dst < 0) continue;
-        const int ts = (int) (past + j) & 31, td = (int) (past + i) & 31;
+    for (int i0 = 0; i0 < n; i0 += N) {
+        // lanes 0 .. 7 look up the sources, 8 .. 15 the targets
+        const int e = i0 + (lane & (N - 1)), j = e < n ? a.rows[s * a.ld + e] : -1;
+        const int64_t at = lane < 2 * N && j > e ? paged_tile(p, s, past + (lane < N ? j : e), hk, D) : -1;
+        const int lo = (int) (uint32_t) at, hi = (int) (at >> 32);
+        const auto of = [&](int l) {
+            return (int64_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readlane(hi, l) << 32 | (uint32_t) __builtin_amdgcn_readlane(lo, l));
+        };
+        uint8_t k[N][B], v[N][B];
+        uint16_t d[N];
 #pragma unroll
-        for (int b = 0; b < B; b++) {
-            const int e = lane + 64 * b;
-            if (e < D / 2) {
-                p.data[dst + paged_k_byte<D>(td, e)] = p.data[src + paged_k_byte<D>(ts, e)];
-                p.data[dst + paged_v_byte<D>(td, e)] = p.data[src + paged_v_byte<D>(ts, e)];
-            }
+        for (int i = 0; i < N; i++) {
+            const int64_t src = of(i);
+            const int t = (int) (past + __builtin_amdgcn_readlane(j, i)) & 31;
+            if (src < 0) continue;
+#pragma unroll
+            for (int b = 0; b < B; b++)
+                if (lane + 64 * b < D / 2) {
+                    k[i][b] = p.data[src + paged_k_byte<D>(t, lane + 64 * b)];
+                    v[i][b] = p.data[src + paged_v_byte<D>(t, lane + 64 * b)];
+                }
+            // scales: of K, then of V, which lie as if they were further blocks
+            if (lane < D / 16) d[i] = *reinterpret_cast<const uint16_t *>(p.data + src + paged_k_scale<D>(t, lane));
         }
-        if (lane < D / 16) {  // scales: of K, then of V, whose lie as if they were further blocks
-            const uint16_t d = *reinterpret_cast<const uint16_t *>(p.data + src + paged_k_scale<D>(ts, lane));
-            *reinterpret_cast<uint16_t *>(p.data + dst + paged_k_scale<D>(td, lane)) = d;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int64_t src = of(i), dst = of(N + i);
+            const int t = (int) (past + i0 + i) & 31;
+            if (src < 0 || dst < 0) continue;
+#pragma unroll
+            for (int b = 0; b < B; b++)
+                if (lane + 64 * b < D / 2) {
+                    p.data[dst + paged_k_byte<D>(t, lane + 64 * b)] = k[i][b];
+                    p.data[dst + paged_v_byte<D>(t, lane + 64 * b)] = v[i][b];
+                }
+            if (lane < D / 16) *reinterpret_cast<uint16_t *>(p.data + dst + paged_k_scale<D>(t, lane)) = d[i];
         }
     }
 }
@@ -1089,8 +1111,9 @@ int gcq_paged_move(const gcq_paged_cache * const * caches, int n_caches, const g
         for (int c0 = 0; c0 < n_caches; c0 += kCaches) {
             const int n = std::min(n_caches - c0, kCaches);
             for (int i = 0; i < n; i++) a.data[i] = (uint8_t *) caches[c0 + i]->data;
-            const unsigned x = paged_grid((int64_t) batch->n_seq * a.p.Hkv * n, 64) / n;
-            with_head_dim(caches[0]->head_dim, [&](auto d) { k_paged_move<decltype(d)::value><<<dim3(x, n), 64, 0, as_stream(stream)>>>(a); });
+            const int64_t x = ((int64_t) batch->n_seq * a.p.Hkv + 3) / 4;
+            paged_grid(x * n, 256);
+            with_head_dim(caches[0]->head_dim, [&](auto d) { k_paged_move<decltype(d)::value><<<dim3((unsigned) x, n), 256, 0, as_stream(stream)>>>(a); });
             check_launch("paged move");
         }
     });
