@@ -113,9 +113,9 @@ __global__ __launch_bounds__(256) void k_draft_tree(const TreeArgs a) {
 typedef int i4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kT = 256, kStep = 4 * kT;  // threads, logits of a workgroup at a time
-constexpr int kSteps = 16;               // .. of a part at most
+constexpr int kSteps = 8;                // .. of a part at most
 constexpr int kDrawT = 512;              // threads of k_verify_draw
-constexpr int kRowGroups = 1024;         // workgroups at a time in k_verify_rows
+constexpr int kRowGroups = 768;          // workgroups at a time in k_verify_rows: three on a CU (800 rows in 16 trees 66 us, 68 with four; one chain 27 and 28)
 constexpr float kHuge = 3.402823466e38f;
 
 // What became of a row: the child that stands (>= 0), or
@@ -640,7 +640,7 @@ __device__ __forceinline__ int draw(const VerifyArgs & a, const Source & z, Draw
 // A workgroup has one part of every abreast-th row: those in work at a time are the next of the order that are not cut off. Four wavefronts
 // read; the fifth meets them once for a part: it has then looked up the next row, and shares the part's sums and, its row's last,
 // decides while they read that.
-__global__ __launch_bounds__(kT + 64, 5) void k_verify_rows(const VerifyArgs a) {
+__global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) {
     struct Met {
         Running p[kT / 64], q[kT / 64];
         int top[kT / 64];
@@ -888,11 +888,10 @@ struct VerifyShape {
 VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     VerifyShape z{};
     const auto parts = [&](int steps) { return (V + steps * kStep - 1) / (steps * kStep); };
-    // A part costs its steps and some four more; workgroups take theirs in as many turns. Parts of up to 16 steps where that is
-    // two turns for all rows, of up to 8 where there are more, so that decisions come early enough to spare rows. (205 rows of 64
-    // chains of 128256 tokens: 77 us with up to 16 steps, 87 with 8; 800 rows of 16 trees: 68 and 56.)
+    // A part costs its steps and some four more; workgroups take theirs in as many turns. Of up to 8 steps: decisions come early enough to
+    // spare rows (128256 tokens, 205 rows in 64 chains: 91 us, 92 with up to 16; 800 rows in 16 trees: 66 and 83).
     int64_t best = INT64_MAX;
-    for (int k = 2; k <= (n_rows * parts(kSteps) <= 2 * kRowGroups ? kSteps : kSteps / 2); k += 2) {
+    for (int k = 2; k <= kSteps; k += 2) {
         const int64_t cost = (n_rows * parts(k) + kRowGroups - 1) / kRowGroups * (k + 4);
         if (cost < best) best = cost, z.steps = k;
     }
@@ -1078,7 +1077,7 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         check_launch("draft verify rows");
         // A path that cannot be all of a sequence's rows tells that rows have several drawn children, of which some will fall: a sum of what is left for
         // each, over the chip as often as most need, by one workgroup from there on. (128256 tokens, trees of 20 to 32 rows, one, 4 and 16
-        // sequences: 36, 55 and 132 us with three launches, 41, 60 and 109 with five.)
+        // sequences: 34, 54 and 128 us with three launches, 40, 60 and 105 with five.)
         const int draws = draft_logits && max_path < a.max_rows && z.blocks > 8 ? (n_seq < 8 ? 3 : 5) : 1;
         for (int i = 0; i < draws; i++) {
             a.last = i == draws - 1;
