@@ -160,15 +160,11 @@ struct VerifyArgs {
     double * drawn;
 };
 
-// 2^(i / 32) as bits, i 2^47 less: with n 2^47 more root n % 32 is 2^(n / 32).
-__constant__ uint64_t kRoots[32] = {
-    0x3ff0000000000000ull, 0x3fefd9b0d3158574ull, 0x3fefb5586cf9890full, 0x3fef9301d0125b51ull, 0x3fef72b83c7d517bull,
-    0x3fef54873168b9aaull, 0x3fef387a6e756238ull, 0x3fef1e9df51fdee1ull, 0x3fef06fe0a31b715ull, 0x3feef1a7373aa9cbull,
-    0x3feedea64c123422ull, 0x3feece086061892dull, 0x3feebfdad5362a27ull, 0x3feeb42b569d4f82ull, 0x3feeab07dd485429ull,
-    0x3feea47eb03a5585ull, 0x3feea09e667f3bcdull, 0x3fee9f75e8ec5f74ull, 0x3feea11473eb0187ull, 0x3feea589994cce13ull,
-    0x3feeace5422aa0dbull, 0x3feeb737b0cdc5e5ull, 0x3feec49182a3f090ull, 0x3feed503b23e255dull, 0x3feee89f995ad3adull,
-    0x3feeff76f2fb5e47ull, 0x3fef199bdd85529cull, 0x3fef3720dcef9069ull, 0x3fef5818dcfba487ull, 0x3fef7c97337b9b5full,
-    0x3fefa4afa2a490daull, 0x3fefd0765b6e4540ull};
+// 2^(i / 32), i of 32, its bits i 2^47 less: with n 2^47 more root n % 32 is 2^(n / 32).
+__device__ __forceinline__ double root_of(int i) {
+    const double y = exp2(i * 0x1p-5);
+    return __hiloint2double(__double2hiint(y) - (i << 15), __double2loint(y));
+}
 
 // exp by a 32nd of a power of two from LDS and four terms of exp's series on what is left, the fifth taken into the others
 // (z^5 = 5/4 a^2 z^3 - 5/16 a^4 z but for a^5 / 16, |z| <= a = ln 2 / 64: 2^-43). 11 operations of 64 bits and 4 others in `weigh4`, where the
@@ -649,7 +645,7 @@ __global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) 
     __shared__ double roots[32];
     __shared__ Met met[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = blockIdx.x % a.parts;
-    if (tid < 32) roots[tid] = __longlong_as_double((long long) kRoots[tid]);
+    if (tid < 32) roots[tid] = root_of(tid);
     int rank = blockIdx.x / a.parts;
     Item it = a.items[rank];
     const int n_items = min(*a.n_items, a.n_rows);
@@ -806,7 +802,7 @@ __global__ __launch_bounds__(kDrawT) void k_verify_draw(const VerifyArgs a) {
     __shared__ DrawLds m;
     __shared__ Path path;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid < 32) m.roots[tid] = __longlong_as_double((long long) kRoots[tid]);
+    if (tid < 32) m.roots[tid] = root_of(tid);
     const bool of_p = (int) blockIdx.x < a.n_seq;
     const int units = of_p ? a.n_seq : min(*a.n_list, a.n_seq) * a.blocks;
     for (int unit = of_p ? blockIdx.x : blockIdx.x - a.n_seq; unit < units; unit += of_p ? a.n_seq : gridDim.x - a.n_seq) {
