@@ -91,8 +91,9 @@ __device__ __forceinline__ int splits(int tiles, int chunk) { return max(1, (til
 // Items of split row tiles have a slot each for their sums. Those are fewer than 2 target: with u tiles in all items' and a chunk of more than
 // u / cut, a row tile has less than tiles cut / u splits more than one, all of them together less than cut <= target, and a split row tile has
 // at most twice as many splits as that.
-// FILL (trees): about the least chunk with which all items are resident at once: 61 rows over 65000 keys in 768 workgroups and not 704, 167 us
-// instead of 185; trees of 16 sequences 65 instead of 73. (Rows in lines keep the splits, and so the roundings, that they had.)
+// FILL (trees): about the least chunk with which all items are resident at once, if their row tiles are: 61 rows over 65000 keys in 768
+// workgroups and not 704, 167 us instead of 185; trees of 16 sequences 65 instead of 73. Not with more, or sequences that the lanes do not
+// hold: 512 of 8 rows took 518 us and not 400. (Rows in lines keep the splits, and so the roundings, that they had.)
 template <int ROWS, bool FILL>
 struct Plan {
     const AttnArgs & a;
@@ -112,17 +113,13 @@ struct Plan {
         }
         u = wave_sum_d(u) * a.p.Hkv;
         n = wave_sum_d(n) * a.p.Hkv;
-        const double cut = fmax(a.target - n, 0.5 * a.target);
-        chunk = __builtin_amdgcn_readfirstlane((int) fmax((double) a.min_chunk, fmin(u / (FILL ? a.target : cut) + 1.0, 1e9)));
-        if (!FILL) return;
-        for (int turn = 0; turn < 8; turn++) {
-            int items = w.rts * splits(w.tiles, chunk);
-            for (int s0 = 64; s0 < a.p.n_seq; s0 += 64) {
-                const SeqWork x = seq_work<ROWS>(a, s0 + lane);
-                items += x.rts * splits(x.tiles, chunk);
-            }
+        const bool fill = FILL && a.p.n_seq <= 64 && n < a.target;
+        const double cut = fill ? a.target : fmax(a.target - n, 0.5 * a.target);
+        chunk = __builtin_amdgcn_readfirstlane((int) fmax((double) a.min_chunk, fmin(u / cut + 1.0, 1e9)));
+        for (int turn = 0; fill && turn < 8; turn++) {
+            const int items = w.rts * splits(w.tiles, chunk);
             const double more = (double) a.p.Hkv * __builtin_amdgcn_readlane(wave_scan(items), 63) / a.target;
-            if (more <= 1.0 || chunk > 1000000) break;  // (all items resident; or one split each, and still too many)
+            if (more <= 1.0) break;  // (all items resident)
             chunk = __builtin_amdgcn_readfirstlane((int) (chunk * fmin(0.5 + 0.5 * more, 1.5)) + 1);
         }
     }
