@@ -1,6 +1,7 @@
 // draft.hip - steps with drafted tokens: the trees' masks and positions, the drafts' verification, and moving the accepted rows
 // together in the caches (include/gcq_draft.h; append and attention of such rows are paged.hip's and paged_attn.hip's).
 #include <algorithm>
+#include <vector>
 
 #include "paged.h"
 
@@ -775,7 +776,7 @@ __global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) 
             if (on) {
                 x = reinterpret_cast<const i4_t *>(a.items + mine)[0], y = reinterpret_cast<const i4_t *>(a.items + mine)[1];
                 on = x.z == 0 || x.w >= 0;
-                for (int c = x.z, u = x.w; on && u >= 0 && u < c && y.x >= 0 && y.x + c < a.n_rows;) {
+                for (int c = x.z, u = x.w; on && u >= 0 && u < c && c < kMaxRows && y.x >= 0 && y.x < a.n_rows - c;) {
                     const int next = agent_load(&a.next[y.x + u]), up = a.parents[y.x + u];
                     on = next == kOpen || next == c || (next <= kFell && c > kFell - next);
                     c = u, u = up;
@@ -1099,6 +1100,11 @@ int gcq_paged_move(const gcq_paged_cache * const * caches, int n_caches, const g
                               caches[c0]->n_head_kv == caches[0]->n_head_kv && caches[c0]->head_dim == caches[0]->head_dim,
                           "paged_move: the caches must be of one shape");
         }
+        const size_t size = gcq_paged_cache_size(caches[0]->n_pages, caches[0]->page_size, caches[0]->n_head_kv, caches[0]->head_dim);
+        std::vector<uintptr_t> at(n_caches);
+        std::transform(caches, caches + n_caches, at.begin(), [](const gcq_paged_cache * c) { return (uintptr_t) c->data; });
+        std::sort(at.begin(), at.end());
+        for (int i = 1; i < n_caches; i++) paged_require(at[i] - at[i - 1] >= size, "paged_move: caches overlap (a row would move twice)");
         if (max_keep == 0) return;
         MoveArgs a{};
         a.p = paged_view(caches[0], batch, 1);

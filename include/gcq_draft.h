@@ -76,7 +76,7 @@ GCQ_API int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, 
 /* In each of n_caches caches of one shape, slot past[s] + i takes what slot past[s] + rows[s][i] holds, for i < count[s] and
  * i < max_keep; rows [n_seq][ld_rows]. All sources as they were before the call. An entry below its own number i, and one
  * whose slots are not there, moves nothing (a path's rows are all at or above their numbers). Of the batch, pages and past are
- * read. caches: an array of pointers, on the host. */
+ * read. caches: an array of pointers, on the host, to caches that share no memory. */
 GCQ_API int gcq_paged_move(const gcq_paged_cache * const * caches, int n_caches, const gcq_paged_batch * batch,
                            const int32_t * count, const int32_t * rows, int64_t ld_rows, int max_keep, void * stream);
 

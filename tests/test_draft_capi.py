@@ -130,7 +130,11 @@ def test_move_refusals():
     _refused(_move(ld_rows=3), "max_keep")
     _refused(_move(max_keep=-1), "max_keep")
     _refused(_move(None, _batch(pages=None)), "pages is NULL")
+    same = _cache()
+    _refused(_move([same, same]), "caches overlap")
+    _refused(_move([_cache(data=P + (1 << 40)), _cache(), _cache(data=P + 4096)]), "caches overlap")
     assert _move(max_keep=0) == 0
+    assert _move([_cache(data=P + (1 << 40)), _cache(), _cache(data=P + (1 << 30))], max_keep=0) == 0
 
 
 def test_python_refusals_without_a_device():
