@@ -511,7 +511,8 @@ def draft_verify(starts: torch.Tensor, parents: torch.Tensor, tokens: torch.Tens
     what follows each row; coins f32 [n], uniform of [0, 1); draft_logits f32 [n, V]: a row's children were drawn from their
     softmax (None: guesses that were not drawn); temperature f32 [S] (None: 1; 0: the largest logit). Rows of logits may be
     strided, unit inner stride. max_rows: no sequence has more rows than this (default n, at most 1024); max_path: a
-    path's rows at most (default max_rows). out: into these."""
+    path's rows at most (default max_rows; for trees their depth and one: shorter results, and with draft_logits the sums of what
+    fallen drafts leave take the whole device where it is less than max_rows). out: into these."""
     d, n, S = torch._C._cuda_getDevice(), parents.numel(), starts.numel() - 1
     if S < 1:
         raise ValueError("starts must hold at least two numbers")
@@ -547,7 +548,7 @@ def draft_verify(starts: torch.Tensor, parents: torch.Tensor, tokens: torch.Tens
 
 
 def paged_move(caches: PagedCache | list[PagedCache], batch: PagedBatch, count: torch.Tensor, rows: torch.Tensor) -> None:
-    """The accepted rows together: in each cache (all layers', of one shape) slot past[s] + i takes what slot past[s] +
+    """The accepted rows together: in each cache (all layers', of one shape, each once) slot past[s] + i takes what slot past[s] +
     rows[s, i] holds, for i < count[s]. count int32 [S], rows int32 [S, m] (strided rows allowed), a DraftPath's. All sources as
     before the call; an entry below its own number, or one whose slots are not there, moves nothing."""
     caches = [caches] if isinstance(caches, PagedCache) else caches
