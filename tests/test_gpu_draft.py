@@ -280,6 +280,17 @@ def test_attention_of_a_long_tree(gops):
     check_tree(case, out, want, bound)
 
 
+@pytest.mark.parametrize("D,Hkv,G,S,longest", [(64, 1, 2, 70, 3000), (128, 8, 2, 64, 1500), (128, 8, 4, 110, 1300), (256, 2, 1, 130, 200)])
+def test_attention_of_more_trees_than_fit(gops, D, Hkv, G, S, longest):
+    """More sequences than lanes, and more row tiles than workgroups that are resident at once; one of them long, so that some are split."""
+    rng = np.random.default_rng(S)
+    rows, past = [int(x) for x in rng.integers(0, 12, S)], [int(x) for x in rng.integers(0, 60, S)]
+    rows[S // 2], past[S // 2] = 20, longest
+    case = Case(gops, rows, past, Hkv, D, 64, seed=S, extra_rows=1)
+    out, want, bound = run_tree(gops, case, G, random_trees(rows, rng), max_rows=20)
+    check_tree(case, out, want, bound)
+
+
 # ------------------------------------------------------------------------------------ verification
 
 
@@ -487,6 +498,35 @@ def test_verify_special_logits(gops, drawn):
     assert verify(gops, rows, *a, max_path=3) == reference(rows, *a)
 
 
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("V,rows", [(150001, [3, 6]), (700001, [5])])
+def test_verify_large_vocabularies(gops, drawn, V, rows):
+    """More parts than lanes: the total and the part are found 64 at a time, by coins from 0 to next to 1."""
+    n = sum(rows)
+    parents, tokens, logits, coins, draft, _ = make_verify(rows, V, True, 3, seed=V, temps=(1.0,))
+    logits = logits * 0.3  # flat: any part may be the one
+    draft = draft * 0.3
+    for root in (0.0, 0.03, 0.5, 0.93, 1 - 2.0 ** -24):
+        coins[np.cumsum([0] + rows[:-1])] = root
+        a = (parents, tokens, logits, coins, draft if drawn else None)
+        assert verify(gops, rows, *a, pad=3) == reference(rows, *a, max_path=n)
+        assert verify(gops, rows, *a, max_path=2) == reference(rows, *a, max_path=2)
+
+
+def test_verify_logits_past_32_bits(gops):
+    """Rows of logits whose offsets pass 32 bits, and lie in one tensor with the drafter's."""
+    rows, V, ld = [4, 2], 5000, 400_000_004
+    a = make_verify(rows, V, True, 2, seed=21)
+    n = sum(rows)
+    both = torch.empty(n * ld, device="cuda").as_strided((n, ld), (ld, 1))
+    logits, draft = both[:, 8:8 + V], both[:, 300_000_000:300_000_000 + V]
+    logits.copy_(torch.from_numpy(a[2]))
+    draft.copy_(torch.from_numpy(a[4]))
+    path = gops.draft_verify(ints(np.concatenate([[0], np.cumsum(rows)])), ints(a[0]), ints(a[1]), logits, torch.from_numpy(a[3]).cuda(),
+                             draft_logits=draft, temperature=torch.from_numpy(a[5]).cuda())
+    assert (path.count.tolist(), path.rows.tolist(), path.tokens.tolist()) == reference(rows, *a, max_path=n)
+
+
 def test_verify_what_is_left(gops):
     """Target and drafter far apart, equal, and equal but for one token: rows that fall until nothing or one token is left."""
     V, n = 1000, 12
@@ -603,6 +643,32 @@ def test_move_in_many_layers(gops):
     for c, w in zip(layers, want):
         w[b] = w[a]
         assert torch.equal(c.data, w)
+
+
+def test_step_in_a_cache_past_four_gigabytes(gops):
+    """Append at positions, tree attention and move at page offsets past 32 bits: the bytes of a small cache."""
+    D, Hkv, page, rows, past = 256, 8, 256, 40, 500
+    size = page * Hkv * 288
+    n_pages = (5 << 30) // size
+    big, small = gops.PagedCache.new(n_pages, page, Hkv, D), gops.PagedCache.new(3, page, Hkv, D)
+    assert big.data.numel() > 1 << 32
+    at = [n_pages - 1, 3, n_pages - 2]
+    starts, before = ints([0, rows]), ints([past])
+    batches = gops.PagedBatch(ints([at]), starts, before), gops.PagedBatch(ints([[0, 1, 2]]), starts, before)
+    parents = ints(random_trees([rows], np.random.default_rng(2)))
+    g = torch.Generator().manual_seed(3)
+    k0, v0 = (torch.randn((past, Hkv, D), generator=g).cuda() for _ in range(2))
+    k, v = (torch.randn((rows, Hkv, D), generator=g).cuda() for _ in range(2))
+    freqs, outs = gops.rope_freqs(D, 10000.0), []
+    for cache, b in zip((big, small), batches):
+        gops.paged_append(cache, gops.PagedBatch(b.pages, ints([0, past]), ints([0])), k0, v0)
+        tree = gops.draft_tree(b, parents)
+        q = gops.paged_append(cache, b, k, v, q=k, freqs=freqs, positions=tree.positions)
+        outs.append(gops.paged_attn(cache, b, q, 1 / 16, tree=tree))
+        gops.paged_move(cache, b, ints([5]), ints([[0, 2, 9, 30, 39]]))
+    assert outs[0].isfinite().all() and torch.equal(*outs)
+    for i, pg in enumerate(at):
+        assert torch.equal(big.data[pg * size:(pg + 1) * size], small.data[i * size:(i + 1) * size])
 
 
 # ------------------------------------------------------------------------------------ together
