@@ -117,6 +117,7 @@ constexpr int kT = 256, kStep = 4 * kT;  // threads, logits of a workgroup at a 
 constexpr int kSteps = 8;                // .. of a part at most
 constexpr int kDrawT = 512;              // threads of k_verify_draw
 constexpr int kRowGroups = 768;          // workgroups at a time in k_verify_rows: three on a CU (800 rows in 16 trees 66 us, 68 with four; one chain 27 and 28)
+constexpr int kApart = 64;               // ints from one row's counter to the next: in one line all rows' workgroups queue, some 8 ns each (64 single rows 34 us, 31 so)
 constexpr float kHuge = 3.402823466e38f;
 
 // What became of a row: the child that stands (>= 0), or
@@ -155,7 +156,7 @@ struct VerifyArgs {
     int * n_items, * n_list, * list;  // the sequences that draw from what is left
     Item * items;
     RowState * state;
-    int * next, * arrived;  // of the rows
+    int * next, * arrived;  // of the rows (arrived kApart apart)
     PartSums * sums;
     SeqState * seq;
     double * drawn;
@@ -229,6 +230,10 @@ struct Running {
     double s;
     // s2 times exp(m2 / t) more
     __device__ __forceinline__ void take(const double * roots, double scale, float m2, double s2) {
+        if (!__any(m > -INFINITY)) {
+            m = m2, s = s2;
+            return;
+        }
         const Soft z{roots, scale, (double) fmaxf(m, m2), 0.0};
         s = s * z.weight(m) + s2 * z.weight(m2);
         m = fmaxf(m, m2);
@@ -335,7 +340,7 @@ __global__ __launch_bounds__(kT) void k_verify_begin(const VerifyArgs a) {
     for (int s = id; s < a.n_seq; s += all_ids) a.seq[s] = SeqState{}, a.count[s] = 0;
     for (int64_t i = id; i < (int64_t) a.n_seq * a.max_path; i += all_ids) a.rows[i] = a.out[i] = -1;
     if (r >= a.n_rows) return;
-    if (lane == 0) a.next[r] = kOpen, a.arrived[r] = 0;
+    if (lane == 0) a.next[r] = kOpen, a.arrived[(int64_t) r * kApart] = 0;
     const auto load = [&](int s0) { return s0 + lane < a.n_seq ? rows_of(a.starts, s0 + lane, a.n_rows, a.max_rows) : Rows{}; };
     const Rows first = load(0);
     Rows w{}, x = first;
@@ -635,8 +640,8 @@ __device__ __forceinline__ int draw(const VerifyArgs & a, const Source & z, Draw
 }
 
 // A workgroup has one part of every abreast-th row: those in work at a time are the next of the order that are not cut off. Four wavefronts
-// read; the fifth meets them once for a part: it has then looked up the next row, and shares the part's sums and, its row's last,
-// decides while they read that.
+// read; the fifth meets them once for a part: it has then looked up the next row and this one's children, and shares the part's sums and,
+// its row's last, decides while they read that.
 __global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) {
     struct Met {
         Running p[kT / 64], q[kT / 64];
@@ -707,6 +712,7 @@ __global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) 
         return;
     }
     Item done{};
+    Children kids{};  // done's
     for (int turn = 0;; turn ^= 1) {
         // the row before: its sums first of the wavefronts, then, for the last of the row's workgroups to end, of the parts
         const auto end = [&] {
@@ -715,8 +721,6 @@ __global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) 
             const bool greedy = !(done.t > 0.0f), drawn = a.draft && !greedy && done.child < done.n;
             const double scale = greedy ? 1.0 : scale_of(done.t);
             PartSums * const sums = a.sums + (int64_t) done.r * a.parts;
-            Children kids{};
-            if (done.child < done.n) kids = children(a, w, done.j, done.j + 1);
             Running p, q;
             int top;
 #pragma unroll 1
@@ -737,7 +741,7 @@ __global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) 
                 if (lane == 0) {
                     share(sums + part, PartSums{p.s, q.s, p.m, q.m, top, 0});
                     stores_done();
-                    last = __hip_atomic_fetch_add(a.arrived + done.r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
+                    last = __hip_atomic_fetch_add(a.arrived + (int64_t) done.r * kApart, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
                 }
                 if (!__builtin_amdgcn_readfirstlane(last)) return;
             }
@@ -748,10 +752,13 @@ __global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) 
             if (lane == 0) {
                 a.state[done.r] = RowState{p.s, q.s, C, p.m, q.m, top, 0};
                 agent_store(&a.next[done.r], next);
-                stores_done();
             }
             // Whoever decides a path's last row to be decided sees the others' decisions, its own being known before they are looked at.
-            const Path path = follow<false>(a, w, done.s, 0, 0, done.j);
+            Path path{1, 0, next, true, 0};
+            if (done.j > 0 || next >= 0) {
+                stores_done();
+                path = follow<false>(a, w, done.s, 0, 0, done.j);
+            }
             if (!path.on || path.then == kOpen || (path.then >= 0 && path.n < a.max_path)) return;
             SeqState & seq = a.seq[done.s];  // (two at once write the same)
             int listed = 1;
@@ -791,6 +798,8 @@ __global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) 
             }
         }
         if (rank >= n_items && lane == 0) met[turn].next.n = -1, met[turn].next.j = 0;
+        kids.at = 0;
+        if (it.child < it.n) kids = children(a, Rows{it.r0, it.n}, it.j, it.j + 1);
         __syncthreads();
         done = it;
         it = met[turn].next;
@@ -897,7 +906,7 @@ VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     z.state = z.items + align256((size_t) n_rows * sizeof(Item));
     z.next = z.state + align256((size_t) n_rows * sizeof(RowState));
     z.arrived = z.next + align256((size_t) n_rows * sizeof(int));
-    z.sums = z.arrived + align256((size_t) n_rows * sizeof(int));
+    z.sums = z.arrived + align256((size_t) n_rows * kApart * sizeof(int));
     z.seq = z.sums + align256((size_t) n_rows * z.parts * sizeof(PartSums));
     z.block_steps = 2;  // (half of the sequences may have something left)
     while (z.block_steps < kSteps && n_seq * parts(z.block_steps) > 2 * kRowGroups) z.block_steps *= 2;
