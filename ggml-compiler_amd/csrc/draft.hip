@@ -473,11 +473,13 @@ __device__ __forceinline__ Path follow(const VerifyArgs & a, const Rows & w, int
 
 // A lane's value and those of the lanes before.
 __device__ __forceinline__ double upto(double v) {
-#pragma unroll 1
-    for (int o = 1; o < 64; o <<= 1) {
-        const double b = __shfl_up(v, o, 64);
-        if ((threadIdx.x & 63) >= (unsigned) o) v += b;
-    }
+    const auto add = [&](auto move) { v += __hiloint2double(move(__double2hiint(v)), move(__double2loint(v))); };
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true); });  // row_shr 1, 2, 4, 8
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true); });
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true); });
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true); });
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false); });  // lane 15 into the next row, then 31 into the upper half
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false); });
     return v;
 }
 
