@@ -116,7 +116,7 @@ typedef int i4_t __attribute__((ext_vector_type(4)));
 constexpr int kT = 256, kStep = 4 * kT;  // threads, logits of a workgroup at a time
 constexpr int kSteps = 8;                // .. of a part at most
 constexpr int kDrawT = 512;              // threads of k_verify_draw
-constexpr int kRowGroups = 768;          // workgroups at a time in k_verify_rows: three on a CU (800 rows in 16 trees 66 us, 68 with four; one chain 27 and 28)
+constexpr int kRowGroups = 768;          // workgroups at a time in k_verify_rows: three on a CU (64 chains 88 us, 99 with four; 16 trees 59 and 64)
 constexpr int kApart = 64;               // ints from one row's counter to the next: in one line all rows' workgroups queue, some 8 ns each (64 single rows 34 us, 31 so)
 constexpr float kHuge = 3.402823466e38f;
 
@@ -897,9 +897,10 @@ VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     VerifyShape z{};
     const auto parts = [&](int steps) { return (V + steps * kStep - 1) / (steps * kStep); };
     // A part costs its steps and some four more; workgroups take theirs in as many turns. Of up to 8 steps: decisions come early enough to
-    // spare rows (128256 tokens, 205 rows in 64 chains: 91 us, 92 with up to 16; 800 rows in 16 trees: 66 and 83).
+    // spare rows (128256 tokens, 205 rows in 64 chains: 91 us, 92 with up to 16; 800 rows in 16 trees: 66 and 83). Of up to 6 where sequences
+    // have many rows, most of which no path comes to (those trees: 59 and, with 4, 62; 128 chains of 8 rows 103, and 92 with 8).
     int64_t best = INT64_MAX;
-    for (int k = 2; k <= kSteps; k += 2) {
+    for (int k = 2; k <= (n_rows >= 16 * (int64_t) n_seq ? 6 : kSteps); k += 2) {
         const int64_t cost = (n_rows * parts(k) + kRowGroups - 1) / kRowGroups * (k + 4);
         if (cost < best) best = cost, z.steps = k;
     }
@@ -1085,7 +1086,7 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         check_launch("draft verify rows");
         // A path that cannot be all of a sequence's rows tells that rows have several drawn children, of which some will fall: a sum of what is left for
         // each, over the chip as often as most need, by one workgroup from there on. (128256 tokens, trees of 20 to 32 rows, one, 4 and 16
-        // sequences: 34, 54 and 128 us with three launches, 40, 60 and 105 with five.)
+        // sequences: 32, 51 and 123 us with three launches, 34, 55 and 100 with five.)
         const int draws = draft_logits && max_path < a.max_rows && z.blocks > 8 ? (n_seq < 8 ? 3 : 5) : 1;
         for (int i = 0; i < draws; i++) {
             a.last = i == draws - 1;
