@@ -159,7 +159,7 @@ struct VerifyArgs {
     int * next, * arrived;  // of the rows (arrived kApart apart)
     PartSums * sums;
     SeqState * seq;
-    double * drawn;
+    double * drawn, * drawn_runs;  // of a sequence's parts of what is left, and of their runs of 256 tokens
 };
 
 // 2^(i / 32), i of 32, its bits i 2^47 less: with n 2^47 more root n % 32 is 2^(n / 32).
@@ -610,9 +610,11 @@ __device__ __forceinline__ int draw(const VerifyArgs & a, const Source & z, Draw
     }
     if (part < 0) return -1;
     want = rest;  // (no part passes it, by rounding: the last token of the last)
-    runs(a, z, m, part, all);
+    const bool fell = z.C > 0.0 && !all;
+    if (!fell) runs(a, z, m, part, all);
     if (threadIdx.x < 64) {
-        d = lane < 4 * z.steps ? m.seg[lane] : 0.0;
+        d = 0.0;
+        if (lane < 4 * z.steps) d = fell ? shared(a.drawn_runs + ((int64_t) z.s * z.parts + part) * (4 * z.steps) + lane) : m.seg[lane];
         const int run = pass(d, upto(d), want, base, hit);
         int token = -1;
         if (run >= 0) {
@@ -837,6 +839,7 @@ __global__ __launch_bounds__(kDrawT) void k_verify_draw(const VerifyArgs a) {
 #pragma unroll 1
                 for (int b = alone ? 0 : own; b < (alone ? a.blocks : own + 1); b++) {
                     const double v = runs(a, z, m, b, false);
+                    if (tid < 4 * a.block_steps) agent_store(a.drawn_runs + ((int64_t) s * a.blocks + b) * (4 * a.block_steps) + tid, m.seg[tid]);
                     if (tid == 0) share(a.drawn + (int64_t) s * a.blocks + b, v);
                 }
                 if (alone) {
@@ -891,7 +894,7 @@ __global__ __launch_bounds__(kDrawT) void k_verify_draw(const VerifyArgs a) {
 struct VerifyShape {
     int steps, parts;
     int blocks, block_steps;
-    size_t items, state, next, arrived, sums, seq, list, drawn, total;  // offsets
+    size_t items, state, next, arrived, sums, seq, list, drawn, drawn_runs, total;  // offsets
 };
 VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     VerifyShape z{};
@@ -916,7 +919,8 @@ VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     z.blocks = (int) parts(z.block_steps);
     z.list = z.seq + align256((size_t) n_seq * sizeof(SeqState));
     z.drawn = z.list + align256((size_t) n_seq * sizeof(int));
-    z.total = z.drawn + align256((size_t) n_seq * z.blocks * sizeof(double));
+    z.drawn_runs = z.drawn + align256((size_t) n_seq * z.blocks * sizeof(double));
+    z.total = z.drawn_runs + align256((size_t) n_seq * z.blocks * 4 * z.block_steps * sizeof(double));
     return z;
 }
 
@@ -1075,7 +1079,7 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         a.count = count, a.rows = rows, a.out = tokens_out;
         a.n_items = (int *) at, a.n_list = a.n_items + 1, a.items = (Item *) (at + z.items), a.state = (RowState *) (at + z.state);
         a.next = (int *) (at + z.next), a.arrived = (int *) (at + z.arrived), a.sums = (PartSums *) (at + z.sums), a.seq = (SeqState *) (at + z.seq);
-        a.list = (int *) (at + z.list), a.drawn = (double *) (at + z.drawn);
+        a.list = (int *) (at + z.list), a.drawn = (double *) (at + z.drawn), a.drawn_runs = (double *) (at + z.drawn_runs);
         hipStream_t st = as_stream(stream);
         k_verify_begin<<<paged_grid(std::max<int64_t>((n_rows + 3) / 4, 1), kT), kT, 0, st>>>(a);
         check_launch("draft verify");
