@@ -93,16 +93,19 @@ __device__ __forceinline__ int splits(int tiles, int chunk) { return max(1, (til
 // at most twice as many splits as that.
 // FILL (trees): about the least chunk with which all items are resident at once, if their row tiles are: 61 rows over 65000 keys in 768
 // workgroups and not 704, 167 us instead of 185; trees of 16 sequences 65 instead of 73. Not with more, or sequences that the lanes do not
-// hold: 512 of 8 rows took 518 us and not 400. (Rows in lines keep the splits, and so the roundings, that they had.)
+// hold: 512 of 8 rows took 518 us and not 400. Then the sequences' order is that of their splits' lengths, longest first: workgroups some 256
+// apart share a CU, and the long ones of one sequence were neighbours there (16 trees over 200 to 30000 keys 213 us, 173 so; over 8191 60 and
+// 58). Not for short splits, which the search for that order would cost 1 us. (Rows in lines keep the splits, and so the roundings, that they had.)
 template <int ROWS, bool FILL>
 struct Plan {
     const AttnArgs & a;
     SeqWork w;  // of sequence s0 + lane
-    int chunk, s, base, slot, lane_at;
+    int chunk, s, base, slot, lane_at, own;  // own: w's sequence
 
     __device__ __forceinline__ Plan(const AttnArgs & args) : a(args) {
         const int lane = threadIdx.x & 63;
         w = seq_work<ROWS>(a, lane);
+        own = lane;
         chunk = a.min_chunk;
         if (!a.parts) return;  // one split each
         double u = (double) w.rts * w.tiles, n = w.rts;
@@ -122,6 +125,17 @@ struct Plan {
             if (more <= 1.0) break;  // (all items resident)
             chunk = __builtin_amdgcn_readfirstlane((int) (chunk * fmin(0.5 + 0.5 * more, 1.5)) + 1);
         }
+        if (fill && a.p.n_seq > 1 && chunk > 32) {
+            // (lanes past the sequences have no rows, whichever they go to)
+            const int ns = splits(w.tiles, chunk), length = w.rts ? (w.tiles + ns - 1) / ns : -1;
+            int rank = 0;
+            for (int i = 0; i < a.p.n_seq; i++) {
+                const int other = __builtin_amdgcn_readlane(length, i);
+                rank += other > length || (other == length && i < lane);
+            }
+            const auto to = [&](int & v) { v = __builtin_amdgcn_ds_permute(4 * rank, v); };
+            to(w.r0), to(w.rows), to(w.tile0), to(w.tiles), to(w.rts), to(w.past), to(own);
+        }
     }
 
     // The sequence found, uniform.
@@ -138,7 +152,7 @@ struct Plan {
         const int lane = threadIdx.x & 63;
         base = slot = 0;
         for (int s0 = 0; s0 < a.p.n_seq; s0 += 64) {
-            if (s0) w = seq_work<ROWS>(a, s0 + lane);
+            if (s0) w = seq_work<ROWS>(a, s0 + lane), own = s0 + lane;
             const int ns = splits(w.tiles, chunk), n = w.rts * a.p.Hkv * ns, sum = wave_scan(n);
             const int m = ns > 1 ? n : 0, sum_m = wave_scan(m);
             const uint64_t at = __ballot(base + sum > id);
@@ -146,7 +160,7 @@ struct Plan {
                 lane_at = __builtin_ctzll(at);
                 base += __builtin_amdgcn_readlane(sum - n, lane_at);
                 slot += __builtin_amdgcn_readlane(sum_m - m, lane_at);
-                s = s0 + lane_at;
+                s = FILL ? __builtin_amdgcn_readlane(own, lane_at) : s0 + lane_at;
                 return true;
             }
             base += __builtin_amdgcn_readlane(sum, 63);

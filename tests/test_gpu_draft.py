@@ -273,6 +273,15 @@ def test_attention_of_trees_scales(gops, scale):
         check_tree(case, out, want, bound)
 
 
+@pytest.mark.parametrize("window", [0, 6000])
+@pytest.mark.parametrize("D,G", [(128, 4), (64, 8)])
+def test_attention_of_trees_of_spread_lengths(gops, D, G, window):
+    """Long splits of sequences of very different lengths, one of them without rows."""
+    case = Case(gops, [40, 0, 33, 64, 1, 25, 40], [9000, 50, 300, 15000, 4000, 100, 9000], 8, D, 64, seed=D, extra_rows=1)
+    out, want, bound = run_tree(gops, case, G, random_trees(case.rows, np.random.default_rng(G)), window=window)
+    check_tree(case, out, want, bound)
+
+
 def test_attention_of_a_long_tree(gops):
     """Past 2^16 keys, many splits, a tree over several of them."""
     case = Case(gops, [61], [70001], 1, 128, 256)
