@@ -93,19 +93,22 @@ __device__ __forceinline__ int splits(int tiles, int chunk) { return max(1, (til
 // at most twice as many splits as that.
 // FILL (trees): about the least chunk with which all items are resident at once, if their row tiles are: 61 rows over 65000 keys in 768
 // workgroups and not 704, 167 us instead of 185; trees of 16 sequences 65 instead of 73. Not with more, or sequences that the lanes do not
-// hold: 512 of 8 rows took 518 us and not 400. Then the sequences' order is that of their splits' lengths, longest first: workgroups some 256
-// apart share a CU, and the long ones of one sequence were neighbours there (16 trees over 200 to 30000 keys 213 us, 173 so; over 8191 60 and
-// 58). Not for short splits, which the search for that order would cost 1 us. (Rows in lines keep the splits, and so the roundings, that they had.)
+// hold: 512 of 8 rows took 518 us and not 400. Then the sequences' order is that of their splits' lengths, longest first, and every second
+// 256 workgroups take theirs the other way round: those 256 apart share a CU, where one sequence's long splits had been neighbours (16 trees
+// over 200 to 30000 keys 213 us, 173 in that order, 166 with the turns; 32 of 8 to 16 rows 59, 56 and 52). Not for short splits: looking for
+// the order would cost them 1 us. (Rows in lines keep the splits, and so the roundings, that they had.)
 template <int ROWS, bool FILL>
 struct Plan {
     const AttnArgs & a;
     SeqWork w;  // of sequence s0 + lane
     int chunk, s, base, slot, lane_at, own;  // own: w's sequence
+    bool sorted;                             // by their splits' lengths
 
     __device__ __forceinline__ Plan(const AttnArgs & args) : a(args) {
         const int lane = threadIdx.x & 63;
         w = seq_work<ROWS>(a, lane);
         own = lane;
+        sorted = false;
         chunk = a.min_chunk;
         if (!a.parts) return;  // one split each
         double u = (double) w.rts * w.tiles, n = w.rts;
@@ -129,6 +132,7 @@ struct Plan {
             // (lanes past the sequences have no rows, whichever they go to)
             const int ns = splits(w.tiles, chunk), length = w.rts ? (w.tiles + ns - 1) / ns : -1;
             int rank = 0;
+            sorted = true;
             for (int i = 0; i < a.p.n_seq; i++) {
                 const int other = __builtin_amdgcn_readlane(length, i);
                 rank += other > length || (other == length && i < lane);
@@ -258,12 +262,13 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     __builtin_amdgcn_s_setprio(3);
     Plan<ROWS, TREE> plan(a);
-    if (!plan.find(blockIdx.x)) {
+    const int unit = TREE && plan.sorted && (blockIdx.x & 256) ? blockIdx.x ^ 255 : blockIdx.x;
+    if (!plan.find(unit)) {
         if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = Part{};
         return;
     }
     const SeqWork sw = plan.picked();
-    const int ns = splits(sw.tiles, plan.chunk), chunk = (sw.tiles + ns - 1) / ns, id = blockIdx.x - plan.base;
+    const int ns = splits(sw.tiles, plan.chunk), chunk = (sw.tiles + ns - 1) / ns, id = unit - plan.base;
     const int split = id % ns, rt = sw.rts - 1 - id / ns % sw.rts, hk = id / ns / sw.rts, slot_of = plan.slot + id;
 
     const int rows = sw.rows * a.G, x0 = rt * ROWS, nr = min(ROWS, rows - x0);  // this tile's rows
