@@ -30,6 +30,8 @@
 
 #include <algorithm>
 
+#include "paged_plan.h"
+
 namespace gcq {
 
 namespace {
@@ -41,7 +43,6 @@ typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kMinChunk = 16;    // tiles of a split: four to a wavefront (32 sequences' step: 25.3 us, with 32 tiles 28.6)
 constexpr float kSlack = 4.0f;   // how far a score's exponent may pass R
 constexpr float kBig = 0x1p20f;  // exponents from here on are no longer exact to 2^-4
 constexpr float kP = 11.0f;      // the exponent of P's scale: with kSlack at most 2^15, f16's largest power; parts down to 2^-35 of 2^R
@@ -84,14 +85,14 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs & a, int s) {
     w.rts = (int) (((int64_t) w.rows * a.G + ROWS - 1) / ROWS);
     return w;
 }
-__device__ __forceinline__ int splits(int tiles, int chunk) { return max(1, (tiles + chunk - 1) / chunk); }
 
 // The plan, the same in every wavefront: tiles per split, and a sequence's first item. Items of a sequence: [KV
 // head][row tile, the last, which sees most, first][split]. The batch's arrays are read once where the sequences fit the lanes.
 // Items of split row tiles have a slot each for their sums. Those are fewer than 2 target: with u tiles in all items' and a chunk of more than
 // u / cut, a row tile has less than tiles cut / u splits more than one, all of them together less than cut <= target, and a split row tile has
 // at most twice as many splits as that.
-// FILL (trees): about the least chunk with which all items are resident at once, if their row tiles are: 61 rows over 65000 keys in 768
+// FILL (trees): about the least chunk with which all items are resident at once, if their row tiles are (in eight turns: where row tiles
+// come near to the target, some items may be left over, which run behind the others): 61 rows over 65000 keys in 768
 // workgroups and not 704, 167 us instead of 185; trees of 16 sequences 65 instead of 73. Not with more, or sequences that the lanes do not
 // hold: 512 of 8 rows took 518 us and not 400. Then the sequences' order is that of their splits' lengths, longest first, and every second
 // 256 workgroups take theirs the other way round: those 256 apart share a CU, where one sequence's long splits had been neighbours (16 trees
@@ -121,12 +122,12 @@ struct Plan {
         n = wave_sum_d(n) * a.p.Hkv;
         const bool fill = FILL && a.p.n_seq <= 64 && n < a.target;
         const double cut = fill ? a.target : fmax(a.target - n, 0.5 * a.target);
-        chunk = __builtin_amdgcn_readfirstlane((int) fmax((double) a.min_chunk, fmin(u / cut + 1.0, 1e9)));
+        chunk = __builtin_amdgcn_readfirstlane(plan_chunk(u, cut, a.min_chunk));
         for (int turn = 0; fill && turn < 8; turn++) {
             const int items = w.rts * splits(w.tiles, chunk);
             const double more = (double) a.p.Hkv * __builtin_amdgcn_readlane(wave_scan(items), 63) / a.target;
             if (more <= 1.0) break;  // (all items resident)
-            chunk = __builtin_amdgcn_readfirstlane((int) (chunk * fmin(0.5 + 0.5 * more, 1.5)) + 1);
+            chunk = __builtin_amdgcn_readfirstlane(plan_longer(chunk, more));
         }
         if (fill && a.p.n_seq > 1 && chunk > 32) {
             // (lanes past the sequences have no rows, whichever they go to)
@@ -242,11 +243,6 @@ __device__ __forceinline__ void tile_load(const uint8_t * t, uint32_t lds, int l
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// Wavefronts per SIMD that the registers (and, heads of 256, LDS) hold; and of a workgroup.
-// (Eight wavefronts to a workgroup, heads of 128: 32 sequences' step 32.1 us for 25.3 with four, four prompts 134 for 86; heads of
-// 256 with 32 rows, whose four wavefronts would fill half the LDS: 52.6 us with eight, 80.3 with four.)
-constexpr int per_simd(int D, int RT) { return D * RT <= 128 ? 4 : D * RT == 256 && RT == 2 ? 3 : 2; }
-constexpr int waves(int D, int rows) { return D == 256 && rows == 32 ? 8 : 4; }
 
 // TREE: the rows see the slots below past (a window's part of them) and those new rows that their masks name. Tiles of slots below
 // past alone are any row's; of the others, the last few, a row's 32 keys come as a word of ones shifted into its mask's. (3 to 5 % more than rows in lines take;
@@ -262,7 +258,7 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     __builtin_amdgcn_s_setprio(3);
     Plan<ROWS, TREE> plan(a);
-    const int unit = TREE && plan.sorted && (blockIdx.x & 256) ? blockIdx.x ^ 255 : blockIdx.x;
+    const int unit = unit_of(blockIdx.x, a.items, TREE && plan.sorted);
     if (!plan.find(unit)) {
         if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = Part{};
         return;
@@ -745,7 +741,7 @@ struct Shape {
 Shape shape_of(const Paged & p, int D, int G, int64_t max_rows, int window, int rows) {
     Shape s{};
     s.rows = rows;
-    s.target = 256 * 4 * per_simd(D, rows / 16) / waves(D, rows);
+    s.target = plan_target(D, rows);
     // row tiles: the rows' whole tiles and one more for each sequence
     const int64_t per_seq = std::min<int64_t>(max_rows, p.n_rows) * G;
     s.tiles = p.Hkv * std::min<int64_t>((int64_t) p.n_rows * G / rows + std::min<int64_t>(p.n_seq, p.n_rows),

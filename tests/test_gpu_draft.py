@@ -911,3 +911,33 @@ def test_nothing_to_do(gops):
     assert tree.mask.shape == (0, 1)
     path = gops.draft_verify(b.starts, e, e, torch.zeros(0, 50, device="cuda"), torch.zeros(0, device="cuda"), max_path=3)
     assert path.count.tolist() == [0, 0] and (path.rows == -1).all() and (path.tokens == -1).all()
+
+
+# ------------------------------------------------------------- long splits of several sequences
+
+
+def check_long(gops, D, Hkv, G, rows, past, page=64, window=0):
+    """Trees over long lines, their past drawn on the device."""
+    case = Case(gops, rows, past, Hkv, D, page, seed=D)
+
+    def fill():
+        total = [p + r for p, r in zip(past, rows)]
+        g = torch.Generator(device="cuda").manual_seed(D + sum(past))
+        k, v = (torch.randn((sum(total), Hkv, D), generator=g, device="cuda") for _ in range(2))
+        b = case.batch(total, [0] * len(total))
+        gops.paged_append(case.cache, b, k, v)
+        case.k, case.v = (x.double() for x in gops.paged_read(case.cache, b, sum(total)))
+        case.key0 = np.concatenate([[0], np.cumsum(total)])
+    case.fill_past = fill
+    out, want, bound = run_tree(gops, case, G, random_trees(rows, np.random.default_rng(D)), window=window)
+    assert not (out == 77.0).any()  # every row is written
+    check_tree(case, out, want, bound)
+
+
+@pytest.mark.parametrize("D,Hkv,G,rows,past,window", [
+    (128, 4, 8, [32] * 5, [100000] * 4 + [1000], 0), (256, 8, 4, [32] * 7, [30000] + [200] * 6, 0),
+    (128, 8, 4, [38, 20, 49, 35], [76116, 41908, 31893, 63026], 0), (256, 8, 2, [44, 40, 40, 37, 39], [1057, 44721, 28100, 7659, 16044], 0),
+    (256, 2, 8, [42, 41, 41, 40], [4358, 4528, 4462, 3610], 4096), (256, 2, 8, [34, 22, 17, 23], [9014, 120, 45050, 31239], 20000)])
+def test_attention_of_trees_nearly_as_many_as_fit(gops, D, Hkv, G, rows, past, window):
+    """More workgroups than are resident at once, the last 256 of the grid not all there."""
+    check_long(gops, D, Hkv, G, rows, past, window=window)
