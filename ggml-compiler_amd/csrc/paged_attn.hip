@@ -268,8 +268,10 @@ __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const A
     const int split = id % ns, rt = sw.rts - 1 - id / ns % sw.rts, hk = id / ns / sw.rts, slot_of = plan.slot + id;
 
     const int rows = sw.rows * a.G, x0 = rt * ROWS, nr = min(ROWS, rows - x0);  // this tile's rows
-    if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = {ns, split, nr, hk, sw.r0, x0, slot_of};
-    if (ns > 1 && slot_of >= a.slots) return;  // (arrays that change under the call: no sums outside the workspace)
+    // (by the unit: workgroups with their items in the other order have a row tile's splits in descending order. Starts that do not ascend, or
+    // arrays that change under the call, may have more than there are)
+    if (a.parts && threadIdx.x == 0) a.parts[blockIdx.x] = all_there(unit, split, ns, a.items) ? Part{ns, split, nr, hk, sw.r0, x0, slot_of} : Part{};
+    if (ns > 1 && slot_of >= a.slots) return;  // (no sums outside the workspace)
     // the slots of its first and last row; of a tree, the last slot that any row may see, and the first and last row's positions as
     // far as a window goes
     const int64_t pos0 = TREE ? sw.past : (int64_t) sw.past + x0 / a.G, pos1 = TREE ? (int64_t) sw.past + sw.rows - 1 : (int64_t) sw.past + (x0 + nr - 1) / a.G;
@@ -650,7 +652,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(const AttnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), d = lane % L;
     const Part w = a.parts[blockIdx.x];
     const int ns = __builtin_amdgcn_readfirstlane(w.ns), split = __builtin_amdgcn_readfirstlane(w.split), item = __builtin_amdgcn_readfirstlane(w.slot) - split;
-    if (ns <= 1 || split >= w.nr || (int) blockIdx.x - split + ns > a.items || item < 0 || item + ns > a.slots) return;  // (starts that do not ascend)
+    if (ns <= 1 || split >= w.nr || item < 0 || item + ns > a.slots) return;  // (starts that do not ascend)
     __shared__ f4_t so[N4][L];
     __shared__ float2 sml[N4];
     const auto weight = [](float from, float to) { return from == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(from - to); };

@@ -28,5 +28,7 @@ constexpr int plan_longer(int chunk, double more) { return (int) (chunk * (more 
 // order. The last of the grid's 256s stay as they are if they are not all there: each has an item of its own and none is left over, also
 // where there are more items than are resident at once.
 constexpr int unit_of(int block, int grid, bool turned) { return turned && (block & 256) && (block | 255) < grid ? block ^ 255 : block; }
+// Whether all splits of the row tile whose split `split` of ns is item `unit` are there to be joined.
+constexpr bool all_there(int unit, int split, int ns, int grid) { return unit - split + ns <= grid; }
 
 }  // namespace gcq

@@ -1,5 +1,5 @@
 // The plan of the paged cache's attention of draft trees (csrc/paged_plan.h), over random batches on the host: each workgroup has an item
-// of its own and every item a workgroup. The sequences are a vector here, there a wavefront's lanes.
+// of its own, every item a workgroup, and every row one that writes it. The sequences are a vector here, there a wavefront's lanes.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -111,6 +111,24 @@ void check(const Batch & b) {
         }
         const int missing = (int) std::count_if(runs.begin(), runs.end(), [](int x) { return x != 1; });
         if (missing) report(b, "items not run once", missing, grid);
+        // the splits of a row tile share its rows, row y to split y % ns's workgroup
+        std::vector<std::vector<int>> rows(n);
+        for (int block = 0; block < grid; block++) {
+            const int unit = unit_of(block, grid, p.sorted);
+            if (unit < 0 || unit >= n || !all_there(unit, p.items[unit].split, p.items[unit].ns, grid)) continue;
+            const Item & it = p.items[unit];
+            const int64_t all = (int64_t) b.rows[it.s] * b.G;
+            auto & seen = rows[it.first_unit];
+            seen.resize(std::min<int64_t>(b.tile_rows, all - (int64_t) it.row_tile * b.tile_rows));
+            for (size_t y = it.split; y < seen.size(); y += it.ns) seen[y]++;
+        }
+        int lost = 0;
+        for (const Item & it : p.items)
+            if (it.split == 0) {
+                const auto & seen = rows[it.first_unit];
+                lost += seen.empty() || std::any_of(seen.begin(), seen.end(), [](int x) { return x != 1; });
+            }
+        if (lost) report(b, "row tiles not written once", lost, grid);
     }
 }
 

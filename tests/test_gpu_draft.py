@@ -929,7 +929,7 @@ def check_long(gops, D, Hkv, G, rows, past, page=64, window=0):
         case.k, case.v = (x.double() for x in gops.paged_read(case.cache, b, sum(total)))
         case.key0 = np.concatenate([[0], np.cumsum(total)])
     case.fill_past = fill
-    out, want, bound = run_tree(gops, case, G, random_trees(rows, np.random.default_rng(D)), window=window)
+    out, want, bound = run_tree(gops, case, G, random_trees(rows, np.random.default_rng(D)), window=window, max_rows=max(rows))
     assert not (out == 77.0).any()  # every row is written
     check_tree(case, out, want, bound)
 
@@ -940,4 +940,13 @@ def check_long(gops, D, Hkv, G, rows, past, page=64, window=0):
     (256, 2, 8, [42, 41, 41, 40], [4358, 4528, 4462, 3610], 4096), (256, 2, 8, [34, 22, 17, 23], [9014, 120, 45050, 31239], 20000)])
 def test_attention_of_trees_nearly_as_many_as_fit(gops, D, Hkv, G, rows, past, window):
     """More workgroups than are resident at once, the last 256 of the grid not all there."""
+    check_long(gops, D, Hkv, G, rows, past, window=window)
+
+
+@pytest.mark.parametrize("D,Hkv,G,rows,past,window", [
+    (128, 8, 4, [4, 4], [130000, 5000], 0), (128, 8, 4, [4, 4], [70000, 70000], 0), (256, 8, 4, [4, 4], [36000, 36000], 0),
+    (64, 8, 1, [2, 2, 1], [67121, 68882, 79389], 0), (128, 8, 4, [1, 1], [84693, 96073], 0), (256, 8, 4, [4, 3, 4], [9028, 50329, 40970], 0),
+    (128, 8, 4, [5, 5, 5], [90000, 100000, 110000], 60000)])
+def test_attention_of_few_rows_behind_long_lines(gops, D, Hkv, G, rows, past, window):
+    """More splits to a row tile than there are row tiles, their workgroups in either order."""
     check_long(gops, D, Hkv, G, rows, past, window=window)

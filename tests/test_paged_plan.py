@@ -8,7 +8,7 @@ from pathlib import Path
 ROOT = Path(__file__).resolve().parents[1]
 
 
-def test_every_item_has_a_workgroup(tmp_path):
+def test_every_item_and_row_has_a_workgroup(tmp_path):
     exe = tmp_path / "paged_plan"
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", f"-I{ROOT / 'ggml-compiler_amd' / 'csrc'}",
                     str(ROOT / "tests" / "cpp" / "paged_plan.cpp"), "-o", str(exe)], check=True, capture_output=True, text=True)
