@@ -831,6 +831,7 @@ __global__ __launch_bounds__(kDrawT) void k_verify_draw(const VerifyArgs a) {
         int u = q.u, n = q.n, then = q.then;
         const bool greedy = !(t > 0.0f);
         const double scale = greedy ? 1.0 : scale_of(t);
+        __syncthreads();  // (the roots, which every wavefront's look for the part takes; and the state is read before it changes)
         if (n <= 0 || n > a.max_path || (then == kNone) != of_p) continue;
         if (u < 0 || u >= w.n || w.r0 < 0 || w.r0 > a.n_rows - w.n) return;
         for (bool alone = false;;) {

@@ -950,3 +950,31 @@ def test_attention_of_trees_nearly_as_many_as_fit(gops, D, Hkv, G, rows, past, w
 def test_attention_of_few_rows_behind_long_lines(gops, D, Hkv, G, rows, past, window):
     """More splits to a row tile than there are row tiles, their workgroups in either order."""
     check_long(gops, D, Hkv, G, rows, past, window=window)
+
+
+# ------------------------------------------------------------- draws of many workgroups at once
+
+
+@pytest.mark.parametrize("kids", [0, 2])
+def test_draws_are_the_same_in_every_wavefront(gops, kids):
+    """Flat distributions over many parts, which each wavefront of a draw's workgroup finds for itself: single rows and guesses that
+    fall, more sequences than workgroups that are resident, beside a second stream's."""
+    S, V = 700, 20011
+    rng = np.random.default_rng(kids)
+    rows = [1 + kids] * S
+    parents = ([-1] + [0] * kids) * S
+    tokens = rng.integers(0, V, S * (1 + kids))
+    logits = np.repeat((rng.standard_normal((S, V)) * 0.5).astype(np.float32), 1 + kids, 0)
+    coins = rng.random(len(tokens)).astype(np.float32)
+    a = (parents, tokens, logits, coins)
+    want = reference(rows, *a, max_path=1 + kids)
+    up = [ints(np.concatenate([[0], np.cumsum(rows)])), ints(parents), ints(tokens), torch.from_numpy(logits).cuda(), torch.from_numpy(coins).cuda()]
+    torch.cuda.synchronize()
+    streams, out = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                out.append(gops.draft_verify(*up, max_rows=1 + kids))
+    torch.cuda.synchronize()
+    for path in out:
+        assert (path.count.tolist(), path.rows.tolist(), path.tokens.tolist()) == want
