@@ -135,7 +135,7 @@ struct __align__(16) PartSums {
 };
 struct __align__(16) SeqState {  // a sequence whose path is known
     int u, n, then, r0;            // the path's last row, its rows (0: not known, or ended), what became of it; the sequence's rows
-    int rows, arrived, listed;
+    int rows, arrived, listed;       // listed: it draws from what is left; not changed behind k_verify_rows
     float t;
 };
 struct __align__(16) Item {  // a row in its order
@@ -832,7 +832,10 @@ __global__ __launch_bounds__(kDrawT) void k_verify_draw(const VerifyArgs a) {
         const bool greedy = !(t > 0.0f);
         const double scale = greedy ? 1.0 : scale_of(t);
         __syncthreads();  // (the roots, which every wavefront's look for the part takes; and the state is read before it changes)
-        if (n <= 0 || n > a.max_path || (then == kNone) != of_p) continue;
+        // A listed sequence's state changes in a launch, by the last of its workgroups, after all of them have read it: the first n_seq
+        // workgroups leave those alone, whatever they have read. (What is drawn from p behind a draft that fell is drawn there.)
+        if (of_p ? q.listed || then != kNone : then == kNone) continue;
+        if (n <= 0 || n > a.max_path) continue;
         if (u < 0 || u >= w.n || w.r0 < 0 || w.r0 > a.n_rows - w.n) return;
         for (bool alone = false;;) {
             PartSums early{0.0, 0.0, -INFINITY, -INFINITY, 0, 0};

@@ -978,3 +978,33 @@ def test_draws_are_the_same_in_every_wavefront(gops, kids):
     torch.cuda.synchronize()
     for path in out:
         assert (path.count.tolist(), path.rows.tolist(), path.tokens.tolist()) == want
+
+
+@pytest.mark.parametrize("S,V", [(300, 5003), (40, 40000)])
+def test_paths_that_go_on_behind_fallen_drafts(gops, S, V):
+    """Drawn trees most of whose first children fall and a later one stands, so that paths go on, and end in rows without children, within
+    the launches that draw: the same in every call, on two streams at once."""
+    rng = np.random.default_rng(S)
+    rows = [9] * S
+    parents = [-1, 0, 0, 0, 0, 1, 2, 3, 4] * S  # four children, one more behind each
+    start = 9 * np.repeat(np.arange(S), 9)
+    base = (rng.standard_normal((S, V)) * 0.8).astype(np.float32)
+    logits = np.repeat(base, 9, 0)
+    draft = np.repeat((base + 1.2 * rng.standard_normal((S, V))).astype(np.float32), 9, 0)
+    tokens = np.array([draws(rng, draft[r:r + 1], 1.0)[0] for r in start + np.maximum(parents, 0)])
+    coins = np.where(np.tile(np.arange(9), S) < 3, 0.8 + 0.2 * rng.random(9 * S), 0.2 * rng.random(9 * S)).astype(np.float32)
+    a = (parents, tokens, logits, coins, draft)
+    want = reference(rows, *a, max_path=4)
+    third = sum(r[1] >= 2 for r in want[1])  # behind a draft that fell
+    assert third > S // 5 and sum(c == 3 for c in want[0]) > S // 8
+    up = [ints(np.concatenate([[0], np.cumsum(rows)])), ints(parents), ints(tokens), torch.from_numpy(logits).cuda(), torch.from_numpy(coins).cuda()]
+    more = torch.from_numpy(draft).cuda()
+    torch.cuda.synchronize()
+    streams, out = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                out.append(gops.draft_verify(*up, draft_logits=more, max_rows=9, max_path=4))
+    torch.cuda.synchronize()
+    for path in out:
+        assert (path.count.tolist(), path.rows.tolist(), path.tokens.tolist()) == want
