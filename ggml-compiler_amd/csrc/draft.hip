@@ -336,9 +336,9 @@ __device__ __forceinline__ int child_after(const int32_t * parents, const Rows &
 // through 64 at a time, 10.
 __global__ __launch_bounds__(kT) void k_verify_begin(const VerifyArgs a) {
     const int lane = threadIdx.x & 63, r = blockIdx.x * (kT / 64) + (threadIdx.x >> 6);
-    const int id = blockIdx.x * kT + threadIdx.x, all_ids = gridDim.x * kT;
+    const int64_t id = (int64_t) blockIdx.x * kT + threadIdx.x, all_ids = (int64_t) gridDim.x * kT;  // (64 threads a row: from 2^25 rows on past 31 bits)
     if (id == 0) *a.n_list = 0;
-    for (int s = id; s < a.n_seq; s += all_ids) a.seq[s] = SeqState{}, a.count[s] = 0;
+    for (int64_t s = id; s < a.n_seq; s += all_ids) a.seq[s] = SeqState{}, a.count[s] = 0;
     for (int64_t i = id; i < (int64_t) a.n_seq * a.max_path; i += all_ids) a.rows[i] = a.out[i] = -1;
     if (r >= a.n_rows) return;
     if (lane == 0) a.next[r] = kOpen, a.arrived[(int64_t) r * kApart] = 0;

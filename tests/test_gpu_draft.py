@@ -1008,3 +1008,17 @@ def test_paths_that_go_on_behind_fallen_drafts(gops, S, V):
     torch.cuda.synchronize()
     for path in out:
         assert (path.count.tolist(), path.rows.tolist(), path.tokens.tolist()) == want
+
+
+def test_verify_more_rows_than_threads_of_31_bits(gops):
+    """A few trees before 2^25 rows of none: 64 threads a row pass 2^31."""
+    rows, V, n = [3, 1, 0, 6] * 20, 5, (1 << 25) + 9
+    a = make_verify(rows, V, False, 2, seed=6)
+    up = []
+    for x, dtype in ((a[0], torch.int32), (a[1], torch.int32), (a[2], torch.float32), (a[3], torch.float32)):
+        x = torch.tensor(np.asarray(x), dtype=dtype, device="cuda")
+        y = torch.zeros((n, *x.shape[1:]), dtype=dtype, device="cuda")
+        y[:len(x)] = x
+        up.append(y)
+    path = gops.draft_verify(ints(np.concatenate([[0], np.cumsum(rows)])), *up, temperature=torch.from_numpy(a[5]).cuda(), max_rows=6, max_path=4)
+    assert (path.count.tolist(), path.rows.tolist(), path.tokens.tolist()) == reference(rows, *a, max_path=4)
