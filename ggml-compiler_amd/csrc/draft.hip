@@ -1088,7 +1088,10 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         a.next = (int *) (at + z.next), a.arrived = (int *) (at + z.arrived), a.sums = (PartSums *) (at + z.sums), a.seq = (SeqState *) (at + z.seq);
         a.list = (int *) (at + z.list), a.drawn = (double *) (at + z.drawn), a.drawn_runs = (double *) (at + z.drawn_runs);
         hipStream_t st = as_stream(stream);
-        k_verify_begin<<<paged_grid(std::max<int64_t>((n_rows + 3) / 4, 1), kT), kT, 0, st>>>(a);
+        // (what cannot be launched is refused before the first one)
+        const unsigned begin_groups = paged_grid(std::max<int64_t>((n_rows + 3) / 4, 1), kT);
+        const unsigned draw_groups = n_rows == 0 ? 0 : paged_grid(n_seq + (draft_logits ? std::min<int64_t>((int64_t) n_seq * z.blocks, 2 * kRowGroups) : 0), kDrawT);
+        k_verify_begin<<<begin_groups, kT, 0, st>>>(a);
         check_launch("draft verify");
         if (n_rows == 0) return;
         a.blocks = z.blocks, a.block_steps = z.block_steps;
@@ -1101,8 +1104,7 @@ int gcq_draft_verify(const int32_t * starts, int n_seq, int64_t n_rows, const in
         const int draws = draft_logits && max_path < a.max_rows && z.blocks > 8 ? (n_seq < 8 ? 3 : 5) : 1;
         for (int i = 0; i < draws; i++) {
             a.last = i == draws - 1;
-            const int64_t groups = n_seq + (draft_logits ? std::min<int64_t>((int64_t) n_seq * z.blocks, 2 * kRowGroups) : 0);
-            k_verify_draw<<<paged_grid(groups, kDrawT), kDrawT, 0, st>>>(a);
+            k_verify_draw<<<draw_groups, kDrawT, 0, st>>>(a);
             check_launch("draft verify draw");
         }
     });

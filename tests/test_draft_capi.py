@@ -141,3 +141,10 @@ def test_python_refusals_without_a_device():
     i = torch.zeros(4, dtype=torch.int32)
     with pytest.raises(ValueError, match="device tensor"):
         ops.DraftTree(i, i, i.view(4, 1))
+
+
+def test_verify_refuses_what_cannot_be_launched():
+    """Before anything is: the draws' workgroups, one to a sequence at the least, are counted first."""
+    _refused(_verify(n_seq=1 << 23), "too many rows")
+    _refused(_verify(n_seq=1 << 23, draft_logits=None), "too many rows")
+    _refused(_verify(n_rows=1 << 26, max_rows=5), "too many rows")
