@@ -211,13 +211,15 @@ __device__ __forceinline__ Range range_of(float m, double scale) {
     const bool odd = !(fabsf(m) < 1e38f) || !(x > -32600.0 && x < -31400.0);  // (root's powers end at 2^-1022)
     return {z.low, odd ? -INFINITY : z.high};
 }
+// A NaN as one that maxima and medians pass over (a signalling one comes out of them).
+__device__ __forceinline__ float quiet(float l) { return __builtin_canonicalizef(l); }
 // The weights of four logits in that range (two, then two: more at a time than the registers hold).
 __device__ __forceinline__ void weigh4(const double * roots, double scale, double m, float low, const float (&l)[4], double (&v)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
 #pragma unroll
         for (int i = e; i < e + 2; i++) {
-            const double d = (double) __builtin_amdgcn_fmed3f(l[i], low, kHuge) - m, t = fma(d, scale, 0x1.8p52), r = fma(d, scale, 0x1.8p52 - t);
+            const double d = (double) __builtin_amdgcn_fmed3f(quiet(l[i]), low, kHuge) - m, t = fma(d, scale, 0x1.8p52), r = fma(d, scale, 0x1.8p52 - t);
             v[i] = power(r) * root(roots, (int) (uint32_t) __double_as_longlong(t));
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -240,9 +242,7 @@ struct Running {
     }
     // in: m's, at first {0, -inf}
     __device__ __forceinline__ void take4(const double * roots, double scale, Range & in, const float (&l)[4]) {
-        // (the largest, NaNs passed over, as medians with infinity: fmaxf quiets its operands first, twice the operations)
-        const auto larger = [](float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); };
-        const float top = larger(larger(l[0], l[1]), larger(l[2], l[3]));
+        const float top = fmaxf(fmaxf(quiet(l[0]), quiet(l[1])), fmaxf(quiet(l[2]), quiet(l[3])));  // (NaNs passed over)
         if (__any(top > in.high)) {
             if (m == -INFINITY && top > -INFINITY) {
                 m = fminf(top, kHuge), s = 0.0;

@@ -1022,3 +1022,25 @@ def test_verify_more_rows_than_threads_of_31_bits(gops):
         up.append(y)
     path = gops.draft_verify(ints(np.concatenate([[0], np.cumsum(rows)])), *up, temperature=torch.from_numpy(a[5]).cuda(), max_rows=6, max_path=4)
     assert (path.count.tolist(), path.rows.tolist(), path.tokens.tolist()) == reference(rows, *a, max_path=4)
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("bits", [0x7fc00000, 0x7f800001, 0xff812345], ids=["quiet", "signalling", "signalling-payload"])
+def test_verify_nans_beside_each_other(gops, bits, drawn):
+    """NaNs of either kind in one, two, three and four of the columns that a thread has at a time, from the first ones to a row's last, of
+    the target's rows and the drafter's: as -inf."""
+    rng = np.random.default_rng(bits & 0xff)
+    V, rows = 5001, [3] * 32
+    parents, tokens, logits, coins, draft, t = make_verify(rows, V, True, 1, seed=31)
+    nan = np.array([bits], np.uint32).view(np.float32)[0]
+
+    def spoil(x):
+        y = x.view(np.uint32)
+        for r in range(len(x)):
+            for at in [0, 4 * int(rng.integers(1, 900)), 4092, 5000 // 4 * 4 - 4]:
+                cols = rng.permutation(4)[:1 + (r + at // 4) % 4]
+                y[r, at + cols] = bits
+        return x
+    a = (parents, tokens, spoil(logits), coins, spoil(draft) if drawn else None, t)
+    assert np.isnan(nan) and np.isnan(logits).sum() > 3 * len(logits)
+    assert verify(gops, rows, *a, max_path=3) == reference(rows, *a, max_path=3)
