@@ -1119,8 +1119,8 @@ int gcq_paged_move(const gcq_paged_cache * const * caches, int n_caches, const g
         paged_need(rows, "rows", 4);
         paged_require(max_keep >= 0 && ld_rows >= max_keep, "paged_move: ld_rows >= max_keep >= 0");
         for (int c0 = 0; c0 < n_caches; c0++) {
-            const Paged p = paged_view(caches[c0], batch, 1);
-            (void) p;
+            paged_view(caches[c0], batch, 1, false);
+            paged_need(caches[c0]->data, "cache data", 16);
             paged_require(caches[c0]->n_pages == caches[0]->n_pages && caches[c0]->page_size == caches[0]->page_size &&
                               caches[c0]->n_head_kv == caches[0]->n_head_kv && caches[c0]->head_dim == caches[0]->head_dim,
                           "paged_move: the caches must be of one shape");
@@ -1130,9 +1130,11 @@ int gcq_paged_move(const gcq_paged_cache * const * caches, int n_caches, const g
         std::transform(caches, caches + n_caches, at.begin(), [](const gcq_paged_cache * c) { return (uintptr_t) c->data; });
         std::sort(at.begin(), at.end());
         for (int i = 1; i < n_caches; i++) paged_require(at[i] - at[i - 1] >= size, "paged_move: caches overlap (a row would move twice)");
+        paged_need(batch->pages, "pages", 4);
+        paged_need(batch->past, "past", 4);
         if (max_keep == 0) return;
         MoveArgs a{};
-        a.p = paged_view(caches[0], batch, 1);
+        a.p = paged_view(caches[0], batch, 1, false);  // (no starts)
         a.count = count, a.rows = rows, a.ld = ld_rows, a.max_keep = max_keep;
         for (int c0 = 0; c0 < n_caches; c0 += kCaches) {
             const int n = std::min(n_caches - c0, kCaches);

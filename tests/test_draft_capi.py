@@ -148,3 +148,13 @@ def test_verify_refuses_what_cannot_be_launched():
     _refused(_verify(n_seq=1 << 23), "too many rows")
     _refused(_verify(n_seq=1 << 23, draft_logits=None), "too many rows")
     _refused(_verify(n_rows=1 << 26, max_rows=5), "too many rows")
+
+
+def test_move_reads_pages_and_past_alone():
+    """A batch without starts, or with any, is moved; pages and past are looked at."""
+    assert _move(None, _batch(starts=None), max_keep=0) == 0
+    assert _move(None, _batch(starts=P + 2), max_keep=0) == 0
+    _refused(_move(None, _batch(starts=None, past=None)), "past is NULL")
+    _refused(_move(None, _batch(past=P + 1)), "past must be 4-byte aligned")
+    _refused(_move(None, _batch(pages=P + 2)), "pages must be 4-byte aligned")
+    _refused(_move([_cache(data=P + 8)]), "cache data must be 16-byte aligned")

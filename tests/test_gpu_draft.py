@@ -1044,3 +1044,21 @@ def test_verify_nans_beside_each_other(gops, bits, drawn):
     a = (parents, tokens, spoil(logits), coins, spoil(draft) if drawn else None, t)
     assert np.isnan(nan) and np.isnan(logits).sum() > 3 * len(logits)
     assert verify(gops, rows, *a, max_path=3) == reference(rows, *a, max_path=3)
+
+
+def test_move_without_starts(gops):
+    """Through the C call: a batch whose starts are NULL."""
+    import ctypes
+
+    from ggml_compiler_amd import _lib
+    case = Case(gops, [9], [30], 1, 64, 32)
+    cache = gops.PagedCache(case.n_pages, 32, 1, 64, torch.randint(0, 256, (case.cache.data.numel(),), dtype=torch.uint8, device="cuda"))
+    batch, count, rows, want = case.batch(), ints([2]), ints([[0, 8]]), cache.data.clone()
+    b = type(batch._c).from_buffer_copy(batch._c)
+    b.starts = None
+    at = (ctypes.c_void_p * 1)(cache._at)
+    _lib.check(_lib.load().gcq_paged_move(at, 1, ctypes.addressof(b), count.data_ptr(), rows.data_ptr(), 2, 2,
+                                          torch.cuda.current_stream().cuda_stream))
+    x, y = (torch.from_numpy(layout_bytes(case, [(0, p)])).cuda().flatten() for p in (38, 31))
+    want[y] = want[x]
+    assert torch.equal(cache.data, want)
