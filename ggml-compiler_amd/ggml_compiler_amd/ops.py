@@ -509,7 +509,8 @@ def draft_verify(starts: torch.Tensor, parents: torch.Tensor, tokens: torch.Tens
     """Which drafts stand against the target, and the token after them (gcq_draft_verify): sequence s owns rows starts[s] ..
     starts[s + 1] - 1 (int32 [S + 1]), trees by parents (int32 [n]). tokens int32 [n]; logits f32 [n, V], the target's for
     what follows each row; coins f32 [n], uniform of [0, 1); draft_logits f32 [n, V]: a row's children were drawn from their
-    softmax (None: guesses that were not drawn); temperature f32 [S] (None: 1; 0: the largest logit). Rows of logits may be
+    softmax (None: guesses that were not drawn); temperature f32 [S] (None: 1; 0: the largest logit). Rows that fill a tree up have
+    parent -1; a child whose token is none falls as if it had been drawn, which biases what follows. Rows of logits may be
     strided, unit inner stride. max_rows: no sequence has more rows than this (default n, at most 1024); max_path: a
     path's rows at most (default max_rows; for trees their depth and one: shorter results, and with draft_logits the sums of what
     fallen drafts leave take the whole device where it is less than max_rows). out: into these."""

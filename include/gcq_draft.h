@@ -62,7 +62,9 @@ GCQ_API size_t gcq_draft_verify_workspace(int n_seq, int64_t n_rows, int64_t n_v
  * whose cumulative sum is above coin times the sum. Temperature 0 (or less, or a NaN): a child stands if it is the
  * target's largest logit (the lowest of equals), which is the next token where none does. All in 64 bits from the f32
  * logits on. A logit that is a NaN counts as -inf (never drawn), +inf as the largest float; where a row's logits are all
- * -inf nothing follows: the token is -1. A draft outside [0, n_vocab) falls. (Where rounding leaves r nothing, it is p.)
+ * -inf nothing follows: the token is -1. A draft outside [0, n_vocab) falls, with draft_logits as a draw from q does that fell; it
+ * was none, and what follows it is not distributed as the target: rows that fill a tree up to a fixed size have no parent
+ * (-1) instead, and are not looked at, whatever else they hold. (Where rounding leaves r nothing, it is p.)
  * Results, ints, for sequence s: count[s], the rows that stand, the root among them (0: no rows); rows [n_seq][max_path] their
  * numbers within the sequence, -1 from count on; tokens_out [n_seq][max_path] the token that follows each: the next row's, for
  * the last one the drawn one. A path ends after max_path rows. Rows past max_rows of a sequence are not looked at. ws:

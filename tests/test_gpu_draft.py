@@ -1062,3 +1062,51 @@ def test_move_without_starts(gops):
     x, y = (torch.from_numpy(layout_bytes(case, [(0, p)])).cuda().flatten() for p in (38, 31))
     want[y] = want[x]
     assert torch.equal(cache.data, want)
+
+
+@pytest.mark.parametrize("drawn,kids,V,t,pad", [(True, 1, 5, 1.0, 0), (True, 1, 37, 0.7, 0), (True, 2, 6, 1.0, 0), (True, 2, 5, 1.6, 3), (False, 1, 11, 1.0, 2),
+                                                (False, 2, 6, 0.8, 0)])
+def test_tokens_are_distributed_as_the_target_sharply(gops, drawn, kids, V, t, pad):
+    """The token after the root, over all drafts by their probabilities, is p to 1 / 512. Each child's chance to stand is measured by G coins
+    of its own with those before it fallen, and the chances of the tokens that are drawn by G coins of the root's with all fallen. A border is
+    off by half a step: a draft's 1 / 2G, a token's two 1 / G, products of probabilities by their sum at most. pad: rows without a parent behind the
+    tree, whose tokens are none and whose logits are NaN, change nothing."""
+    G = 1024
+    rng = np.random.default_rng(V)
+    x, y = rng.standard_normal(V).astype(np.float32) * 1.5, rng.standard_normal(V).astype(np.float32) * 1.5
+    p, q = (np.exp(z.astype(np.float64) / t) for z in (x, y))
+    p, q = p / p.sum(), q / q.sum()
+    rows = 1 + kids + pad
+    spoilt = [np.nan] * V
+    logits, draft = (torch.tensor([z.tolist()] * (1 + kids) + [spoilt] * pad, dtype=torch.float32, device="cuda").repeat(G, 1) for z in (x, y))
+    starts, parents = ints(rows * np.arange(G + 1)), ints([-1] + [0] * kids + [-1] * pad).repeat(G)
+    grid, fallen = ((np.arange(G) + 0.5) / G).astype(np.float32), np.float32(1 - 2.0 ** -24)
+
+    def sweep(drafts, which):
+        """The child that stood (0: none) and the token, for G coins of row `which`."""
+        coins = np.full((G, rows), fallen, np.float32)
+        coins[:, which] = grid
+        path = gops.draft_verify(starts, parents, ints([0, *drafts] + [-1] * pad).repeat(G), logits, torch.from_numpy(coins.reshape(-1)).cuda(),
+                                 draft_logits=draft if drawn else None, temperature=torch.full((G,), t, device="cuda"), max_rows=rows, max_path=2)
+        assert (path.count == (path.rows[:, 1] >= 0) + 1).all()
+        return path.rows[:, 1].clamp(min=0).cpu().numpy(), path.tokens[:, 0].cpu().numpy()
+
+    sets = [(c,) for c in range(V)] if kids == 1 else [(c, d) for c in range(V) for d in range(V)]
+    weight = [math.prod(q[c] for c in cs) for cs in sets]
+    if not drawn:
+        sets, weight = [tuple(int(c) for c in rng.permutation(V)[:kids])], [1.0]
+    got = np.zeros(V)
+    for cs, w in zip(sets, weight):
+        for i, c in enumerate(cs):
+            child, token = sweep(cs, 1 + i)
+            stands = child == 1 + i
+            assert (token[stands] == c).all() and (child >= 1 + i).sum() + (child == 0).sum() == G
+            got[c] += w * stands.mean()
+            w *= 1 - stands.mean()
+            if w == 0:  # it stands whatever its coin
+                break
+        else:
+            child, token = sweep(cs, 0)
+            assert (child == 0).all()
+            got += w * np.bincount(token, minlength=V) / G
+    assert np.abs(got - p).max() <= (kids / 2 + 1) / G + 1e-9
