@@ -647,7 +647,7 @@ __device__ __forceinline__ int draw(const VerifyArgs & a, const Source & z, Draw
 // A workgroup has one part of every abreast-th row: those in work at a time are the next of the order that are not cut off. Four wavefronts
 // read; the fifth meets them once for a part: it has then looked up the next row and this one's children, and shares the part's sums and,
 // its row's last, decides while they read that. Bound by HBM, arithmetic in 64 bits and, at the end, what one row's decision takes (6 us): 64 chains of 128256 tokens, 149 MB,
-// 55 us (47 without the fifth's work, 42 without arithmetic); 16 trees, where decisions follow each other, 73 MB, 38 us; one chain 10.
+// 55 us (47 without the fifth's work, 42 without arithmetic); 16 trees, where decisions follow each other, 73 MB, 37 us; one chain 10.
 __global__ __launch_bounds__(kT + 64, 4) void k_verify_rows(const VerifyArgs a) {
     struct Met {
         Running p[kT / 64], q[kT / 64];
@@ -908,7 +908,9 @@ VerifyShape verify_shape(int n_seq, int64_t n_rows, int64_t V) {
     const auto parts = [&](int steps) { return (V + steps * kStep - 1) / (steps * kStep); };
     // A part costs its steps and some four more; workgroups take theirs in as many turns. Of up to 8 steps: decisions come early enough to
     // spare rows (128256 tokens, 205 rows in 64 chains: 91 us, 92 with up to 16; 800 rows in 16 trees: 66 and 83). Of up to 6 where sequences
-    // have many rows, most of which no path comes to (those trees: 59 and, with 4, 62; 128 chains of 8 rows 103, and 92 with 8).
+    // have many rows, most of which no path comes to (those trees 59, with 4 62). With 6 and with 8: drawn trees, 32 of 18 to 24 rows 138 us and 151, 16
+    // of 24 to 32 114 and 118, 16 of 38 to 50 161 and 176; guesses 73 and 75, 57 and 59, 61 and 62, but 64 of 38 to 50 rows 104 and 101. Below 16 rows a
+    // sequence: 128 chains of 6 to 8 rows 240 and 244, over 32000 tokens 107 and 96; 64 trees of 6 to 8 rows over those 43 and 40; drawn ones of 12 to 16 188 and 183.
     int64_t best = INT64_MAX;
     for (int k = 2; k <= (n_rows >= 16 * (int64_t) n_seq ? 6 : kSteps); k += 2) {
         const int64_t cost = (n_rows * parts(k) + kRowGroups - 1) / kRowGroups * (k + 4);

@@ -246,7 +246,7 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 
 // TREE: the rows see the slots below past (a window's part of them) and those new rows that their masks name. Tiles of slots below
 // past alone are any row's; of the others, the last few, a row's 32 keys come as a word of ones shifted into its mask's. (3 to 5 % more than rows in lines take;
-// a tree of 61 rows over 65000 keys 160 us, 16 of 20 to 40 over 200 to 8191 58.)
+// a tree of 61 rows over 65000 keys 163 us, 16 of 20 to 40 over 200 to 8191 58.)
 template <int D, int RT, int NW, bool TREE>
 __global__ __launch_bounds__(64 * NW, per_simd(D, RT)) void k_paged_attn(const AttnArgs a) {
     constexpr int ROWS = 16 * RT, NB = D / 32, NT = D / 16, RING = 2, NL = kTileLoads<D>, P = D + 4;

@@ -61,7 +61,7 @@ GCQ_API size_t gcq_draft_verify_workspace(int n_seq, int64_t n_rows, int64_t n_v
  * The first child that stands is the next row; where none does, the next token is drawn from r with row 0's coin: the lowest token
  * whose cumulative sum is above coin times the sum. Temperature 0 (or less, or a NaN): a child stands if it is the
  * target's largest logit (the lowest of equals), which is the next token where none does. All in 64 bits from the f32
- * logits on. A logit that is a NaN counts as -inf (never drawn), +inf as the largest float; where a row's logits are all
+ * logits on, the exponentials to 2^-43 of themselves. A logit that is a NaN counts as -inf (never drawn), +inf as the largest float; where a row's logits are all
  * -inf nothing follows: the token is -1. A draft outside [0, n_vocab) falls, with draft_logits as a draw from q does that fell; it
  * was none, and what follows it is not distributed as the target: rows that fill a tree up to a fixed size have no parent
  * (-1) instead, and are not looked at, whatever else they hold. (Where rounding leaves r nothing, it is p.)
