@@ -1,5 +1,6 @@
 // The plan of the paged cache's attention of draft trees (csrc/paged_plan.h), over random batches on the host: each workgroup has an item
-// of its own, every item a workgroup, and every row one that writes it. The sequences are a vector here, there a wavefront's lanes.
+// of its own, every item a workgroup, and every row one that writes it; the
+// workspace holds the sums of split row tiles. The sequences are a vector here, there a wavefront's lanes.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -98,6 +99,8 @@ void check(const Batch & b) {
     const int n = (int) p.items.size();
     sorted += p.sorted, over += p.sorted && n > p.target;
     if (n > p.grid) report(b, "items past the grid", n - p.grid, p.grid);
+    const int sums = (int) std::count_if(p.items.begin(), p.items.end(), [](const Item & it) { return it.ns > 1; });
+    if (sums > std::min(p.grid, 2 * p.target)) report(b, "sums past the workspace", sums, p.grid);
     // (any grid that holds the items will do)
     std::vector<int> grids{p.grid, n};
     for (int more : {1, 77, 256, 300}) grids.push_back(n + more);
